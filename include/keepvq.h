@@ -451,6 +451,90 @@ int keepvq_grouped_projection_bytes(const keepvq_grouped_projection_args* args, 
 int keepvq_grouped_projection_bytes_served(int64_t routes, int64_t slots, int64_t out_dim, int64_t in_dim, int64_t groups);
 
 /* ------------------------------------------------------------------------------------------
+ * Products over 16-bit experts, and their gradients: what the quantised operators above are for
+ * E8P codes, for experts (or single projections) that stay in fp16 / bf16, as
+ * HighPrecisionSwitchLinear keeps them (src/ramp/nn/).  Route r goes to expert e = indices[r] and
+ * reads activation row r / x_div (x_div = top_k: token layout; 1: a row per route).
+ *
+ *   keepvq_switch_matmul        out[r] = W[e] x[r / x_div]
+ *   keepvq_switch_matmul_grads  dx[t] = sum over the routes of row t of W[e]^T grad[r]
+ *                               dweight[e] = sum over the routes of expert e of grad[r] x[r / x_div]^T
+ *
+ * An index outside [0, experts) is a dead route: its output row is zero and it adds nothing to a
+ * gradient; experts without routes get zero gradients.  All sums are held in fp32 and rounded once;
+ * an expert's routes are added up in their order, so a call gives the same bits every time.  Rows
+ * are dense, in_dim is a multiple of 8, pointers are aligned to 16 bytes; a row of `grad` is
+ * grad_ld >= out_dim values long, a multiple of 8, and those behind out_dim are zero.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct keepvq_switch_matmul_args {
+  const void* x;          /* [routes / x_div, in_dim] */
+  const void* weight;     /* [experts, out_dim, in_dim] */
+  const void* grad;       /* [routes, grad_ld], the gradient of `out` (grads only) */
+  int32_t dtype;          /* keepvq_dtype of every matrix here: fp16 or bf16 */
+  const void* indices;    /* [routes] */
+  int32_t index_bits;     /* 32 or 64, signed */
+  int32_t x_div;
+  int64_t routes;
+  int64_t experts, out_dim, in_dim;
+  int64_t grad_ld;
+  void* out;              /* [routes, out_dim] (forward only) */
+  void* dx;               /* [routes / x_div, in_dim], or NULL: not wanted (grads only) */
+  void* dweight;          /* [experts, out_dim, in_dim], or NULL: not wanted (grads only) */
+  void* workspace;        /* keepvq_switch_matmul_workspace_bytes(), 256-byte aligned */
+  int64_t workspace_bytes;
+} keepvq_switch_matmul_args;
+
+/* `grads` 0: scratch of keepvq_switch_matmul; 1: of keepvq_switch_matmul_grads. */
+int64_t keepvq_switch_matmul_workspace_bytes(int64_t routes, int64_t experts, int64_t out_dim, int64_t in_dim, int32_t x_div, int32_t grads);
+int keepvq_switch_matmul(const keepvq_switch_matmul_args* args, void* stream);
+int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
+ * Low-rank products chosen per route, added onto a base, and their gradients: adapters of many
+ * requests beside one projection, or a correction per expert of a routed layer.  With
+ * B = left[e], A = right[e], e = indices[r]:
+ *
+ *   keepvq_switch_low_rank        out[r] = base[r] + scale * B (A x[r / x_div])
+ *   keepvq_switch_low_rank_grads  q = scale * B^T grad[r]:   dx[t] = sum over the routes of row t of A^T q
+ *                                 dleft[e] = scale * sum over e's routes of grad[r] (A x)^T
+ *                                 dright[e] = sum over e's routes of q x^T
+ *
+ * A dead route (see above) leaves out[r] = base[r].  The inner vectors A x and q are sums in fp32
+ * and enter the second product as the sum of two 16-bit values (16 bits of them, 22 for fp16),
+ * scaled by a power of two per row so that fp16 neither overflows nor loses small ones.  out and
+ * base have the type out_dtype: the activations', or fp32.  base may be out.  rank is a multiple
+ * of 8 up to 128; in_dim and pointers as above, grad as above.
+ * ------------------------------------------------------------------------------------------ */
+typedef struct keepvq_switch_low_rank_args {
+  const void* x;          /* [routes / x_div, in_dim] */
+  const void* left;       /* [sets, out_dim, rank] */
+  const void* right;      /* [sets, rank, in_dim] */
+  const void* grad;       /* [routes, grad_ld] (grads only) */
+  int32_t dtype;          /* of x, left, right, grad and the gradients: fp16 or bf16 */
+  const void* indices;    /* [routes] */
+  int32_t index_bits;     /* 32 or 64, signed */
+  int32_t x_div;
+  int64_t routes;
+  int64_t sets, out_dim, in_dim, rank;
+  int64_t grad_ld;
+  float scale;
+  int32_t out_dtype;
+  const void* base;       /* [routes, base_ld] or NULL (forward only) */
+  int64_t base_ld;
+  void* out;              /* [routes, out_ld] (forward only) */
+  int64_t out_ld;
+  void* dx;               /* [routes / x_div, in_dim] or NULL (grads only) */
+  void* dleft;            /* [sets, out_dim, rank] or NULL (grads only) */
+  void* dright;           /* [sets, rank, in_dim] or NULL (grads only) */
+  void* workspace;        /* keepvq_switch_low_rank_workspace_bytes(), 256-byte aligned */
+  int64_t workspace_bytes;
+} keepvq_switch_low_rank_args;
+
+int64_t keepvq_switch_low_rank_workspace_bytes(int64_t routes, int64_t sets, int64_t out_dim, int64_t in_dim, int64_t rank, int32_t x_div, int32_t grads);
+int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream);
+int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Expert parallelism: packing routes for the dispatch all-to-all and summing them after the
  * combine all-to-all.
  *

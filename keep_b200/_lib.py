@@ -138,6 +138,24 @@ class EpCombineArgs(Structure):
     ]
 
 
+class SwitchMatmulArgs(Structure):
+    _fields_ = [
+        ("x", c_void_p), ("weight", c_void_p), ("grad", c_void_p), ("dtype", c_int32), ("indices", c_void_p), ("index_bits", c_int32),
+        ("x_div", c_int32), ("routes", c_int64), ("experts", c_int64), ("out_dim", c_int64), ("in_dim", c_int64), ("grad_ld", c_int64),
+        ("out", c_void_p), ("dx", c_void_p), ("dweight", c_void_p), ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
+class SwitchLowRankArgs(Structure):
+    _fields_ = [
+        ("x", c_void_p), ("left", c_void_p), ("right", c_void_p), ("grad", c_void_p), ("dtype", c_int32), ("indices", c_void_p),
+        ("index_bits", c_int32), ("x_div", c_int32), ("routes", c_int64), ("sets", c_int64), ("out_dim", c_int64), ("in_dim", c_int64),
+        ("rank", c_int64), ("grad_ld", c_int64), ("scale", c_float), ("out_dtype", c_int32), ("base", c_void_p), ("base_ld", c_int64),
+        ("out", c_void_p), ("out_ld", c_int64), ("dx", c_void_p), ("dleft", c_void_p), ("dright", c_void_p),
+        ("workspace", c_void_p), ("workspace_bytes", c_int64),
+    ]
+
+
 SCORE_FUNCS = {"softmax": 0, "sigmoid": 1, "sqrtsoftplus": 2}
 STATIC_SCRATCH_BYTES = 8 << 20  # KEEPVQ_STATIC_SCRATCH_BYTES
 STAGE_ROUTER, STAGE_PREPARE, STAGE_GATE_UP, STAGE_DOWN, STAGE_COMBINE, STAGE_ALL = 1, 2, 4, 8, 16, 31
@@ -147,6 +165,7 @@ EXTRA_STRUCTS = {
     "keepvq_router_logits_args": RouterLogitsArgs, "keepvq_routed_topk_args": RoutedTopkArgs,
     "keepvq_expert_weights": ExpertWeights, "keepvq_moe_layer_args": MoELayerArgs,
     "keepvq_residency_args": ResidencyArgs, "keepvq_grouped_projection_args": GroupedProjectionArgs, "keepvq_ep_pack_args": EpPackArgs, "keepvq_ep_peer_args": EpPeerArgs, "keepvq_ep_combine_args": EpCombineArgs,
+    "keepvq_switch_matmul_args": SwitchMatmulArgs, "keepvq_switch_low_rank_args": SwitchLowRankArgs,
 }
 
 _SIGNATURES = {
@@ -175,6 +194,12 @@ _SIGNATURES = {
     "keepvq_wait_selftest_workspace_bytes": (c_int64, []),
     "keepvq_wait_selftest": (c_int, [c_void_p, c_int64, c_int64, c_void_p]),
     "keepvq_grid_wait_selftest": (c_int, [POINTER(MoELayerArgs), c_int32, c_int32, c_int32, c_int64, ctypes.c_uint64, c_void_p]),
+    "keepvq_switch_matmul_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int32, c_int32]),
+    "keepvq_switch_matmul": (c_int, [POINTER(SwitchMatmulArgs), c_void_p]),
+    "keepvq_switch_matmul_grads": (c_int, [POINTER(SwitchMatmulArgs), c_void_p]),
+    "keepvq_switch_low_rank_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_int32]),
+    "keepvq_switch_low_rank": (c_int, [POINTER(SwitchLowRankArgs), c_void_p]),
+    "keepvq_switch_low_rank_grads": (c_int, [POINTER(SwitchLowRankArgs), c_void_p]),
     "keepvq_ep_pack": (c_int, [POINTER(EpPackArgs), c_void_p]),
     "keepvq_ep_combine": (c_int, [POINTER(EpCombineArgs), c_void_p]),
     "keepvq_ep_dispatch_peer": (c_int, [POINTER(EpPackArgs), POINTER(EpPeerArgs), c_void_p]),
@@ -259,6 +284,8 @@ def _by_field(args, values):
 pack_layer_args = packer(MoELayerArgs)
 pack_grouped_args = packer(GroupedProjectionArgs)
 pack_matvec_args = packer(MatvecArgs)
+pack_switch_matmul_args = packer(SwitchMatmulArgs)
+pack_switch_low_rank_args = packer(SwitchLowRankArgs)
 _SAME_DEVICE = contextlib.nullcontext()
 
 

@@ -1,0 +1,160 @@
+"""Products over 16-bit experts chosen per route, and their gradients.
+
+The counterpart of ``vq_switch`` for experts (or single projections of a layer) that stay in fp16 or
+bf16, as the reference's ``HighPrecisionSwitchLinear`` (``src/ramp/nn/``) keeps them:
+
+* ``switch_matmul(x, weight, indices)``         ``out[r] = W[e] x[row(r)]``
+* ``switch_matmul_grads(grad, x, weight, indices)``  the gradients of ``x`` and ``weight``
+
+``x`` leading shape equals ``indices.shape[:-1]`` (token layout: result ``[..., k, out]``) or
+``indices.shape`` (a row per route: result ``[..., out]``), as in ``vq_switch_qmv``.  ``weight`` is
+``[experts, out, in]`` in x's dtype, ``in`` a multiple of 8.  Routes may come in any order; an index outside
+``[0, experts)`` is a dead route: zeros, and no part of any gradient.  Sums are fp32 with one rounding, in
+an order that depends on the call alone: the same call gives the same bits.
+
+``switch_matmul`` records a gradient formula where grad mode is on and an input requires one.  A CUDA graph
+captures ``switch_matmul`` under ``torch.no_grad()`` and ``switch_matmul_grads``, not a recorded backward
+pass: autograd would tie the capture to the streams of whatever other graphs of the same leaves are alive.
+"""
+
+from __future__ import annotations
+
+from functools import lru_cache
+
+import torch
+
+from . import _lib
+from .vq import as_device
+
+__all__ = ["switch_matmul", "switch_matmul_grads"]
+
+_DTYPES = (torch.float16, torch.bfloat16)
+
+
+def _indices(indices, device) -> torch.Tensor:
+    indices = as_device(indices, device)
+    if indices.dtype.is_floating_point or indices.dtype.is_complex or indices.dtype == torch.bool:
+        raise ValueError(f"indices must use an integer dtype, found {indices.dtype}")
+    if indices.ndim < 1:
+        raise ValueError("indices must have at least one dimension")
+    if indices.dtype == torch.uint32:  # 0xFFFFFFFF, a pick without an expert, becomes -1: same bits
+        indices = indices.view(torch.int32)
+    elif indices.dtype not in (torch.int32, torch.int64):
+        indices = indices.to(torch.int64)
+    return indices.contiguous()
+
+
+def _x_div(x: torch.Tensor, indices: torch.Tensor, in_dim: int) -> int:
+    """Routes per row of x: 1, or the picks of a token."""
+    if x.ndim < 1 or int(x.shape[-1]) != in_dim:
+        raise ValueError(f"x trailing dimension must be {in_dim}, found {tuple(x.shape)}")
+    if tuple(x.shape[:-1]) == tuple(indices.shape):
+        return 1
+    if tuple(x.shape[:-1]) == tuple(indices.shape[:-1]):
+        return int(indices.shape[-1])
+    raise ValueError(
+        "x leading shape must either match indices leading shape for "
+        f"token routing or the full indices shape for per-route routing; found x {tuple(x.shape)} and indices {tuple(indices.shape)}")
+
+
+def _dense(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and on a 16-byte boundary (a view may start inside an allocation)."""
+    t = t.contiguous()
+    return t.clone() if t.data_ptr() % 16 else t
+
+
+def _grad_rows(grad: torch.Tensor, out_shape: tuple, dtype: torch.dtype) -> tuple[torch.Tensor, int]:
+    """The output gradient as rows of a multiple of 8 values, zeros behind its own."""
+    if tuple(grad.shape) != out_shape or grad.dtype != dtype:
+        raise ValueError(f"grad must be {out_shape} {dtype}, found {tuple(grad.shape)} {grad.dtype}")
+    ld = -(-out_shape[-1] // 8) * 8
+    return _dense(grad if ld == out_shape[-1] else torch.nn.functional.pad(grad, (0, ld - out_shape[-1]))), ld
+
+
+def _no_capture(what: str, grads: str) -> None:
+    if torch.cuda.is_current_stream_capturing():
+        raise _lib.KeepVQError(f"{what}: a recorded gradient cannot be captured; capture the call under torch.no_grad() and {grads}")
+
+
+@lru_cache(maxsize=256)
+def _scratch_bytes(routes: int, experts: int, out_dim: int, in_dim: int, x_div: int, grads: bool) -> int:
+    nbytes = int(_lib.load().keepvq_switch_matmul_workspace_bytes(routes, experts, out_dim, in_dim, x_div, int(grads)))
+    if nbytes < 0:
+        _lib.check(nbytes, "keepvq_switch_matmul_workspace_bytes")
+    return nbytes
+
+
+def _check(x: torch.Tensor, weight: torch.Tensor, indices):
+    if x.dtype not in _DTYPES or weight.dtype != x.dtype:
+        raise ValueError(f"x and weight must share one of fp16 / bf16, found {x.dtype} and {weight.dtype}")
+    if weight.ndim != 3 or 0 in weight.shape:
+        raise ValueError(f"weight must be [experts, out, in], found {tuple(weight.shape)}")
+    if int(weight.shape[2]) % 8 != 0:
+        raise ValueError("the input dimension must be divisible by 8")
+    device = _lib.require_cuda(x, weight)
+    indices = _indices(indices, device)
+    x_div = _x_div(x, indices, int(weight.shape[2]))
+    return device, indices, x_div, tuple(indices.shape) + (int(weight.shape[1]),)
+
+
+def _call(name: str, device, x, weight, grad, indices, x_div, grad_ld, out, dx, dweight):
+    experts, out_dim, in_dim = (int(s) for s in weight.shape)
+    routes = indices.numel()
+    nbytes = _scratch_bytes(routes, experts, out_dim, in_dim, max(x_div, 1), grad is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)  # of this call alone, as every scratch of the operators
+    address = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+    args = _lib.pack_switch_matmul_args(
+        x.data_ptr(), weight.data_ptr(), address(grad), _lib.dtype_tag(x.dtype), indices.data_ptr(), 8 * indices.element_size(), max(x_div, 1), routes,
+        experts, out_dim, in_dim, grad_ld, address(out), address(dx), address(dweight), ws.data_ptr(), nbytes)
+    with _lib.on_device(device):
+        _lib.check(getattr(_lib.load(), name)(args, _lib.stream_handle(device)), name)
+
+
+def _forward(x, weight, indices) -> torch.Tensor:
+    device, indices, x_div, out_shape = _check(x, weight, indices)
+    out = torch.empty(out_shape, dtype=x.dtype, device=device)
+    if out.numel():
+        _call("keepvq_switch_matmul", device, _dense(x), _dense(weight), None, indices, x_div, 0, out, None, None)
+    return out
+
+
+def switch_matmul_grads(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor, indices, *, x_grad: bool = True,
+                        weight_grad: bool = True) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    """The gradients of ``x`` and ``weight`` where ``grad`` is that of ``switch_matmul(x, weight, indices)``,
+    in their dtype; None for one that is not wanted.  A row's gradient is the fp32 sum over its picks,
+    rounded once; experts without routes get zeros."""
+    device, indices, x_div, out_shape = _check(x, weight, indices)
+    _lib.require_cuda(x, grad)
+    grad, grad_ld = _grad_rows(grad, out_shape, x.dtype)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=device) if x_grad else None
+    dweight = torch.empty(weight.shape, dtype=x.dtype, device=device) if weight_grad else None
+    if indices.numel() == 0:
+        return dx.zero_() if x_grad else None, dweight.zero_() if weight_grad else None
+    if x_grad or weight_grad:
+        _call("keepvq_switch_matmul_grads", device, _dense(x), _dense(weight), grad, indices, x_div, grad_ld, None, dx, dweight)
+    return dx, dweight
+
+
+class _SwitchMatmul(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, indices):
+        ctx.save_for_backward(x, weight, indices)
+        return _forward(x, weight, indices)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        _no_capture("switch_matmul", "switch_matmul_grads")
+        x, weight, indices = ctx.saved_tensors
+        dx, dweight = switch_matmul_grads(grad, x, weight, indices, x_grad=ctx.needs_input_grad[0], weight_grad=ctx.needs_input_grad[1])
+        return dx, dweight, None
+
+
+def switch_matmul(x: torch.Tensor, weight: torch.Tensor, indices) -> torch.Tensor:
+    """``x`` [tokens, in] with ``indices`` [tokens, k] -> [tokens, k, out]; ``x`` [..., k, in] with
+    ``indices`` [..., k] -> [..., k, out]: every route against the expert it names."""
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
+        _lib.require_cuda(x, weight)
+        _no_capture("switch_matmul", "switch_matmul_grads")
+        return _SwitchMatmul.apply(x, weight, as_device(indices, x.device))
+    return _forward(x, weight, indices)

@@ -1,0 +1,118 @@
+"""Refusals of the products over 16-bit experts and low-rank adapters: they come before any device work."""
+
+import ctypes
+
+import pytest
+import torch
+
+from keep_b200 import _lib
+from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+from keep_b200.low_rank import LowRank, switch_low_rank, switch_low_rank_grads
+
+NULL, SHAPE, DTYPE, ALIGN, UNSUPPORTED, CAPACITY = -1, -2, -3, -4, -5, -7
+F16 = torch.float16
+
+
+def rows(*shape, dtype=F16):
+    return torch.zeros(shape, dtype=dtype)
+
+
+@pytest.mark.parametrize("x,weight,message", [
+    (rows(4, 16, dtype=torch.float32), rows(3, 8, 16, dtype=torch.float32), "fp16 / bf16"),
+    (rows(4, 16), rows(3, 8, 16, dtype=torch.bfloat16), "fp16 / bf16"),
+    (rows(4, 16), rows(8, 16), "weight must be"),
+    (rows(4, 16), rows(0, 8, 16), "weight must be"),
+    (rows(4, 12), rows(3, 8, 12), "divisible by 8")])
+def test_matmul_refuses(x, weight, message):
+    for call in (lambda: switch_matmul(x, weight, torch.zeros(4, 2, dtype=torch.int32)),
+                 lambda: switch_matmul_grads(rows(4, 2, 8), x, weight, torch.zeros(4, 2, dtype=torch.int32))):
+        with pytest.raises(ValueError, match=message):
+            call()
+
+
+@pytest.mark.parametrize("left,right,message", [
+    (rows(3, 8, 4, dtype=torch.float32), rows(3, 4, 16, dtype=torch.float32), "fp16 / bf16"),
+    (rows(3, 8, 4), rows(3, 5, 16), "left must be"),
+    (rows(3, 8, 4), rows(2, 4, 16), "left must be"),
+    (rows(3, 8, 0), rows(3, 0, 16), "left must be"),
+    (rows(3, 8, 129), rows(3, 129, 16), "at most 128"),
+    (rows(3, 8, 4), rows(3, 4, 12), "divisible by 8")])
+def test_low_rank_refuses(left, right, message):
+    x, indices = rows(4, 16), torch.zeros(4, dtype=torch.int32)
+    for call in (lambda: switch_low_rank(x, left, right, indices), lambda: switch_low_rank_grads(rows(4, 8), x, left, right, indices), lambda: LowRank(left, right)):
+        with pytest.raises(ValueError, match=message):
+            call()
+
+
+def test_cpu_tensors_are_refused():
+    with pytest.raises(_lib.KeepVQError, match="no CPU path"):
+        switch_matmul(rows(4, 16), rows(3, 8, 16), torch.zeros(4, 2, dtype=torch.int32))
+    with pytest.raises(_lib.KeepVQError, match="no CPU path"):
+        switch_low_rank(rows(4, 16), rows(3, 8, 4), rows(3, 4, 16), torch.zeros(4, dtype=torch.int32))
+    with pytest.raises(ValueError, match="found torch.bfloat16"):
+        switch_low_rank(rows(4, 16, dtype=torch.bfloat16), rows(3, 8, 4), rows(3, 4, 16), torch.zeros(4, dtype=torch.int32))
+
+
+# ---- the C entry points: arguments of a valid call, each case with one of them changed; none reaches a CUDA call ----
+
+def matmul_args(**change):
+    a = _lib.SwitchMatmulArgs(x=256, weight=256, grad=256, dtype=1, indices=256, index_bits=32, x_div=2, routes=8, experts=3, out_dim=24, in_dim=16, grad_ld=24,
+                              out=256, dx=256, dweight=256, workspace=256, workspace_bytes=1 << 30)
+    for name, value in change.items():
+        setattr(a, name, value)
+    return a
+
+
+def low_rank_args(**change):
+    a = _lib.SwitchLowRankArgs(x=256, left=256, right=256, grad=256, dtype=1, indices=256, index_bits=32, x_div=2, routes=8, sets=3, out_dim=24, in_dim=16, rank=8,
+                               grad_ld=24, scale=1.0, out_dtype=1, base=256, base_ld=24, out=256, out_ld=24, dx=256, dleft=256, dright=256, workspace=256, workspace_bytes=1 << 30)
+    for name, value in change.items():
+        setattr(a, name, value)
+    return a
+
+
+BOTH = [(dict(dtype=0), DTYPE), (dict(dtype=7), DTYPE), (dict(index_bits=16), DTYPE), (dict(routes=-1), SHAPE), (dict(routes=7), SHAPE), (dict(x_div=0), SHAPE),
+        (dict(in_dim=12), SHAPE), (dict(out_dim=0), SHAPE), (dict(routes=1 << 25), CAPACITY), (dict(workspace=None), NULL), (dict(workspace=264), ALIGN),
+        (dict(workspace_bytes=64), CAPACITY), (dict(x=None), NULL), (dict(indices=None), NULL), (dict(x=258), ALIGN), (dict(indices=258), ALIGN)]
+
+
+@pytest.mark.parametrize("change,status", BOTH + [(dict(experts=0), SHAPE), (dict(experts=1 << 15), CAPACITY), (dict(weight=None), NULL), (dict(weight=264), ALIGN)])
+def test_the_matmul_entry_points_refuse(change, status):
+    lib = _lib.load()
+    assert lib.keepvq_switch_matmul(matmul_args(**change), None) == status
+    assert lib.keepvq_switch_matmul_grads(matmul_args(**change), None) == status
+
+
+@pytest.mark.parametrize("change,status", BOTH + [(dict(sets=0), SHAPE), (dict(sets=1 << 15), CAPACITY), (dict(left=None), NULL), (dict(right=264), ALIGN),
+                                                  (dict(rank=12), SHAPE), (dict(rank=0), SHAPE), (dict(rank=136), UNSUPPORTED)])
+def test_the_low_rank_entry_points_refuse(change, status):
+    lib = _lib.load()
+    assert lib.keepvq_switch_low_rank(low_rank_args(**change), None) == status
+    assert lib.keepvq_switch_low_rank_grads(low_rank_args(**change), None) == status
+
+
+def test_what_only_one_direction_looks_at():
+    lib = _lib.load()
+    assert lib.keepvq_switch_matmul(matmul_args(out=None), None) == NULL
+    assert lib.keepvq_switch_matmul_grads(matmul_args(grad=None), None) == NULL
+    assert lib.keepvq_switch_matmul_grads(matmul_args(grad_ld=16), None) == SHAPE
+    assert lib.keepvq_switch_matmul_grads(matmul_args(grad_ld=28), None) == SHAPE
+    assert lib.keepvq_switch_low_rank(low_rank_args(out=None), None) == NULL
+    assert lib.keepvq_switch_low_rank(low_rank_args(out_dtype=2), None) == DTYPE
+    assert lib.keepvq_switch_low_rank(low_rank_args(base_ld=23), None) == SHAPE
+    assert lib.keepvq_switch_low_rank(low_rank_args(out_ld=23), None) == SHAPE
+    assert lib.keepvq_switch_low_rank_grads(low_rank_args(grad_ld=16), None) == SHAPE
+    for name, args in (("keepvq_switch_matmul", matmul_args), ("keepvq_switch_low_rank", low_rank_args)):
+        assert getattr(lib, name)(args(routes=0), None) == 0  # nothing to do, nothing launched
+        assert getattr(lib, name)(ctypes.cast(None, ctypes.POINTER(type(args()))), None) == NULL
+        assert getattr(lib, name + "_grads")(ctypes.cast(None, ctypes.POINTER(type(args()))), None) == NULL
+
+
+def test_scratch_sizes():
+    lib = _lib.load()
+    assert lib.keepvq_switch_matmul_workspace_bytes(8, 3, 24, 12, 2, 0) == SHAPE
+    assert lib.keepvq_switch_matmul_workspace_bytes(8, 1 << 15, 24, 16, 2, 0) == CAPACITY
+    assert lib.keepvq_switch_low_rank_workspace_bytes(8, 3, 24, 16, 136, 2, 0) == UNSUPPORTED
+    # a row's gradient is summed over its picks in fp32
+    assert lib.keepvq_switch_matmul_workspace_bytes(4096, 8, 512, 1024, 2, 1) >= 4096 * 1024 * 4
+    assert lib.keepvq_switch_matmul_workspace_bytes(0, 1, 8, 8, 1, 0) > 0

@@ -1,0 +1,254 @@
+"""Products over 16-bit experts (switch_matmul and its gradients) against a plain 64-bit form."""
+
+import pytest
+import torch
+
+import switch_reference as ref
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+def make(cuda, tokens, k, experts, inp, out, dtype=BF16, per_route=False, dead=0.0, seed=0, one_expert=None):
+    gen = torch.Generator(device=cuda).manual_seed(seed)
+    rand = lambda *shape: torch.randn(shape, generator=gen, device=cuda)  # noqa: E731
+    x = rand(*((tokens, k, inp) if per_route else (tokens, inp))).to(dtype)
+    weight = (rand(experts, out, inp) * inp ** -0.5).to(dtype)
+    indices = ref.picks(gen, tokens, k, experts, dead) if one_expert is None else torch.full((tokens, k), one_expert, dtype=torch.int32, device=cuda)
+    return x, weight, indices, (0.1 * rand(tokens, k, out)).to(dtype)
+
+
+# tokens, picks, experts, in, out: single tokens, sizes below and across the tiles, widths that fill no tile,
+# one expert for all, more experts than routes, hundreds of routes an expert
+SIZES = [(1, 6, 8, 256, 136), (1, 1, 1, 8, 8), (3, 2, 5, 72, 200), (17, 4, 6, 136, 72), (130, 1, 1, 128, 264), (5, 6, 300, 64, 40), (257, 6, 7, 520, 136),
+         (700, 2, 3, 64, 1000), (64, 6, 48, 1024, 512), (1021, 6, 24, 392, 328)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("per_route", [False, True])
+@pytest.mark.parametrize("size", SIZES)
+def test_forward_and_gradients(cuda, size, per_route, dtype):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, *size, dtype=dtype, per_route=per_route, dead=0.15 if size[0] > 2 else 0.0, seed=sum(size))
+    ref.close(switch_matmul(x, weight, indices), ref.matmul(x, weight, indices))
+    dx, dweight = switch_matmul_grads(grad, x, weight, indices)
+    want_x, want_w = ref.matmul_grads(grad, x, weight, indices)
+    ref.close(dx, want_x)
+    ref.close(dweight, want_w)
+
+
+@pytest.mark.parametrize("out", [1, 7, 100, 513])
+def test_output_widths_that_are_no_multiple_of_eight(cuda, out):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 37, 3, 5, 264, out, dead=0.2, seed=out)
+    ref.close(switch_matmul(x, weight, indices), ref.matmul(x, weight, indices))
+    for got, want in zip(switch_matmul_grads(grad, x, weight, indices), ref.matmul_grads(grad, x, weight, indices)):
+        ref.close(got, want)
+
+
+def test_dead_routes_only_and_routes_of_one_expert_only(cuda):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    for k in (1, 3):
+        x, weight, indices, grad = make(cuda, 19, k, 4, 128, 72, one_expert=-1)
+        assert not switch_matmul(x, weight, indices).any()
+        assert not any(g.any() for g in switch_matmul_grads(grad, x, weight, indices))
+        x, weight, indices, grad = make(cuda, 190, k, 4, 128, 72, one_expert=2)  # the same index several times in a row of picks
+        ref.close(switch_matmul(x, weight, indices), ref.matmul(x, weight, indices))
+        dx, dweight = switch_matmul_grads(grad, x, weight, indices)
+        ref.close(dx, ref.matmul_grads(grad, x, weight, indices)[0])
+        assert not dweight[[0, 1, 3]].any()
+
+
+def test_values_that_are_not_finite_stay_where_they_belong(cuda):
+    """Neighbouring experts, tokens and rows share tiles with them."""
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 40, 1, 3, 136, 200, seed=3)
+    indices[:] = torch.arange(40, device=cuda)[:, None] % 2
+    want, want_grads = ref.matmul(x, weight, indices), ref.matmul_grads(grad, x, weight, indices)
+    for bad in (float("nan"), float("inf")):
+        w = weight.clone()
+        w[2] = bad  # an expert without routes, right behind the last with some
+        ref.close(switch_matmul(x, w, indices), want)
+        ref.close(switch_matmul_grads(grad, x, w, indices)[0], want_grads[0])
+        w = weight.clone()
+        w[1] = bad
+        keep = indices[:, 0] == 0
+        ref.close(switch_matmul(x, w, indices)[keep], [t[keep] for t in want])
+        ref.close(switch_matmul_grads(grad, x, w, indices)[0][keep], [t[keep] for t in want_grads[0]])
+        rows = x.clone()
+        rows[7] = bad  # expert 1's
+        got = switch_matmul(rows, weight, indices)
+        others = torch.arange(40, device=cuda) != 7
+        ref.close(got[others], [t[others] for t in want])
+        assert not torch.isfinite(got[7]).any()
+        ref.close(switch_matmul_grads(grad, rows, weight, indices)[1][0], [t[0] for t in want_grads[1]])
+        g = grad.clone()
+        g[9] = bad
+        dx, dweight = switch_matmul_grads(g, x, weight, indices)
+        others = torch.arange(40, device=cuda) != 9
+        ref.close(dx[others], [t[others] for t in want_grads[0]])
+        ref.close(dweight[0], [t[0] for t in want_grads[1]])
+
+
+@pytest.mark.parametrize("kind", [torch.int64, torch.uint32, torch.int16])
+def test_index_types(cuda, kind):
+    from keep_b200.dense_switch import switch_matmul
+
+    x, weight, indices, _ = make(cuda, 9, 2, 4, 64, 48)
+    want = switch_matmul(x, weight, indices)
+    if kind == torch.uint32:
+        indices[2, 1] = -1
+        want[2, 1] = 0
+        other = indices.view(torch.uint32)
+    else:
+        other = indices.to(kind)
+    if kind == torch.int64:
+        other[3, 0] += 1 << 32  # not an expert, whatever its low word says
+        want[3, 0] = 0
+    assert torch.equal(switch_matmul(x, weight, other), want)
+
+
+def test_strides_alignment_and_leading_shapes(cuda):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 12, 2, 4, 64, 48)
+    want, (want_x, want_w) = switch_matmul(x, weight, indices), switch_matmul_grads(grad, x, weight, indices)
+    odd = lambda t: torch.cat([t.new_zeros(1), t.flatten()])[1:].view(t.shape)  # noqa: E731 - starts 2 bytes into its allocation
+    across = lambda t: t.transpose(-1, -2).contiguous().transpose(-1, -2)  # noqa: E731
+    for change in (odd, across):
+        assert torch.equal(switch_matmul(change(x), change(weight), indices.t().contiguous().t()), want)
+        dx, dw = switch_matmul_grads(change(grad), change(x), change(weight), indices)
+        assert torch.equal(dx, want_x) and torch.equal(dw, want_w)
+    assert torch.equal(switch_matmul(x.view(3, 4, 64), weight, indices.view(3, 4, 2)), want.view(3, 4, 2, 48))
+    assert torch.equal(switch_matmul(x[5], weight, indices[5]), want[5])
+
+
+def test_no_routes(cuda):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 4, 2, 3, 64, 48)
+    assert tuple(switch_matmul(x[:0], weight, indices[:0]).shape) == (0, 2, 48)
+    assert tuple(switch_matmul(x, weight, indices[:, :0]).shape) == (4, 0, 48)
+    dx, dw = switch_matmul_grads(grad[:, :0], x, weight, indices[:, :0])
+    assert tuple(dx.shape) == (4, 64) and not dx.any() and not dw.any()
+
+
+def test_a_call_repeats_bit_for_bit_and_does_not_depend_on_the_order_of_other_rows(cuda):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 777, 6, 10, 512, 264, seed=8)
+    y, (dx, dw) = switch_matmul(x, weight, indices), switch_matmul_grads(grad, x, weight, indices)
+    for _ in range(3):
+        assert torch.equal(switch_matmul(x, weight, indices), y)
+        again = switch_matmul_grads(grad, x, weight, indices)
+        assert torch.equal(again[0], dx) and torch.equal(again[1], dw)
+    only_x, none = switch_matmul_grads(grad, x, weight, indices, weight_grad=False)
+    assert none is None and torch.equal(only_x, dx)
+    none, only_w = switch_matmul_grads(grad, x, weight, indices, x_grad=False)
+    assert none is None and torch.equal(only_w, dw)
+
+
+def test_gradients_against_differences(cuda):
+    """Small integers: every product, sum and rounding is exact, and the product is linear in x and in the
+    weights, so a central difference IS the derivative along its direction."""
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    gen = torch.Generator(device=cuda).manual_seed(4)
+    ints = lambda *shape: torch.randint(-1, 2, shape, generator=gen, device=cuda).to(BF16)  # noqa: E731
+    x, weight, grad = ints(20, 40), ints(3, 24, 40), ints(20, 2, 24)
+    indices = ref.picks(gen, 20, 2, 3, dead=0.2)
+    dx, dw = switch_matmul_grads(grad, x, weight, indices)
+    for _ in range(4):
+        d, e = ints(20, 40), ints(3, 24, 40)
+        of_x = (switch_matmul(x + d, weight, indices).double() - switch_matmul(x - d, weight, indices).double()) / 2
+        of_w = (switch_matmul(x, weight + e, indices).double() - switch_matmul(x, weight - e, indices).double()) / 2
+        assert (grad.double() * of_x).sum() == (dx.double() * d.double()).sum()
+        assert (grad.double() * of_w).sum() == (dw.double() * e.double()).sum()
+
+
+def test_autograd_records_the_same_gradients(cuda):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 30, 3, 5, 128, 72)
+    want = switch_matmul_grads(grad, x, weight, indices)
+    xs, ws = x.clone().requires_grad_(), weight.clone().requires_grad_()
+    switch_matmul(xs, ws, indices).backward(grad)
+    assert torch.equal(xs.grad, want[0]) and torch.equal(ws.grad, want[1])
+    frozen = x.clone().requires_grad_()
+    y = switch_matmul(frozen, weight, indices)
+    assert torch.equal(torch.autograd.grad(y, frozen, grad)[0], want[0])
+    with torch.no_grad():
+        assert not switch_matmul(xs, ws, indices).requires_grad
+
+
+def test_captured_calls_follow_their_inputs(cuda):
+    from keep_b200 import _lib
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 50, 2, 6, 128, 136, dead=0.1)
+    leaf = x.clone().requires_grad_()
+    alive = switch_matmul(leaf, weight, indices)  # an eager graph of a leaf, alive during the capture
+    graphs, outs = [], []
+    for _ in range(2):  # two graphs, replayed in turn: each has its own workspace
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph), torch.no_grad():
+            outs.append((switch_matmul(x, weight, indices), *switch_matmul_grads(grad, x, weight, indices)))
+        graphs.append(graph)
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        with pytest.raises(_lib.KeepVQError, match="cannot be captured"):
+            switch_matmul(leaf, weight, indices)
+    torch.autograd.grad(alive, leaf, grad)
+    for seed in (1, 2):
+        new = make(cuda, 50, 2, 6, 128, 136, dead=0.1, seed=seed)
+        for old, fresh in zip((x, weight, indices, grad), new):
+            old.copy_(fresh)
+        want = (switch_matmul(x, weight, indices), *switch_matmul_grads(grad, x, weight, indices))
+        for graph in graphs:
+            graph.replay()
+        torch.cuda.synchronize()
+        for got in outs:
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_calls_on_two_streams_at_once(cuda):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    problems = [make(cuda, 300, 3, 8, 512, 264, seed=s) for s in (1, 2)]
+    want = [(switch_matmul(x, w, i), *switch_matmul_grads(g, x, w, i)) for x, w, i, g in problems]
+    streams = [torch.cuda.Stream() for _ in problems]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for n, (stream, (x, w, i, g)) in enumerate(zip(streams, problems)):
+            with torch.cuda.stream(stream):
+                got[n].append((switch_matmul(x, w, i), *switch_matmul_grads(g, x, w, i)))
+    torch.cuda.synchronize()
+    for n in range(2):
+        for result in got[n]:
+            assert all(torch.equal(a, b) for a, b in zip(result, want[n]))
+
+
+def test_weights_beyond_32_bit_offsets(cuda):
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    experts, out, inp = 1100, 1024, 2048  # 2.3e9 values
+    weight = torch.zeros((experts, out, inp), dtype=BF16, device=cuda)
+    gen = torch.Generator(device=cuda).manual_seed(1)
+    for e in (0, experts - 1):
+        weight[e] = torch.randn((out, inp), generator=gen, device=cuda).to(BF16)
+    x = torch.randn((40, inp), generator=gen, device=cuda).to(BF16)
+    grad = torch.randn((40, 2, out), generator=gen, device=cuda).to(BF16)
+    indices = torch.tensor([[0, experts - 1]], dtype=torch.int32, device=cuda).repeat(40, 1)
+    small = weight[[0, experts - 1]]
+    few = torch.tensor([[0, 1]], dtype=torch.int32, device=cuda).repeat(40, 1)
+    ref.close(switch_matmul(x, weight, indices), ref.matmul(x, small, few))
+    dx, dw = switch_matmul_grads(grad, x, weight, indices)
+    want_x, want_w = ref.matmul_grads(grad, x, small, few)
+    ref.close(dx, want_x)
+    ref.close(dw[[0, experts - 1]], want_w)
+    assert not dw[1:experts - 1].any()
