@@ -1,90 +1,391 @@
-// Products over 16-bit experts chosen per route, and their gradients.
+// Products over 16-bit experts chosen per route, and their gradients, on the 5th-generation tensor
+// cores.
 //
 //   forward   out[r]    = W[e_r] x[r / x_div]
 //   dx        dx[r]     = W[e_r]^T grad[r], summed over a row's picks in fp32
 //   dweight   dW[e]     = sum over e's routes of grad[r] x[r / x_div]^T
+//
+// One kernel for the three: a tile of 128 values along a result's rows (the M operand: weight rows,
+// weight columns, columns of x) times up to N_MAX result rows (the N operand: a set's routes, or columns
+// of grad).  The routes are the N operand because N is free in steps of 16: a set of five routes costs one
+// such step of the tensor core and its own rows of shared memory, not a tile of 128.
+//
+//            M operand [128]                      N operand [<= N_MAX]                 contraction
+//   forward  W[e] rows        (K-major box)       x rows, gathered     (K-major)       in_dim
+//   dx       W[e] columns     (MN-major box)      grad rows, gathered  (K-major)       out_dim
+//   dweight  x columns, rows gathered (MN-major)  grad columns, rows gathered (MN-major)  e's routes
+//
+// The rows of a set are wherever the caller has them: TMA gathers four at a time by their index, and
+// fills rows past the end of a matrix with zeros (the ragged end of a set's routes in dweight).
+#include "async_copy.cuh"
 #include "switch_plan.cuh"
 
 namespace keepvq {
 namespace dense {
 
+using fast::elect_one;
+using fast::global_timer_ns;
+using fast::mbar_complete;
+using fast::mbar_expect_tx;
+using fast::mbar_init;
+using fast::smem_addr;
+
 enum { FORWARD = 0, INPUT_GRAD = 1, WEIGHT_GRAD = 2 };
-constexpr int TILE = 64, STEP = 16;
+constexpr int M_TILE = 128, K_BLOCK = 64, N_STEP = 16;  // K_BLOCK: 128 bytes, a swizzled row
+constexpr int MM_THREADS = 256;
+enum { WARP_M = 0, WARP_N = 1, WARP_MMA = 2, WARP_OUT = 4 };  // loaders of the two operands, the issuer, four warps of the epilogue
+constexpr uint64_t MM_WAIT_NS = 2000000000ull;
+
+// ---- instructions ---------------------------------------------------------------------------------
+__device__ __forceinline__ void tma_box_3d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+}
+// Four rows of a matrix, 128 bytes of each from column x on.  The map's box is one row high.
+__device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* map, int32_t x, const int4& rows, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar) : "memory");
+}
+__device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+               ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+// 32 columns of this thread's lane of tensor memory.
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                 "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]), "=r"(v[18]), "=r"(v[19]), "=r"(v[20]),
+                 "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]), "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+               : "r"(taddr) : "memory");
+}
+
+// Operand tiles with the 128-byte swizzle.  K-major: rows of 128 bytes along the contraction, groups of
+// eight 1024 bytes apart.  MN-major: 64 values of M or N in 128 bytes, a row per step of the contraction,
+// groups of eight 1024 bytes apart, the next 64 values one box (64 rows) on.
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn_major) {
+  const uint64_t lead = mn_major ? (K_BLOCK * 128) >> 4 : 1;
+  return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (lead << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// Wait of a whole warp, bounded by time: false when the deadline passes or another warp gave up.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint64_t deadline, volatile int* abort_flag) {
+  for (uint32_t spin = 0;; ++spin) {
+    if (__all_sync(0xFFFFFFFFu, mbar_complete(bar, parity))) return true;
+    if ((spin & 31u) == 31u) {
+      if (__any_sync(0xFFFFFFFFu, *abort_flag)) return false;
+      if (__any_sync(0xFFFFFFFFu, global_timer_ns() > deadline)) { *abort_flag = 1; return false; }
+    }
+  }
+}
+
+template <uint32_t STAGES>
+struct Ring {
+  uint32_t index = 0, phase = 0;
+  __device__ __forceinline__ void advance() {
+    if (++index == STAGES) { index = 0; phase ^= 1u; }
+  }
+};
+
+template <int N_MAX>
+struct Shape {
+  static constexpr uint32_t A_BYTES = M_TILE * K_BLOCK * 2, B_BYTES = N_MAX * K_BLOCK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  static constexpr uint32_t STAGES = 192 * 1024 / STAGE_BYTES;  // 4 or 8: as many weights in flight either way
+  static constexpr uint32_t OUT_BYTES = 4 * 32 * 32 * 2;        // a 32 x 32 piece of the result for each warp of the epilogue
+  static constexpr uint32_t SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + OUT_BYTES;
+  static constexpr uint32_t TMEM_COLS = 2 * N_MAX;              // two accumulators: one is written while the other is drained
+};
+
+struct MatmulArgs {
+  int x_div, sets, dtype;
+  int64_t routes, out_dim, in_dim;
+  void* out;        // result rows
+  float* route_dx;  // dx before the pick sum, or null
+  Plan plan;
+};
 
 template <typename T>
-__device__ __forceinline__ float widen(T v);
+__device__ __forceinline__ uint16_t bits_of(float v);
 template <>
-__device__ __forceinline__ float widen(__half v) { return __half2float(v); }
+__device__ __forceinline__ uint16_t bits_of<__half>(float v) { return __half_as_ushort(__float2half_rn(v)); }
 template <>
-__device__ __forceinline__ float widen(__nv_bfloat16 v) { return __bfloat162float(v); }
+__device__ __forceinline__ uint16_t bits_of<__nv_bfloat16>(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 
-// 64 x 64 outputs per block, 4 x 4 per thread, operands widened to fp32 in shared memory.
-template <typename T, int MODE>
-__global__ void __launch_bounds__(256) switch_matmul_kernel(keepvq_switch_matmul_args a, Plan plan, float* route_dx) {
-  __shared__ float left[STEP][TILE + 1], right[STEP][TILE + 1];  // [contraction][output column], [contraction][output row]
-  const T *x = static_cast<const T*>(a.x), *w = static_cast<const T*>(a.weight), *g = static_cast<const T*>(a.grad);
-  int set, start, size;
-  if (MODE == WEIGHT_GRAD) {
-    set = blockIdx.z;
-    start = plan.offset[set];
-    size = plan.offset[set + 1] - start;
-  } else {
-    if (static_cast<int>(blockIdx.x) >= *plan.tiles) {
-      if (MODE == FORWARD)  // dead routes
-        for (int64_t r = plan.offset[a.experts] + blockIdx.x - *plan.tiles; r < a.routes; r += gridDim.x - *plan.tiles)
-          for (int64_t n = blockIdx.y * 256 + threadIdx.x; n < a.out_dim; n += gridDim.y * 256) store_from_float(a.out, a.dtype, plan.order[r] * a.out_dim + n, 0.0f);
-      return;
-    }
-    const int4 t = plan.tile[blockIdx.x];
-    set = t.x; start = t.y; size = t.z;
+// One tile of the result.
+struct Item {
+  int set, start, size;  // size: routes (the N operand's rows, or the contraction of dweight)
+  int m0, n0;            // first value along a result's row; first result row (dweight)
+  int n;                 // result rows
+  int k_blocks;
+};
+
+template <int MODE, int N_MAX>
+__global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs a, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map) {
+  using S = Shape<N_MAX>;
+  constexpr uint32_t STAGES = S::STAGES;
+  constexpr bool M_MN = MODE != FORWARD, N_MN = MODE == WEIGHT_GRAD;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t bars[2 * STAGES + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ int abort_flag;
+  grid_launch_dependents();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
+  const uint32_t full = smem_addr(bars), empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16;
+  if (tid == 0) {
+    abort_flag = 0;
+    for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 2); mbar_init(empty + 8 * s, 1); }
+    for (uint32_t s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  const int64_t col0 = static_cast<int64_t>(MODE == WEIGHT_GRAD ? blockIdx.x : blockIdx.y) * TILE;
-  const int64_t row0 = MODE == WEIGHT_GRAD ? blockIdx.y * TILE : 0;
-  const int64_t depth = MODE == FORWARD ? a.in_dim : MODE == INPUT_GRAD ? a.out_dim : size;
-  const int64_t cols = MODE == FORWARD ? a.out_dim : a.in_dim, rows = MODE == WEIGHT_GRAD ? a.out_dim : size;
-  const T* we = w + set * a.out_dim * a.in_dim;
-  float sum[4][4] = {};
-  const int tr = threadIdx.x / 16, tc = threadIdx.x % 16;
-  for (int64_t k0 = 0; k0 < depth; k0 += STEP) {
-    for (int i = threadIdx.x; i < STEP * TILE; i += 256) {
-      const int k = i / TILE, c = i % TILE;
-      const int64_t kk = k0 + k;
-      float lv = 0.0f, rv = 0.0f;
-      if (kk < depth) {
-        if (MODE == FORWARD) {
-          if (col0 + c < cols) lv = widen(we[(col0 + c) * a.in_dim + kk]);
-          if (c < rows) rv = widen(x[plan.order[start + c] / a.x_div * a.in_dim + kk]);
-        } else if (MODE == INPUT_GRAD) {
-          if (col0 + c < cols) lv = widen(we[kk * a.in_dim + col0 + c]);
-          if (c < rows) rv = widen(g[plan.order[start + c] * a.grad_ld + kk]);
-        } else {
-          const int64_t r = plan.order[start + kk];
-          if (col0 + c < cols) lv = widen(x[r / a.x_div * a.in_dim + col0 + c]);
-          if (row0 + c < rows) rv = widen(g[r * a.grad_ld + row0 + c]);
+  if (warp == WARP_MMA) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(S::TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+  const uint32_t tmem = tmem_slot;
+  grid_wait();
+  const uint64_t deadline = global_timer_ns() + MM_WAIT_NS;
+  volatile int* aborted = &abort_flag;
+
+  const int cols = static_cast<int>(MODE == FORWARD ? a.out_dim : a.in_dim);  // of a result row
+  const int m_tiles = (cols + M_TILE - 1) / M_TILE;
+  const int n_tiles = MODE == WEIGHT_GRAD ? static_cast<int>((a.out_dim + N_MAX - 1) / N_MAX) : 0;
+  const int depth_blocks = static_cast<int>(((MODE == FORWARD ? a.in_dim : a.out_dim) + K_BLOCK - 1) / K_BLOCK);
+  const int64_t items = static_cast<int64_t>(m_tiles) * (MODE == WEIGHT_GRAD ? static_cast<int64_t>(n_tiles) * a.sets : *a.plan.tiles);
+  // Every role walks the same items on its own clock.
+  auto item_at = [&](int64_t i) {
+    Item it;
+    const int64_t outer = i / m_tiles;
+    it.m0 = static_cast<int>(i - outer * m_tiles) * M_TILE;
+    if (MODE == WEIGHT_GRAD) {
+      it.set = static_cast<int>(outer / n_tiles);
+      it.n0 = static_cast<int>(outer - static_cast<int64_t>(it.set) * n_tiles) * N_MAX;
+      it.start = a.plan.offset[it.set];
+      it.size = a.plan.offset[it.set + 1] - it.start;
+      it.n = min(N_MAX, static_cast<int>(a.out_dim) - it.n0);
+      it.k_blocks = (it.size + K_BLOCK - 1) / K_BLOCK;
+    } else {
+      const int4 t = a.plan.tile[outer];
+      it.set = t.x; it.start = t.y; it.size = t.z;
+      it.n0 = 0;
+      it.n = it.size;
+      it.k_blocks = depth_blocks;
+    }
+    return it;
+  };
+  bool ok = true, mma_issued = false;
+
+  if (warp == WARP_M || warp == WARP_N) {
+    // ================= the loaders ===============================================================
+    Ring<STAGES> r;
+    const uint32_t tile = ring + (warp == WARP_N ? S::A_BYTES : 0);
+    const CUtensorMap* map = warp == WARP_M ? &m_map : &n_map;
+    const int rows_end = static_cast<int>(MODE == WEIGHT_GRAD && warp == WARP_M ? a.routes / a.x_div : a.routes);  // of the gathered matrix: zeros from here on
+    const int div = (MODE == FORWARD && warp == WARP_N) || (MODE == WEIGHT_GRAD && warp == WARP_M) ? a.x_div : 1;
+    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      const Item it = item_at(i);
+      auto row_at = [&](int p) { return a.plan.order[it.start + p] / div; };
+      int4 rows[2];
+      if (MODE != WEIGHT_GRAD && warp == WARP_N) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {  // rows past the last route repeat it: nobody looks at their columns
+          const int q = (u * 32 + lane) * 4, last = it.size - 1;
+          if (q < it.size) rows[u] = make_int4(row_at(q), row_at(min(q + 1, last)), row_at(min(q + 2, last)), row_at(min(q + 3, last)));
         }
       }
-      left[k][c] = lv;
-      right[k][c] = rv;
+      for (int kb = 0; kb < it.k_blocks; ++kb) {
+        int steps = 0;
+        if (MODE == WEIGHT_GRAD) {  // 16 quads of rows, two lanes each
+          const int first = kb * K_BLOCK, q = first + (lane & 15) * 4;
+          steps = min(K_BLOCK, (it.size - first + N_STEP - 1) / N_STEP * N_STEP);
+          auto row_or_end = [&](int p) { return p < it.size ? row_at(p) : rows_end; };
+          rows[0] = make_int4(row_or_end(q), row_or_end(q + 1), row_or_end(q + 2), row_or_end(q + 3));
+        }
+        ok = wait_for(empty + 8 * r.index, r.phase ^ 1u, deadline, aborted);
+        if (!ok) break;
+        const uint32_t bar = full + 8 * r.index, dst = tile + r.index * S::STAGE_BYTES;
+        if (MODE == WEIGHT_GRAD) {
+          const int width = warp == WARP_M ? M_TILE : it.n, col0 = warp == WARP_M ? it.m0 : it.n0, boxes = (width + 63) / 64;
+          if (lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>(boxes * steps * 128));
+          __syncwarp();
+          if ((lane & 15) * 4 < steps)
+            for (int b = lane >> 4; b < boxes; b += 2) tma_rows4(dst + b * (K_BLOCK * 128) + (lane & 15) * 512, map, col0 + b * 64, rows[0], bar);
+        } else if (warp == WARP_N) {
+          if (lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>((it.size + 3) / 4 * 512));
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < (N_MAX > 128 ? 2 : 1); ++u) {
+            const int q = u * 32 + lane;
+            if (q * 4 < it.size) tma_rows4(dst + q * 512, map, kb * K_BLOCK, rows[u], bar);
+          }
+        } else if (elect_one()) {
+          mbar_expect_tx(bar, S::A_BYTES);
+          if (MODE == FORWARD) tma_box_3d(dst, map, kb * K_BLOCK, it.m0, it.set, bar);
+          else
+            for (int b = 0; b < 2; ++b) tma_box_3d(dst + b * (K_BLOCK * 128), map, it.m0 + b * 64, kb * K_BLOCK, it.set, bar);
+        }
+        __syncwarp();
+        r.advance();
+      }
     }
-    __syncthreads();
+  } else if (warp == WARP_MMA) {
+    // ================= the issuer =================================================================
+    Ring<STAGES> r;
+    Ring<2> acc;
+    // fp32 accumulator, fp16 or bf16 operands, M = 128
+    const uint32_t format = a.dtype == KEEPVQ_BF16 ? 1u : 0u;
+    const uint32_t idesc0 = (1u << 4) | (format << 7) | (format << 10) | (static_cast<uint32_t>(M_MN) << 15) | (static_cast<uint32_t>(N_MN) << 16) | ((M_TILE >> 4) << 24);
+    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      const Item it = item_at(i);
+      if (it.k_blocks == 0) continue;  // (an expert without routes: the epilogue writes zeros)
+      ok = wait_for(acc_empty + 8 * acc.index, acc.phase ^ 1u, deadline, aborted);
+      const uint32_t idesc = idesc0 | (static_cast<uint32_t>((it.n + N_STEP - 1) / N_STEP * N_STEP >> 3) << 17);
+      for (int kb = 0; kb < it.k_blocks && ok; ++kb) {
+        ok = wait_for(full + 8 * r.index, r.phase, deadline, aborted);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        const int steps = MODE == WEIGHT_GRAD ? min(4, (it.size - kb * K_BLOCK + N_STEP - 1) / N_STEP) : 4;  // of 16
+        if (elect_one()) {
+          const uint32_t stage = ring + r.index * S::STAGE_BYTES;
+          const uint64_t ad = operand_desc(stage, M_MN), bd = operand_desc(stage + S::A_BYTES, N_MN);
+          for (int k = 0; k < steps; ++k)  // 16 of the contraction: 32 bytes of a row, or 16 rows of 128
+            mma_16bit(tmem + acc.index * N_MAX, ad + k * (M_MN ? 128 : 2), bd + k * (N_MN ? 128 : 2), idesc, (kb | k) != 0);
+          mma_commit(empty + 8 * r.index);
+          if (kb == it.k_blocks - 1) mma_commit(acc_full + 8 * acc.index);
+        }
+        __syncwarp();
+        mma_issued = true;
+        r.advance();
+      }
+      acc.advance();
+    }
+  } else if (warp >= WARP_OUT) {
+    // ================= the epilogue ================================================================
+    const int quadrant = warp & 3;
+    const uint32_t lanes = tmem + (static_cast<uint32_t>(quadrant * 32) << 16);
+    uint16_t* piece = reinterpret_cast<uint16_t*>(smem_raw + (ring - smem_addr(smem_raw)) + STAGES * S::STAGE_BYTES) + quadrant * 32 * 32;  // [result row][32 values]
+    const bool whole = cols % 8 == 0;
+    Ring<2> acc;
+    if (MODE == FORWARD || (MODE == INPUT_GRAD && !a.route_dx)) {  // rows of dead routes
+      for (int64_t p = a.plan.offset[a.sets] + blockIdx.x * 4 + quadrant; p < a.routes; p += gridDim.x * 4) {
+        uint16_t* row = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(a.plan.order[p]) * cols;
+        if (whole)
+          for (int c = lane * 8; c < cols; c += 256) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+        else
+          for (int c = lane; c < cols; c += 32) row[c] = 0;
+      }
+    }
+    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+      const Item it = item_at(i);
+      if (it.k_blocks > 0) {
+        ok = wait_for(acc_full + 8 * acc.index, acc.phase, deadline, aborted);
+        if (!ok) break;
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+      }
+      const int col = it.m0 + quadrant * 32;
+      for (int c0 = 0; c0 < it.n; c0 += 32) {
+        uint32_t v[32];
+        if (it.k_blocks > 0) {
+          tmem_ld32(lanes + acc.index * N_MAX + c0, v);
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+        } else {
 #pragma unroll
-    for (int k = 0; k < STEP; ++k)
+          for (int j = 0; j < 32; ++j) v[j] = 0;
+        }
+        const int n = min(32, it.n - c0);
+        // the row that result row c0 + lane is
+        const int64_t row = lane >= n ? 0 : MODE == WEIGHT_GRAD ? it.set * a.out_dim + it.n0 + c0 + lane : a.plan.order[it.start + c0 + lane];
+        if (MODE == INPUT_GRAD && a.route_dx) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
+          for (int j = 0; j < 32; ++j) {
+            const int64_t to = __shfl_sync(0xFFFFFFFFu, static_cast<int>(row), j);
+            if (j < n && col + lane < cols) a.route_dx[to * cols + col + lane] = __uint_as_float(v[j]);
+          }
+          continue;
+        }
+        if (a.dtype == KEEPVQ_BF16) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) sum[i][j] += right[k][tr * 4 + i] * left[k][tc + 16 * j];
-    __syncthreads();
+          for (int j = 0; j < 32; ++j) piece[j * 32 + lane] = bits_of<__nv_bfloat16>(__uint_as_float(v[j]));
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) piece[j * 32 + lane] = bits_of<__half>(__uint_as_float(v[j]));
+        }
+        __syncwarp();
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {  // eight result rows of 64 bytes at a time
+          const int j = u * 8 + (lane >> 2), c = col + (lane & 3) * 8;
+          const int64_t to = __shfl_sync(0xFFFFFFFFu, row, j);
+          const uint4 eight = *reinterpret_cast<const uint4*>(piece + j * 32 + (lane & 3) * 8);
+          uint16_t* dst = static_cast<uint16_t*>(a.out) + to * cols + c;
+          if (j < n) {
+            if (whole) {
+              if (c < cols) *reinterpret_cast<uint4*>(dst) = eight;
+            } else {
+              const uint32_t pair[4] = {eight.x, eight.y, eight.z, eight.w};
+#pragma unroll
+              for (int d = 0; d < 8; ++d)
+                if (c + d < cols) dst[d] = static_cast<uint16_t>(pair[d >> 1] >> (16 * (d & 1)));
+            }
+          }
+        }
+        __syncwarp();
+      }
+      if (it.k_blocks > 0) {
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) mbar_arrive(acc_empty + 8 * acc.index);
+        acc.advance();
+      }
+    }
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t row = row0 + tr * 4 + i, col = col0 + tc + 16 * j;
-      if (row >= rows || col >= cols) continue;
-      if (MODE == FORWARD) store_from_float(a.out, a.dtype, plan.order[start + row] * a.out_dim + col, sum[i][j]);
-      else if (MODE == WEIGHT_GRAD) store_from_float(a.dweight, a.dtype, (set * a.out_dim + row) * a.in_dim + col, sum[i][j]);
-      else if (route_dx) route_dx[plan.order[start + row] * a.in_dim + col] = sum[i][j];
-      else store_from_float(a.dx, a.dtype, plan.order[start + row] * a.in_dim + col, sum[i][j]);
-    }
+
+  __syncthreads();  // every role has left its loop
+  if (*aborted) {
+    // What is in flight is waited for, bounded: the issuer's products by one more commit, copies by time.
+    if (tid == 0) atomicExch(a.plan.status, 1);
+    const uint64_t grace = global_timer_ns() + 20000000ull;
+    if (warp == WARP_MMA && mma_issued && elect_one()) mma_commit(acc_full);
+    while (global_timer_ns() < grace) __nanosleep(1000);
+  }
+  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+  __syncthreads();
+  if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLS) : "memory");
 }
+
+// ---- host ------------------------------------------------------------------------------------------
+
+// A tensor map of 16-bit values in this GPU's own memory: `sets` matrices [rows, width], boxes of 64 values
+// by box_rows rows of one of them (0: single rows, to be gathered).
+static int value_map(CUtensorMap* map, const void* base, int dtype, int64_t width, int64_t row_values, int64_t rows, int64_t sets, uint32_t box_rows) {
+  typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
+                                  CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static EncodeTiled encode = nullptr;
+  if (!encode) {
+    void* fn = nullptr;
+    cudaDriverEntryPointQueryResult found = cudaDriverEntryPointSymbolNotFound;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &found);
+    if (e != cudaSuccess) return note_cuda_error(e);
+    if (found != cudaDriverEntryPointSuccess || !fn) return KEEPVQ_ERR_UNSUPPORTED;
+    encode = reinterpret_cast<EncodeTiled>(fn);
+  }
+  const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(sets)};
+  const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_values * 2), static_cast<cuuint64_t>(row_values * 2 * rows)};
+  const cuuint32_t box[3] = {K_BLOCK, box_rows ? box_rows : 1, 1}, steps[3] = {1, 1, 1};
+  const CUresult r = encode(map, dtype == KEEPVQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, box_rows ? 3 : 2, const_cast<void*>(base), dims, strides, box,
+                            steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? KEEPVQ_OK : KEEPVQ_ERR_LAUNCH;
+}
+
+// Routes per tile: 64 leave room for twice the stages, which is what a call wants whose experts have few
+// routes each and whose time is reading the weights.
+static int tile_routes(int64_t routes, int64_t experts) { return routes <= 48 * experts ? 64 : 256; }
 
 struct Layout {
   Plan plan;
@@ -94,7 +395,7 @@ struct Layout {
 static Layout lay_out(void* base, int64_t routes, int64_t experts, int64_t in_dim, int x_div, bool grads) {
   Scratch s{static_cast<char*>(base)};
   Layout l;
-  l.plan = take_plan(s, routes, experts, TILE);
+  l.plan = take_plan(s, routes, experts, tile_routes(routes, experts));
   l.route_dx = grads && x_div > 1 ? s.take<float>(routes * in_dim) : nullptr;
   l.bytes = s.used;
   return l;
@@ -106,15 +407,33 @@ static int check_sizes(int64_t routes, int64_t experts, int64_t out_dim, int64_t
   return KEEPVQ_OK;
 }
 
+template <int MODE, int N_MAX>
+static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cudaStream_t s) {
+  using S = Shape<N_MAX>;
+  MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.routes, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan};
+  CUtensorMap m_map, n_map;
+  int rc = MODE == WEIGHT_GRAD ? value_map(&m_map, a.x, a.dtype, a.in_dim, a.in_dim, a.routes / a.x_div, 1, 0)
+                               : value_map(&m_map, a.weight, a.dtype, a.in_dim, a.in_dim, a.out_dim, a.experts, MODE == FORWARD ? M_TILE : K_BLOCK);
+  if (rc) return rc;
+  rc = MODE == FORWARD ? value_map(&n_map, a.x, a.dtype, a.in_dim, a.in_dim, a.routes / a.x_div, 1, 0) : value_map(&n_map, a.grad, a.dtype, a.out_dim, a.grad_ld, a.routes, 1, 0);
+  if (rc) return rc;
+  auto kernel = switch_matmul_kernel<MODE, N_MAX>;
+  static uint64_t configured = 0;  // one bit per device: the shared-memory opt-in is a per-device attribute of the function
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !((configured >> dev) & 1ull)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM_BYTES);
+    if (e != cudaSuccess) return note_cuda_error(e);
+    if (dev >= 0 && dev < 64) configured |= 1ull << dev;
+  }
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  const cudaError_t e = launch_after(true, kernel, sms, MM_THREADS, S::SMEM_BYTES, s, m, m_map, n_map);
+  return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
+}
 template <int MODE>
 static int launch(const keepvq_switch_matmul_args& a, const Layout& l, cudaStream_t s) {
-  auto blocks = [](int64_t n) { return static_cast<unsigned>((n + TILE - 1) / TILE); };
-  const dim3 grid = MODE == WEIGHT_GRAD ? dim3(blocks(a.in_dim), blocks(a.out_dim), static_cast<unsigned>(a.experts))
-                                        : dim3(static_cast<unsigned>(max_tiles(a.routes, a.experts, TILE) + 1), blocks(MODE == FORWARD ? a.out_dim : a.in_dim));
-  if (a.dtype == KEEPVQ_BF16) switch_matmul_kernel<__nv_bfloat16, MODE><<<grid, 256, 0, s>>>(a, l.plan, l.route_dx);
-  else switch_matmul_kernel<__half, MODE><<<grid, 256, 0, s>>>(a, l.plan, l.route_dx);
-  KEEPVQ_CHECK_LAUNCH();
-  return KEEPVQ_OK;
+  if (MODE != WEIGHT_GRAD && tile_routes(a.routes, a.experts) == 64) return launch_tiles<MODE, MODE == WEIGHT_GRAD ? 256 : 64>(a, l, s);
+  return launch_tiles<MODE, 256>(a, l, s);
 }
 
 static int check_call(const keepvq_switch_matmul_args& a, bool grads) {
@@ -148,7 +467,7 @@ int keepvq_switch_matmul(const keepvq_switch_matmul_args* args, void* stream) {
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   if (a.routes == 0) return KEEPVQ_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (const int rc = make_plan({a.indices, a.index_bits}, a.routes, a.experts, TILE, 16, l.plan, s)) return rc;
+  if (const int rc = make_plan({a.indices, a.index_bits}, a.routes, a.experts, tile_routes(a.routes, a.experts), N_STEP, l.plan, s)) return rc;
   return launch<FORWARD>(a, l, s);
 }
 
@@ -160,13 +479,13 @@ int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stre
   const Layout l = lay_out(a.workspace, a.routes, a.experts, a.in_dim, a.x_div, true);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (a.routes == 0) {
+    const cudaError_t e = a.dweight ? cudaMemsetAsync(a.dweight, 0, a.experts * a.out_dim * a.in_dim * 2, s) : cudaSuccess;
+    return e == cudaSuccess ? KEEPVQ_OK : keepvq::note_cuda_error(e);
+  }
   const Indices indices{a.indices, a.index_bits};
-  if (const int rc = make_plan(indices, a.routes, a.experts, TILE, 16, l.plan, s)) return rc;
-  if (a.dx && a.routes > 0) {
-    if (!l.route_dx) {  // a dead route's row
-      const cudaError_t e = cudaMemsetAsync(a.dx, 0, a.routes * a.in_dim * 2, s);
-      if (e != cudaSuccess) return keepvq::note_cuda_error(e);
-    }
+  if (const int rc = make_plan(indices, a.routes, a.experts, tile_routes(a.routes, a.experts), N_STEP, l.plan, s)) return rc;
+  if (a.dx) {
     if (const int rc = launch<INPUT_GRAD>(a, l, s)) return rc;
     if (l.route_dx)
       if (const int rc = sum_picks(l.route_dx, indices, a.experts, a.routes / a.x_div, a.x_div, a.in_dim, a.dx, a.dtype, s)) return rc;
