@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(256) factor_grad_kernel(const void* v, int64_t
   if (i >= wide * rank) return;
   const int64_t n = ACROSS ? i / rank : i % wide, j = ACROSS ? i % rank : i / wide;
   float sum = 0.0f;
-  for (int p = plan.offset[e]; p < plan.offset[e + 1]; ++p) {
+  for (int p = plan.offset[e]; p < plan.offset[e] + plan.count[e]; ++p) {
     const int64_t r = plan.order[p];
     sum += inner[r * rank + j] * load_as_float(v, dtype, r / x_div * ld + n);
   }

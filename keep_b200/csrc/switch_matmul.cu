@@ -15,8 +15,12 @@
 //   dx       W[e] columns     (MN-major box)      grad rows, gathered  (K-major)       out_dim
 //   dweight  x columns, rows gathered (MN-major)  grad columns, rows gathered (MN-major)  e's routes
 //
-// The rows of a set are wherever the caller has them: TMA gathers four at a time by their index, and
-// fills rows past the end of a matrix with zeros (the ragged end of a set's routes in dweight).
+// Two forms:
+//   FEW   few routes per set, the time is reading weights: one CTA per tile, up to 64 result rows, the
+//         set's rows gathered by TMA, four at a time by their index, straight from the caller's matrix
+//   MANY  two CTAs (of one TPC) per tile of 256 x 256, whose tensor cores work as one: each loads half of
+//         both operands.  TMA's row gather is too slow here (about 80 cycles for four rows, measured: 229
+//         TFLOP/s at 768 routes a set), so rows are first copied into the sets' order
 #include "async_copy.cuh"
 #include "switch_plan.cuh"
 
@@ -31,30 +35,76 @@ using fast::mbar_init;
 using fast::smem_addr;
 
 enum { FORWARD = 0, INPUT_GRAD = 1, WEIGHT_GRAD = 2 };
-constexpr int M_TILE = 128, K_BLOCK = 64, N_STEP = 16;  // K_BLOCK: 128 bytes, a swizzled row
+constexpr int M_TILE = 128, K_BLOCK = 64, N_STEP = 16, BOX_ROWS = 32;  // M_TILE: of a CTA.  // K_BLOCK: 128 bytes, a swizzled row
 constexpr int MM_THREADS = 256;
 enum { WARP_M = 0, WARP_N = 1, WARP_MMA = 2, WARP_OUT = 4 };  // loaders of the two operands, the issuer, four warps of the epilogue
 constexpr uint64_t MM_WAIT_NS = 2000000000ull;
 
 // ---- instructions ---------------------------------------------------------------------------------
+// PAIR: the barrier may be the first CTA's, the copy's target is this CTA's.
+template <bool PAIR>
 __device__ __forceinline__ void tma_box_3d(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t bar) {
-  asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
-               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+  if (PAIR) asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4}], [%5];"
+                         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
+  else asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+                    ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 // Four rows of a matrix, 128 bytes of each from column x on.  The map's box is one row high.
 __device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* map, int32_t x, const int4& rows, uint32_t bar) {
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar) : "memory");
 }
+template <bool PAIR>
 __device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-               "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-               ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+  if (PAIR) asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                         ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
+  else asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                    "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                    ::"r"(d_tmem), "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
 }
+// An arrival, when the products issued so far are done, on this barrier (of both CTAs of a pair).
+template <bool PAIR>
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+  if (PAIR) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"(static_cast<uint16_t>(3)) : "memory");
+  else asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ uint32_t cluster_rank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ uint32_t of_first_cta(uint32_t addr) {
+  uint32_t mapped;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(mapped) : "r"(addr));
+  return mapped;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
+}
+// PAIR: the barrier may be the other CTA's.  (Nothing but the copies themselves is ordered by this arrival;
+// with .release.cluster it cost more than a K block's products.)
+template <bool PAIR>
+__device__ __forceinline__ void expect_bytes(uint32_t bar, uint32_t bytes) {
+  if (PAIR) asm volatile("mbarrier.arrive.expect_tx.relaxed.cluster.shared::cluster.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  else mbar_expect_tx(bar, bytes);
+}
+__device__ __forceinline__ void arrive_cluster(uint32_t bar) { asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory"); }
+template <bool PAIR>
+__device__ __forceinline__ void tmem_alloc(uint32_t slot, uint32_t columns) {
+  if (PAIR) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  } else {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(columns) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
+  if (PAIR) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+  else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
+}
 // 32 columns of this thread's lane of tensor memory.
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
   asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -91,10 +141,12 @@ struct Ring {
   }
 };
 
-template <int N_MAX>
+template <bool MANY>
 struct Shape {
-  static constexpr uint32_t A_BYTES = M_TILE * K_BLOCK * 2, B_BYTES = N_MAX * K_BLOCK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
-  static constexpr uint32_t STAGES = 192 * 1024 / STAGE_BYTES;  // 4 or 8: as many weights in flight either way
+  static constexpr int N_MAX = MANY ? 256 : 64, N_CTA = MANY ? 128 : 64;  // result rows of a tile; of its N operand in a CTA
+  static constexpr int PAD = MANY ? 32 : N_STEP;                           // what the number of result rows is rounded up to
+  static constexpr uint32_t A_BYTES = M_TILE * K_BLOCK * 2, STAGE_BYTES = A_BYTES + N_CTA * K_BLOCK * 2;
+  static constexpr uint32_t STAGES = 192 * 1024 / STAGE_BYTES;  // 6 or 8
   static constexpr uint32_t OUT_BYTES = 4 * 32 * 32 * 2;        // a 32 x 32 piece of the result for each warp of the epilogue
   static constexpr uint32_t SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + OUT_BYTES;
   static constexpr uint32_t TMEM_COLS = 2 * N_MAX;              // two accumulators: one is written while the other is drained
@@ -115,60 +167,66 @@ __device__ __forceinline__ uint16_t bits_of<__half>(float v) { return __half_as_
 template <>
 __device__ __forceinline__ uint16_t bits_of<__nv_bfloat16>(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
 
-// One tile of the result.
+// One tile of the result, or a CTA's half of it.
 struct Item {
-  int set, start, size;  // size: routes (the N operand's rows, or the contraction of dweight)
+  int set, start, size;  // size: routes (the N operand's rows, or the contraction of dweight); start: their first place
   int m0, n0;            // first value along a result's row; first result row (dweight)
-  int n;                 // result rows
+  int n, n_pad;          // result rows; rounded up
   int k_blocks;
 };
 
-template <int MODE, int N_MAX>
+template <int MODE, bool MANY>
 __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs a, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map) {
-  using S = Shape<N_MAX>;
+  using S = Shape<MANY>;
+  static_assert(MANY || MODE != WEIGHT_GRAD, "the rows of dweight's operands are copied first");
   constexpr uint32_t STAGES = S::STAGES;
   constexpr bool M_MN = MODE != FORWARD, N_MN = MODE == WEIGHT_GRAD;
+  constexpr int CTAS = MANY ? 2 : 1, N_MAX = S::N_MAX;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t bars[2 * STAGES + 4];
   __shared__ uint32_t tmem_slot;
   __shared__ int abort_flag;
-  grid_launch_dependents();
+  // MANY neither starts early nor lets its successor: blocks that wait on the SMs for a grid of full-sized
+  // clusters can keep the last of those clusters from being placed, and then both wait for good
+  if (!MANY) grid_launch_dependents();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int rank = MANY ? static_cast<int>(cluster_rank()) : 0;  // in the pair; the first CTA issues for both
   const uint32_t ring = (smem_addr(smem_raw) + 1023u) & ~1023u;
   const uint32_t full = smem_addr(bars), empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16;
   if (tid == 0) {
     abort_flag = 0;
-    for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 2); mbar_init(empty + 8 * s, 1); }
-    for (uint32_t s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4); }
+    for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 2 * CTAS); mbar_init(empty + 8 * s, 1); }
+    for (uint32_t s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4 * CTAS); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == WARP_MMA) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)), "r"(S::TMEM_COLS) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-  }
+  if (warp == WARP_MMA) tmem_alloc<MANY>(smem_addr(&tmem_slot), S::TMEM_COLS);
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
+  if (MANY) cluster_sync();
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
-  grid_wait();
+  if (!MANY) grid_wait();
   const uint64_t deadline = global_timer_ns() + MM_WAIT_NS;
   volatile int* aborted = &abort_flag;
+  // the first CTA's barriers that both CTAs of a pair arrive on
+  const uint32_t full0 = MANY ? of_first_cta(full) : full, acc_empty0 = MANY ? of_first_cta(acc_empty) : acc_empty;
 
   const int cols = static_cast<int>(MODE == FORWARD ? a.out_dim : a.in_dim);  // of a result row
-  const int m_tiles = (cols + M_TILE - 1) / M_TILE;
+  const int m_tiles = (cols + CTAS * M_TILE - 1) / (CTAS * M_TILE);
   const int n_tiles = MODE == WEIGHT_GRAD ? static_cast<int>((a.out_dim + N_MAX - 1) / N_MAX) : 0;
   const int depth_blocks = static_cast<int>(((MODE == FORWARD ? a.in_dim : a.out_dim) + K_BLOCK - 1) / K_BLOCK);
   const int64_t items = static_cast<int64_t>(m_tiles) * (MODE == WEIGHT_GRAD ? static_cast<int64_t>(n_tiles) * a.sets : *a.plan.tiles);
+  const int first_item = blockIdx.x / CTAS, item_step = gridDim.x / CTAS;
   // Every role walks the same items on its own clock.
   auto item_at = [&](int64_t i) {
     Item it;
     const int64_t outer = i / m_tiles;
-    it.m0 = static_cast<int>(i - outer * m_tiles) * M_TILE;
+    it.m0 = (static_cast<int>(i - outer * m_tiles) * CTAS + rank) * M_TILE;
     if (MODE == WEIGHT_GRAD) {
       it.set = static_cast<int>(outer / n_tiles);
       it.n0 = static_cast<int>(outer - static_cast<int64_t>(it.set) * n_tiles) * N_MAX;
       it.start = a.plan.offset[it.set];
-      it.size = a.plan.offset[it.set + 1] - it.start;
+      it.size = a.plan.count[it.set];
       it.n = min(N_MAX, static_cast<int>(a.out_dim) - it.n0);
       it.k_blocks = (it.size + K_BLOCK - 1) / K_BLOCK;
     } else {
@@ -178,6 +236,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
       it.n = it.size;
       it.k_blocks = depth_blocks;
     }
+    it.n_pad = (it.n + S::PAD - 1) / S::PAD * S::PAD;
     return it;
   };
   bool ok = true, mma_issued = false;
@@ -187,78 +246,67 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     Ring<STAGES> r;
     const uint32_t tile = ring + (warp == WARP_N ? S::A_BYTES : 0);
     const CUtensorMap* map = warp == WARP_M ? &m_map : &n_map;
-    const int rows_end = static_cast<int>(MODE == WEIGHT_GRAD && warp == WARP_M ? a.routes / a.x_div : a.routes);  // of the gathered matrix: zeros from here on
-    const int div = (MODE == FORWARD && warp == WARP_N) || (MODE == WEIGHT_GRAD && warp == WARP_M) ? a.x_div : 1;
-    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+    for (int64_t i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
-      auto row_at = [&](int p) { return a.plan.order[it.start + p] / div; };
-      int4 rows[2];
-      if (MODE != WEIGHT_GRAD && warp == WARP_N) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {  // rows past the last route repeat it: nobody looks at their columns
-          const int q = (u * 32 + lane) * 4, last = it.size - 1;
-          if (q < it.size) rows[u] = make_int4(row_at(q), row_at(min(q + 1, last)), row_at(min(q + 2, last)), row_at(min(q + 3, last)));
-        }
+      const int half = it.n_pad / CTAS;  // of the N operand, in this CTA
+      int4 rows;
+      if (!MANY && warp == WARP_N && lane * 4 < it.size) {  // rows past the last route repeat it: nobody looks at their columns
+        const int div = MODE == FORWARD ? a.x_div : 1, last = it.size - 1, q = lane * 4;
+        auto row_at = [&](int p) { return a.plan.order[it.start + min(p, last)] / div; };
+        rows = make_int4(row_at(q), row_at(q + 1), row_at(q + 2), row_at(q + 3));
       }
       for (int kb = 0; kb < it.k_blocks; ++kb) {
-        int steps = 0;
-        if (MODE == WEIGHT_GRAD) {  // 16 quads of rows, two lanes each
-          const int first = kb * K_BLOCK, q = first + (lane & 15) * 4;
-          steps = min(K_BLOCK, (it.size - first + N_STEP - 1) / N_STEP * N_STEP);
-          auto row_or_end = [&](int p) { return p < it.size ? row_at(p) : rows_end; };
-          rows[0] = make_int4(row_or_end(q), row_or_end(q + 1), row_or_end(q + 2), row_or_end(q + 3));
-        }
         ok = wait_for(empty + 8 * r.index, r.phase ^ 1u, deadline, aborted);
         if (!ok) break;
-        const uint32_t bar = full + 8 * r.index, dst = tile + r.index * S::STAGE_BYTES;
-        if (MODE == WEIGHT_GRAD) {
-          const int width = warp == WARP_M ? M_TILE : it.n, col0 = warp == WARP_M ? it.m0 : it.n0, boxes = (width + 63) / 64;
-          if (lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>(boxes * steps * 128));
+        const uint32_t bar = full0 + 8 * r.index, dst = tile + r.index * S::STAGE_BYTES;
+        if (!MANY && warp == WARP_N) {
+          if (lane == 0) expect_bytes<MANY>(bar, static_cast<uint32_t>((it.size + 3) / 4 * 512));
           __syncwarp();
-          if ((lane & 15) * 4 < steps)
-            for (int b = lane >> 4; b < boxes; b += 2) tma_rows4(dst + b * (K_BLOCK * 128) + (lane & 15) * 512, map, col0 + b * 64, rows[0], bar);
-        } else if (warp == WARP_N) {
-          if (lane == 0) mbar_expect_tx(bar, static_cast<uint32_t>((it.size + 3) / 4 * 512));
-          __syncwarp();
-#pragma unroll
-          for (int u = 0; u < (N_MAX > 128 ? 2 : 1); ++u) {
-            const int q = u * 32 + lane;
-            if (q * 4 < it.size) tma_rows4(dst + q * 512, map, kb * K_BLOCK, rows[u], bar);
-          }
+          if (lane * 4 < it.size) tma_rows4(dst + lane * 512, map, kb * K_BLOCK, rows, bar);
         } else if (elect_one()) {
-          mbar_expect_tx(bar, S::A_BYTES);
-          if (MODE == FORWARD) tma_box_3d(dst, map, kb * K_BLOCK, it.m0, it.set, bar);
-          else
-            for (int b = 0; b < 2; ++b) tma_box_3d(dst + b * (K_BLOCK * 128), map, it.m0 + b * 64, kb * K_BLOCK, it.set, bar);
+          if (MODE == WEIGHT_GRAD) {  // 64 places of the set's routes (those behind the last are not multiplied) by 64 columns
+            const int boxes = warp == WARP_M ? 2 : (half + 63) / 64, col0 = warp == WARP_M ? it.m0 : it.n0 + rank * half;
+            expect_bytes<MANY>(bar, static_cast<uint32_t>(boxes * (K_BLOCK * 128)));
+            for (int b = 0; b < boxes; ++b) tma_box_3d<MANY>(dst + b * (K_BLOCK * 128), map, col0 + b * 64, it.start + kb * K_BLOCK, 0, bar);
+          } else if (warp == WARP_N) {
+            const int boxes = (half + BOX_ROWS - 1) / BOX_ROWS;  // (rows behind the tile's: nobody looks at their columns)
+            expect_bytes<MANY>(bar, static_cast<uint32_t>(boxes * (BOX_ROWS * 128)));
+            for (int b = 0; b < boxes; ++b) tma_box_3d<MANY>(dst + b * (BOX_ROWS * 128), map, kb * K_BLOCK, it.start + rank * half + b * BOX_ROWS, 0, bar);
+          } else {
+            expect_bytes<MANY>(bar, S::A_BYTES);
+            if (MODE == FORWARD) tma_box_3d<MANY>(dst, map, kb * K_BLOCK, it.m0, it.set, bar);
+            else
+              for (int b = 0; b < 2; ++b) tma_box_3d<MANY>(dst + b * (K_BLOCK * 128), map, it.m0 + b * 64, kb * K_BLOCK, it.set, bar);
+          }
         }
         __syncwarp();
         r.advance();
       }
     }
-  } else if (warp == WARP_MMA) {
+  } else if (warp == WARP_MMA && rank == 0) {
     // ================= the issuer =================================================================
     Ring<STAGES> r;
     Ring<2> acc;
-    // fp32 accumulator, fp16 or bf16 operands, M = 128
+    // fp32 accumulator, fp16 or bf16 operands
     const uint32_t format = a.dtype == KEEPVQ_BF16 ? 1u : 0u;
-    const uint32_t idesc0 = (1u << 4) | (format << 7) | (format << 10) | (static_cast<uint32_t>(M_MN) << 15) | (static_cast<uint32_t>(N_MN) << 16) | ((M_TILE >> 4) << 24);
-    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+    const uint32_t idesc0 = (1u << 4) | (format << 7) | (format << 10) | (static_cast<uint32_t>(M_MN) << 15) | (static_cast<uint32_t>(N_MN) << 16) | ((CTAS * M_TILE >> 4) << 24);
+    for (int64_t i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks == 0) continue;  // (an expert without routes: the epilogue writes zeros)
       ok = wait_for(acc_empty + 8 * acc.index, acc.phase ^ 1u, deadline, aborted);
-      const uint32_t idesc = idesc0 | (static_cast<uint32_t>((it.n + N_STEP - 1) / N_STEP * N_STEP >> 3) << 17);
+      const uint32_t idesc = idesc0 | (static_cast<uint32_t>(it.n_pad >> 3) << 17);
       for (int kb = 0; kb < it.k_blocks && ok; ++kb) {
         ok = wait_for(full + 8 * r.index, r.phase, deadline, aborted);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        const int steps = MODE == WEIGHT_GRAD ? min(4, (it.size - kb * K_BLOCK + N_STEP - 1) / N_STEP) : 4;  // of 16
+        const int steps = MODE == WEIGHT_GRAD ? min(4, (it.size - kb * K_BLOCK + ROW_STEP - 1) / ROW_STEP) : 4;  // of 16
         if (elect_one()) {
           const uint32_t stage = ring + r.index * S::STAGE_BYTES;
           const uint64_t ad = operand_desc(stage, M_MN), bd = operand_desc(stage + S::A_BYTES, N_MN);
           for (int k = 0; k < steps; ++k)  // 16 of the contraction: 32 bytes of a row, or 16 rows of 128
-            mma_16bit(tmem + acc.index * N_MAX, ad + k * (M_MN ? 128 : 2), bd + k * (N_MN ? 128 : 2), idesc, (kb | k) != 0);
-          mma_commit(empty + 8 * r.index);
-          if (kb == it.k_blocks - 1) mma_commit(acc_full + 8 * acc.index);
+            mma_16bit<MANY>(tmem + acc.index * N_MAX, ad + k * (M_MN ? 128 : 2), bd + k * (N_MN ? 128 : 2), idesc, (kb | k) != 0);
+          mma_commit<MANY>(empty + 8 * r.index);
+          if (kb == it.k_blocks - 1) mma_commit<MANY>(acc_full + 8 * acc.index);
         }
         __syncwarp();
         mma_issued = true;
@@ -274,15 +322,15 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     const bool whole = cols % 8 == 0;
     Ring<2> acc;
     if (MODE == FORWARD || (MODE == INPUT_GRAD && !a.route_dx)) {  // rows of dead routes
-      for (int64_t p = a.plan.offset[a.sets] + blockIdx.x * 4 + quadrant; p < a.routes; p += gridDim.x * 4) {
-        uint16_t* row = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(a.plan.order[p]) * cols;
+      for (int64_t p = blockIdx.x * 4 + quadrant; p < *a.plan.dead_count; p += gridDim.x * 4) {
+        uint16_t* row = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(a.plan.dead[p]) * cols;
         if (whole)
           for (int c = lane * 8; c < cols; c += 256) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
         else
           for (int c = lane; c < cols; c += 32) row[c] = 0;
       }
     }
-    for (int64_t i = blockIdx.x; i < items && ok; i += gridDim.x) {
+    for (int64_t i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks > 0) {
         ok = wait_for(acc_full + 8 * acc.index, acc.phase, deadline, aborted);
@@ -340,7 +388,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
       if (it.k_blocks > 0) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
-        if (lane == 0) mbar_arrive(acc_empty + 8 * acc.index);
+        if (lane == 0) arrive_cluster(acc_empty0 + 8 * acc.index);
         acc.advance();
       }
     }
@@ -351,12 +399,13 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     // What is in flight is waited for, bounded: the issuer's products by one more commit, copies by time.
     if (tid == 0) atomicExch(a.plan.status, 1);
     const uint64_t grace = global_timer_ns() + 20000000ull;
-    if (warp == WARP_MMA && mma_issued && elect_one()) mma_commit(acc_full);
+    if (warp == WARP_MMA && mma_issued && elect_one()) mma_commit<MANY>(acc_full);
     while (global_timer_ns() < grace) __nanosleep(1000);
   }
   asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
   __syncthreads();
-  if (warp == WARP_MMA) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(S::TMEM_COLS) : "memory");
+  if (MANY) cluster_sync();  // nobody arrives here, and nothing reads this CTA's memory, any more
+  if (warp == WARP_MMA) tmem_free<MANY>(tmem, S::TMEM_COLS);
 }
 
 // ---- host ------------------------------------------------------------------------------------------
@@ -383,19 +432,24 @@ static int value_map(CUtensorMap* map, const void* base, int dtype, int64_t widt
   return r == CUDA_SUCCESS ? KEEPVQ_OK : KEEPVQ_ERR_LAUNCH;
 }
 
-// Routes per tile: 64 leave room for twice the stages, which is what a call wants whose experts have few
-// routes each and whose time is reading the weights.
-static int tile_routes(int64_t routes, int64_t experts) { return routes <= 48 * experts ? 64 : 256; }
+// FEW reads the weights as fast as they come up to some 32 routes per expert; what MANY takes beside that,
+// copying the rows into the experts' order, is two bytes in and out per value of a route.
+static bool many_routes(int64_t routes, int64_t experts) { return routes > 16 * experts && routes >= 256; }
 
 struct Layout {
   Plan plan;
-  float* route_dx;  // [routes, in_dim], where a row has several picks
+  uint16_t *x, *grad;  // rows in the plan's order (MANY)
+  float* route_dx;     // [routes, in_dim], where a row has several picks
   int64_t bytes;
 };
-static Layout lay_out(void* base, int64_t routes, int64_t experts, int64_t in_dim, int x_div, bool grads) {
+static Layout lay_out(void* base, int64_t routes, int64_t experts, int64_t out_dim, int64_t in_dim, int x_div, bool grads) {
   Scratch s{static_cast<char*>(base)};
+  const bool many = many_routes(routes, experts);
+  const int64_t places = max_places(routes, experts);
   Layout l;
-  l.plan = take_plan(s, routes, experts, tile_routes(routes, experts));
+  l.plan = take_plan(s, routes, experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX);
+  l.x = many || grads ? s.take<uint16_t>(places * in_dim) : nullptr;
+  l.grad = grads ? s.take<uint16_t>(places * align_up(out_dim, 8)) : nullptr;
   l.route_dx = grads && x_div > 1 ? s.take<float>(routes * in_dim) : nullptr;
   l.bytes = s.used;
   return l;
@@ -407,17 +461,20 @@ static int check_sizes(int64_t routes, int64_t experts, int64_t out_dim, int64_t
   return KEEPVQ_OK;
 }
 
-template <int MODE, int N_MAX>
+template <int MODE, bool MANY>
 static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cudaStream_t s) {
-  using S = Shape<N_MAX>;
+  using S = Shape<MANY>;
   MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.routes, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan};
+  const int64_t places = max_places(a.routes, a.experts), grad_ld = MANY ? align_up(a.out_dim, 8) : a.grad_ld;
   CUtensorMap m_map, n_map;
-  int rc = MODE == WEIGHT_GRAD ? value_map(&m_map, a.x, a.dtype, a.in_dim, a.in_dim, a.routes / a.x_div, 1, 0)
+  int rc = MODE == WEIGHT_GRAD ? value_map(&m_map, l.x, a.dtype, a.in_dim, a.in_dim, places, 1, K_BLOCK)
                                : value_map(&m_map, a.weight, a.dtype, a.in_dim, a.in_dim, a.out_dim, a.experts, MODE == FORWARD ? M_TILE : K_BLOCK);
   if (rc) return rc;
-  rc = MODE == FORWARD ? value_map(&n_map, a.x, a.dtype, a.in_dim, a.in_dim, a.routes / a.x_div, 1, 0) : value_map(&n_map, a.grad, a.dtype, a.out_dim, a.grad_ld, a.routes, 1, 0);
+  const uint32_t box = MODE == WEIGHT_GRAD ? K_BLOCK : MANY ? BOX_ROWS : 0;
+  rc = MODE == FORWARD ? value_map(&n_map, MANY ? l.x : a.x, a.dtype, a.in_dim, a.in_dim, MANY ? places : a.routes / a.x_div, 1, box)
+                       : value_map(&n_map, MANY ? l.grad : a.grad, a.dtype, a.out_dim, grad_ld, MANY ? places : a.routes, 1, box);
   if (rc) return rc;
-  auto kernel = switch_matmul_kernel<MODE, N_MAX>;
+  auto kernel = switch_matmul_kernel<MODE, MANY>;
   static uint64_t configured = 0;  // one bit per device: the shared-memory opt-in is a per-device attribute of the function
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -427,13 +484,24 @@ static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cud
     if (dev >= 0 && dev < 64) configured |= 1ull << dev;
   }
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  const cudaError_t e = launch_after(true, kernel, sms, MM_THREADS, S::SMEM_BYTES, s, m, m_map, n_map);
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(MANY ? sms / 2 * 2 : sms);
+  config.blockDim = dim3(MM_THREADS);
+  config.dynamicSmemBytes = S::SMEM_BYTES;
+  config.stream = s;
+  cudaLaunchAttribute attribute = {};
+  if (MANY) {
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = 2;
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  } else {
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+  }
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, m, m_map, n_map);
   return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
-}
-template <int MODE>
-static int launch(const keepvq_switch_matmul_args& a, const Layout& l, cudaStream_t s) {
-  if (MODE != WEIGHT_GRAD && tile_routes(a.routes, a.experts) == 64) return launch_tiles<MODE, MODE == WEIGHT_GRAD ? 256 : 64>(a, l, s);
-  return launch_tiles<MODE, 256>(a, l, s);
 }
 
 static int check_call(const keepvq_switch_matmul_args& a, bool grads) {
@@ -455,7 +523,7 @@ extern "C" {
 int64_t keepvq_switch_matmul_workspace_bytes(int64_t routes, int64_t experts, int64_t out_dim, int64_t in_dim, int32_t x_div, int32_t grads) {
   using namespace keepvq::dense;
   if (const int rc = check_sizes(routes, experts, out_dim, in_dim, x_div)) return rc;
-  return lay_out(nullptr, routes, experts, in_dim, x_div, grads != 0).bytes;
+  return lay_out(nullptr, routes, experts, out_dim, in_dim, x_div, grads != 0).bytes;
 }
 
 int keepvq_switch_matmul(const keepvq_switch_matmul_args* args, void* stream) {
@@ -463,12 +531,16 @@ int keepvq_switch_matmul(const keepvq_switch_matmul_args* args, void* stream) {
   if (!args) return KEEPVQ_ERR_NULL;
   const keepvq_switch_matmul_args& a = *args;
   if (const int rc = check_call(a, false)) return rc;
-  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.in_dim, a.x_div, false);
+  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.out_dim, a.in_dim, a.x_div, false);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   if (a.routes == 0) return KEEPVQ_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (const int rc = make_plan({a.indices, a.index_bits}, a.routes, a.experts, tile_routes(a.routes, a.experts), N_STEP, l.plan, s)) return rc;
-  return launch<FORWARD>(a, l, s);
+  const bool many = many_routes(a.routes, a.experts);
+  if (const int rc = make_plan({a.indices, a.index_bits}, a.routes, a.experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX, many ? Shape<true>::PAD : N_STEP, l.plan, s)) return rc;
+  if (!many) return launch_tiles<FORWARD, false>(a, l, s);
+  const RowCopy x{a.x, l.x, a.in_dim, a.in_dim, a.x_div};
+  if (const int rc = copy_rows(&x, 1, a.routes, a.experts, l.plan, s)) return rc;
+  return launch_tiles<FORWARD, true>(a, l, s);
 }
 
 int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stream) {
@@ -476,7 +548,7 @@ int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stre
   if (!args) return KEEPVQ_ERR_NULL;
   const keepvq_switch_matmul_args& a = *args;
   if (const int rc = check_call(a, true)) return rc;
-  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.in_dim, a.x_div, true);
+  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.out_dim, a.in_dim, a.x_div, true);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.routes == 0) {
@@ -484,13 +556,17 @@ int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stre
     return e == cudaSuccess ? KEEPVQ_OK : keepvq::note_cuda_error(e);
   }
   const Indices indices{a.indices, a.index_bits};
-  if (const int rc = make_plan(indices, a.routes, a.experts, tile_routes(a.routes, a.experts), N_STEP, l.plan, s)) return rc;
+  const bool many = many_routes(a.routes, a.experts);
+  if (const int rc = make_plan(indices, a.routes, a.experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX, many ? Shape<true>::PAD : N_STEP, l.plan, s)) return rc;
+  const RowCopy copies[2] = {{a.grad, l.grad, a.grad_ld, align_up(a.out_dim, 8), 1}, {a.x, l.x, a.in_dim, a.in_dim, a.x_div}};
+  if (many || a.dweight)
+    if (const int rc = copy_rows(copies, a.dweight ? 2 : 1, a.routes, a.experts, l.plan, s)) return rc;
   if (a.dx) {
-    if (const int rc = launch<INPUT_GRAD>(a, l, s)) return rc;
+    if (const int rc = many ? launch_tiles<INPUT_GRAD, true>(a, l, s) : launch_tiles<INPUT_GRAD, false>(a, l, s)) return rc;
     if (l.route_dx)
       if (const int rc = sum_picks(l.route_dx, indices, a.experts, a.routes / a.x_div, a.x_div, a.in_dim, a.dx, a.dtype, s)) return rc;
   }
-  return a.dweight ? launch<WEIGHT_GRAD>(a, l, s) : KEEPVQ_OK;
+  return a.dweight ? launch_tiles<WEIGHT_GRAD, true>(a, l, s) : KEEPVQ_OK;
 }
 
 }  // extern "C"

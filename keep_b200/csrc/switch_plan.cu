@@ -9,13 +9,14 @@ namespace dense {
 // per warp) starts; the warp then walks the routes once more and keeps its own in their order.  A
 // sort would need several launches or atomics that leave an order of their own.
 constexpr int PLAN_THREADS = 256, PLAN_WARPS = PLAN_THREADS / 32;
+constexpr unsigned PLAN_EARLY_BLOCKS = 148;  // more of them would crowd the SMs while they wait for their predecessor
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(Indices indices, int routes, int sets, int tile_routes, int tile_step, Plan plan) {
   grid_launch_dependents();
   grid_wait();
   extern __shared__ int32_t count[];  // [sets]
-  __shared__ int warp_routes[PLAN_WARPS], warp_tiles[PLAN_WARPS];
-  __shared__ int own_offset[PLAN_WARPS], own_tile[PLAN_WARPS], own_count[PLAN_WARPS];
+  __shared__ int warp_sums[3][PLAN_WARPS];
+  __shared__ int own_place[PLAN_WARPS], own_tile[PLAN_WARPS], own_count[PLAN_WARPS];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   for (int e = tid; e < sets; e += PLAN_THREADS) count[e] = 0;
   if (tid < PLAN_WARPS) own_count[tid] = 0;
@@ -25,52 +26,59 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(Indices indices, int
     if (e >= 0) atomicAdd(&count[e], 1);
   }
   __syncthreads();
-  // exclusive scan over the sets; a thread has a contiguous run of them
+  // exclusive scans over the sets of (routes, places, tiles); a thread has a contiguous run of them
+  auto places_of = [](int n) { return (n + ROW_STEP - 1) / ROW_STEP * ROW_STEP; };
+  auto tiles_of = [&](int n) { return (n + tile_routes - 1) / tile_routes; };
   const int run = (sets + PLAN_THREADS - 1) / PLAN_THREADS, first = min(sets, tid * run), last = min(sets, first + run);
-  int n = 0, t = 0;
-  for (int e = first; e < last; ++e) { n += count[e]; t += (count[e] + tile_routes - 1) / tile_routes; }
-  int n_scan = n, t_scan = t;
-  for (int d = 1; d < 32; d <<= 1) {
-    const int a = __shfl_up_sync(0xFFFFFFFFu, n_scan, d), b = __shfl_up_sync(0xFFFFFFFFu, t_scan, d);
-    if (lane >= d) { n_scan += a; t_scan += b; }
+  int own[3] = {}, before[3], total[3] = {};
+  for (int e = first; e < last; ++e) { own[0] += count[e]; own[1] += places_of(count[e]); own[2] += tiles_of(count[e]); }
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    int scan = own[k];
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xFFFFFFFFu, scan, d);
+      if (lane >= d) scan += v;
+    }
+    if (lane == 31) warp_sums[k][warp] = scan;
+    before[k] = scan - own[k];
   }
-  if (lane == 31) { warp_routes[warp] = n_scan; warp_tiles[warp] = t_scan; }
   __syncthreads();
-  int n_before = n_scan - n, t_before = t_scan - t, live = 0, tiles = 0;
-  for (int w = 0; w < PLAN_WARPS; ++w) {
-    if (w < warp) { n_before += warp_routes[w]; t_before += warp_tiles[w]; }
-    live += warp_routes[w];
-    tiles += warp_tiles[w];
-  }
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+    for (int w = 0; w < PLAN_WARPS; ++w) {
+      if (w < warp) before[k] += warp_sums[k][w];
+      total[k] += warp_sums[k][w];
+    }
   const int own0 = blockIdx.x * PLAN_WARPS;
   for (int e = first; e < last; ++e) {
     if (e >= own0 && e < own0 + PLAN_WARPS) {
-      own_offset[e - own0] = n_before;
-      own_tile[e - own0] = t_before;
-      own_count[e - own0] = count[e];
-      plan.offset[e] = n_before;
+      own_place[e - own0] = plan.offset[e] = before[1];
+      own_count[e - own0] = plan.count[e] = count[e];
+      own_tile[e - own0] = before[2];
     }
-    n_before += count[e];
-    t_before += (count[e] + tile_routes - 1) / tile_routes;
+    before[1] += places_of(count[e]);
+    before[2] += tiles_of(count[e]);
   }
+  const int dead = routes - total[0];
   if (blockIdx.x == 0 && tid == 0) {
     *plan.status = 0;
-    *plan.tiles = tiles;
-    plan.offset[sets] = live;
+    *plan.tiles = total[2];
+    *plan.dead_count = dead;
+    plan.offset[sets] = total[1];
   }
   __syncthreads();
   const int e = own0 + warp;  // e == sets: the dead routes
   if (e > sets) return;
-  int at = e < sets ? own_offset[warp] : live;
-  const int mine = e < sets ? own_count[warp] : routes - live;
+  const int mine = e < sets ? own_count[warp] : dead;
   if (mine == 0) return;
+  int32_t* to = e < sets ? plan.order + own_place[warp] : plan.dead;
   if (e < sets) {
-    const int parts = (mine + tile_routes - 1) / tile_routes;
-    const int part = (mine + parts - 1) / parts, per = (part + tile_step - 1) / tile_step * tile_step;
-    for (int p = lane; p < parts; p += 32) plan.tile[own_tile[warp] + p] = make_int4(e, at + p * per, max(0, min(per, mine - p * per)), 0);
+    const int parts = tiles_of(mine), part = (mine + parts - 1) / parts, per = (part + tile_step - 1) / tile_step * tile_step;
+    for (int p = lane; p < parts; p += 32) plan.tile[own_tile[warp] + p] = make_int4(e, own_place[warp] + p * per, min(per, mine - p * per), 0);
+    if (mine + lane < places_of(mine)) to[mine + lane] = -1;
   }
-  const int want = e < sets ? e : -1, end = at + mine;
-  for (int base = 0; base < routes && at < end; base += 128) {
+  const int want = e < sets ? e : -1;
+  for (int base = 0, at = 0; base < routes && at < mine; base += 128) {
     int found[4];
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
@@ -80,10 +88,26 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_kernel(Indices indices, int
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const unsigned hits = __ballot_sync(0xFFFFFFFFu, found[u] == want);
-      if (found[u] == want) plan.order[at + __popc(hits & ((1u << lane) - 1u))] = base + u * 32 + lane;
+      if (found[u] == want) to[at + __popc(hits & ((1u << lane) - 1u))] = base + u * 32 + lane;
       at += __popc(hits);
     }
   }
+}
+
+// HBM-bound; a block per place.
+__global__ void __launch_bounds__(128) copy_rows_kernel(RowCopy a, RowCopy b, Plan plan, int sets) {
+  if (static_cast<int>(blockIdx.x) >= plan.offset[sets]) return;
+  const RowCopy& c = blockIdx.y ? b : a;
+  const int route = plan.order[blockIdx.x];
+  const uint4* in = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(c.in) + (route < 0 ? 0 : route / c.div) * c.ld);
+  uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(c.out) + blockIdx.x * c.width);
+  for (int i = threadIdx.x; i < c.width / 8; i += 128) out[i] = route < 0 ? make_uint4(0, 0, 0, 0) : in[i];
+}
+
+int copy_rows(const RowCopy* copies, int count, int64_t routes, int64_t sets, const Plan& plan, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>(max_places(routes, sets)), count);
+  const cudaError_t e = launch_after(false, copy_rows_kernel, grid, 128, 0, s, copies[0], copies[count - 1], plan, static_cast<int>(sets));
+  return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
 }
 
 int make_plan(const Indices& indices, int64_t routes, int64_t sets, int tile_routes, int tile_step, const Plan& plan, cudaStream_t s) {
@@ -93,15 +117,13 @@ int make_plan(const Indices& indices, int64_t routes, int64_t sets, int tile_rou
     if (e != cudaSuccess) return note_cuda_error(e);
   }
   const unsigned blocks = static_cast<unsigned>((sets + 1 + PLAN_WARPS - 1) / PLAN_WARPS);
-  const cudaError_t e = launch_after(true, plan_kernel, blocks, PLAN_THREADS, smem, s, indices, static_cast<int>(routes), static_cast<int>(sets), tile_routes, tile_step, plan);
+  const cudaError_t e = launch_after(blocks <= PLAN_EARLY_BLOCKS, plan_kernel, blocks, PLAN_THREADS, smem, s, indices, static_cast<int>(routes), static_cast<int>(sets), tile_routes, tile_step, plan);
   return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
 }
 
 // HBM-bound: 4 bytes in per value and pick, 2 out; a thread has eight neighbouring values of a row.
 template <typename T>
 __global__ void __launch_bounds__(256) sum_picks_kernel(const float* __restrict__ in, Indices indices, int sets, int64_t rows, int picks, int64_t width, T* __restrict__ out) {
-  grid_launch_dependents();
-  grid_wait();
   const int64_t per_row = width / 8, total = rows * per_row;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += 256ll * gridDim.x) {
     const int64_t row = i / per_row, c = (i - row * per_row) * 8;
@@ -123,8 +145,8 @@ int sum_picks(const float* routes, const Indices& indices, int64_t sets, int64_t
   if (blocks > 148 * 32) blocks = 148 * 32;
   const dim3 grid(static_cast<unsigned>(blocks));
   const cudaError_t e = dtype == KEEPVQ_BF16
-      ? launch_after(true, sum_picks_kernel<__nv_bfloat16>, grid, 256, 0, s, routes, indices, static_cast<int>(sets), rows, picks, width, static_cast<__nv_bfloat16*>(out))
-      : launch_after(true, sum_picks_kernel<__half>, grid, 256, 0, s, routes, indices, static_cast<int>(sets), rows, picks, width, static_cast<__half*>(out));
+      ? launch_after(false, sum_picks_kernel<__nv_bfloat16>, grid, 256, 0, s, routes, indices, static_cast<int>(sets), rows, picks, width, static_cast<__nv_bfloat16*>(out))
+      : launch_after(false, sum_picks_kernel<__half>, grid, 256, 0, s, routes, indices, static_cast<int>(sets), rows, picks, width, static_cast<__half*>(out));
   return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
 }
 
