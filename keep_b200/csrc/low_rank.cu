@@ -2,80 +2,606 @@
 // A = right[e] of a route's set e:
 //   p = A x,  out = base + scale B p;   q = scale B^T grad,  dx = A^T q,
 //   dA = sum q x^T,  dB = scale sum grad p^T
+//
+// The rank is 8 to 128, so all of it is bound by reading x, grad, base and the factors once; what there
+// is to multiply stays on mma.sync, whose fragments come straight from global memory in 16-byte loads
+// (the order of a contraction is free, so a lane's eight neighbouring values serve two instructions).
+//
+// Two products with a vector in between (low_rank_kernel): a cluster of CTAs takes the rows of one set, up
+// to MT * 16, and splits the first contraction over its CTAs and their warps; the partial inner vectors meet in
+// shared memory, once per CTA and once over the cluster; the CTAs then split the width of the result.  So
+// the inner vectors never leave the SMs, and one row of one set still has a whole cluster's loads in
+// flight.  Forward: A, then B.  Input gradient: B^T, then A^T, whose fragments are transposed in registers.
+//
+// Inner vectors are fp32 sums; for the second product each is split into the sum of two 16-bit values, scaled
+// by a power of two per row for fp16 so that neither its range nor its small values are lost.
 #include "switch_plan.cuh"
 
 namespace keepvq {
 namespace dense {
 
-constexpr int LR_MAX_RANK = 128;
+constexpr int LR_MAX_RANK = 128, LR_WARPS = 8, LR_THREADS = LR_WARPS * 32, CHUNK = 32;
 
-// inner[r, j] = factor * sum_k m[e][j or k][k or j] v[row, k]: one warp per (route, j).
-template <bool ACROSS>
-__global__ void __launch_bounds__(256) inner_kernel(const void* v, int64_t ld, int x_div, const void* m, int64_t depth, int rank, int dtype, Indices indices, int sets, int64_t routes, float factor, float* inner) {
-  const int64_t i = blockIdx.x * 8ll + threadIdx.x / 32;
-  if (i >= routes * rank) return;
-  const int64_t r = i / rank, j = i - r * rank;
-  const int e = indices.set_of(r, sets), lane = threadIdx.x % 32;
-  float sum = 0.0f;
-  if (e >= 0)
-    for (int64_t k = lane; k < depth; k += 32)
-      sum += load_as_float(v, dtype, r / x_div * ld + k) * load_as_float(m, dtype, ACROSS ? (e * depth + k) * rank + j : (e * rank + j) * depth + k);
-  for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-  if (lane == 0) inner[i] = factor * sum;
-}
-
-// out[r, n] = base[r, n] + factor * sum_j inner[r, j] left[e][n][j]
-__global__ void __launch_bounds__(256) outer_kernel(keepvq_switch_low_rank_args a, Indices indices, const float* inner) {
-  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= a.routes * a.out_dim) return;
-  const int64_t r = i / a.out_dim, n = i - r * a.out_dim;
-  const int e = indices.set_of(r, static_cast<int>(a.sets));
-  float sum = 0.0f;
-  if (e >= 0)
-    for (int64_t j = 0; j < a.rank; ++j) sum += inner[r * a.rank + j] * load_as_float(a.left, a.dtype, (e * a.out_dim + n) * a.rank + j);
-  const float base = a.base ? load_as_float(a.base, a.out_dtype, r * a.base_ld + n) : 0.0f;
-  store_from_float(a.out, a.out_dtype, r * a.out_ld + n, e < 0 ? base : base + a.scale * sum);
-}
-
-// dx[t, k] = sum over picks, j of q[r, j] right[e][j][k]
-__global__ void __launch_bounds__(256) input_grad_kernel(keepvq_switch_low_rank_args a, Indices indices, const float* q) {
-  const int64_t i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= a.routes / a.x_div * a.in_dim) return;
-  const int64_t t = i / a.in_dim, k = i - t * a.in_dim;
-  float sum = 0.0f;
-  for (int64_t r = t * a.x_div; r < (t + 1) * a.x_div; ++r) {
-    const int e = indices.set_of(r, static_cast<int>(a.sets));
-    if (e < 0) continue;
-    for (int64_t j = 0; j < a.rank; ++j) sum += q[r * a.rank + j] * load_as_float(a.right, a.dtype, (e * a.rank + j) * a.in_dim + k);
+// ---- fragments ------------------------------------------------------------------------------------
+template <typename T>
+struct Mma;
+template <>
+struct Mma<__nv_bfloat16> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  store_from_float(a.dx, a.dtype, i, sum);
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) { return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u)); }
+  static constexpr bool SCALED = false;  // the range is fp32's
+};
+template <>
+struct Mma<__half> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float x, float y) {
+    const __half2 v = __floats2half2_rn(x, y);
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  static __device__ __forceinline__ float2 unpack(uint32_t v) { return __half22float2(*reinterpret_cast<const __half2*>(&v)); }
+  static constexpr bool SCALED = true;
+};
+// Two values as the sum of two 16-bit ones.  An infinity has no rest (inf - inf).
+template <typename T>
+__device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t& low) {
+  high = Mma<T>::pack(x, y);
+  const float2 h = Mma<T>::unpack(high);
+  low = Mma<T>::pack(isinf(h.x) ? 0.0f : x - h.x, isinf(h.y) ? 0.0f : y - h.y);
+}
+// An 8 x 8 matrix of 16-bit values, a row's pairs in four lanes, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t t;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  return t;
+}
+__device__ __forceinline__ uint4 load16(const uint16_t* p, bool there) { return there ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
+__device__ __forceinline__ uint2 load8(const uint16_t* p, bool there) { return there ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0); }
+__device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// A power of two not below `most`, within what has a reciprocal; 1 for zero and for what is not finite.
+__device__ __forceinline__ float power_above(float most) {
+  const uint32_t e = (__float_as_uint(most) >> 23) & 0xFFu;
+  return most == 0.0f || e == 255u ? 1.0f : __uint_as_float(min(max(e + 1u, 2u), 252u) << 23);
 }
 
-// grad[e][wide][j] or [e][j][wide] = factor * sum over e's routes of inner[r, j] v[row, wide]
-template <bool ACROSS>
-__global__ void __launch_bounds__(256) factor_grad_kernel(const void* v, int64_t ld, int x_div, int64_t wide, int rank, int dtype, Plan plan, const float* inner, float factor, void* out) {
-  const int64_t e = blockIdx.y, i = blockIdx.x * 256ll + threadIdx.x;
-  if (i >= wide * rank) return;
-  const int64_t n = ACROSS ? i / rank : i % wide, j = ACROSS ? i % rank : i / wide;
-  float sum = 0.0f;
-  for (int p = plan.offset[e]; p < plan.offset[e] + plan.count[e]; ++p) {
-    const int64_t r = plan.order[p];
-    sum += inner[r * rank + j] * load_as_float(v, dtype, r / x_div * ld + n);
+__device__ __forceinline__ uint32_t lr_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t lr_cluster_size() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r)); return r; }
+__device__ __forceinline__ void lr_cluster_sync() { asm volatile("barrier.cluster.arrive.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory"); }
+__device__ __forceinline__ float peer_float(const float* p, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(static_cast<uint32_t>(__cvta_generic_to_shared(p))), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
+}
+
+// ---- one product after the other ---------------------------------------------------------------------
+
+// Inner vectors as the gradients of the factors take them: per block of 16 places, [rank][16 places] of
+// 16-bit values, the two whose sum they are apart; a lane's four places of a fragment (2q, 2q + 1, 2q + 8,
+// 2q + 9) side by side.  `unit`: the power of two a block is divided by (fp16).
+struct Inner {
+  uint16_t *high, *low;
+  float* unit;
+};
+
+struct LowRankArgs {
+  const uint16_t* in;      // rows of the first contraction: x, or grad
+  int64_t in_ld;           // multiple of 8
+  int in_div;              // routes per row of `in`
+  const uint16_t* first;   // its factor: right, or left (transposed)
+  const uint16_t* second;  // left, or right (transposed); null: no second product
+  int64_t depth, width;    // of the first contraction; of the result
+  int rank, sets, routes;
+  float first_scale, second_scale;
+  const void* base;        // null: zeros
+  int64_t base_ld;
+  void* out;
+  int64_t out_ld;
+  int out32;               // base and out are fp32
+  int whole;               // their rows can be taken 16 bytes at a time
+  int dead_rows;           // rows without a set are the kernel's (their base, or zeros)
+  int solo;                // a tile per route, no plan
+  Indices indices;
+  Plan plan;
+  Inner keep;              // where to leave the inner vectors; null: nowhere
+};
+
+// RP: the rank rounded up (zeros).  MT: 16-row tiles.  BACK: both factors are used transposed.
+template <typename T, int RP, int MT, bool BACK>
+__global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) {
+  constexpr int ROWS = MT * 16, RT = RP / 8, V = RP >= 32 ? 8 : 4;  // V: neighbouring ranks a lane holds
+  extern __shared__ __align__(16) float sm[];
+  float* part = sm;                                     // [warps][ROWS][RP]
+  float* own = part + LR_WARPS * ROWS * RP;             // [ROWS][RP] of this CTA; then of the cluster
+  float* unit = own + 2 * ROWS * RP;                    // [ROWS]
+  int* route_of = reinterpret_cast<int*>(unit + ROWS);  // [ROWS]
+  float* inner = own + ROWS * RP;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int ctas = static_cast<int>(lr_cluster_size()), rank = static_cast<int>(lr_cluster_rank());
+  const int tile = blockIdx.x / ctas;
+
+  auto plain_row = [&](int64_t r) {  // a route without a set
+    const int64_t step = a.out32 ? 4 : 2;
+    for (int64_t n = tid; n < a.width; n += LR_THREADS) {
+      if (step == 4) static_cast<uint32_t*>(a.out)[r * a.out_ld + n] = a.base ? static_cast<const uint32_t*>(a.base)[r * a.base_ld + n] : 0u;
+      else static_cast<uint16_t*>(a.out)[r * a.out_ld + n] = a.base ? static_cast<const uint16_t*>(a.base)[r * a.base_ld + n] : static_cast<uint16_t>(0);
+    }
+  };
+  int set, start = 0, size = 1;
+  if (a.solo) {
+    set = a.indices.set_of(tile, a.sets);
+    if (set < 0) {  // uniform over the cluster
+      if (rank == 0 && a.dead_rows) plain_row(tile);
+      return;
+    }
+    if (tid < ROWS) route_of[tid] = tile;
+  } else {
+    if (a.dead_rows)
+      for (int p = blockIdx.x; p < *a.plan.dead_count; p += gridDim.x) plain_row(a.plan.dead[p]);
+    if (tile >= *a.plan.tiles) return;
+    const int4 t = a.plan.tile[tile];
+    set = t.x; start = t.y; size = t.z;
+    if (tid < ROWS) route_of[tid] = a.plan.order[start + min(tid, size - 1)];  // rows past the last repeat it and are not stored
   }
-  store_from_float(out, dtype, e * wide * rank + i, factor * sum);
+  __syncthreads();
+
+  // ---- the first product: rows [ROWS, depth] times the factor -> [ROWS, RP]
+  {
+    float acc[MT][RT][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < RT; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
+    int row[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) row[m][h] = route_of[m * 16 + h * 8 + g] / a.in_div;
+    const int64_t factor = static_cast<int64_t>(set) * a.rank * a.depth;
+#pragma unroll 2
+    for (int64_t k0 = (rank * LR_WARPS + warp) * CHUNK; k0 < a.depth; k0 += ctas * LR_WARPS * CHUNK) {
+      const int64_t k = k0 + q * 8;
+      const bool there = k < a.in_ld;  // (values of `in` between depth and in_ld are zeros)
+      uint4 v[MT][2];
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) v[m][h] = load16(a.in + row[m][h] * a.in_ld + k, there);
+      if (!BACK) {
+#pragma unroll
+        for (int n = 0; n < RT; ++n) {
+          const int j = n * 8 + g;
+          const uint4 w = load16(a.first + factor + j * a.depth + k, j < a.rank && there);
+#pragma unroll
+          for (int m = 0; m < MT; ++m) {
+            const uint32_t a0[4] = {v[m][0].x, v[m][1].x, v[m][0].y, v[m][1].y}, a1[4] = {v[m][0].z, v[m][1].z, v[m][0].w, v[m][1].w};
+            Mma<T>::run(acc[m][n], a0, w.x, w.y);
+            Mma<T>::run(acc[m][n], a1, w.z, w.w);
+          }
+        }
+      } else {
+        // the factor's rows lie along the contraction: 8 x 8 blocks of it are transposed in registers.  Row i of a
+        // block is the contraction index that the other operand's lane order wants there.
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int64_t r0 = k0 + 8 * (g >> 1) + 4 * j + (g & 1);
+#pragma unroll
+          for (int c = 0; c < RP / (4 * V); ++c) {
+            uint32_t w0[V / 2], w1[V / 2];
+            const int col = c * 4 * V + q * V;
+            const bool in_rank = col < a.rank;
+            if (V == 8) {
+              const uint4 x0 = load16(a.first + factor + r0 * a.rank + col, in_rank && r0 < a.depth), x1 = load16(a.first + factor + (r0 + 2) * a.rank + col, in_rank && r0 + 2 < a.depth);
+#pragma unroll
+              for (int t = 0; t < V / 2; ++t) { w0[t] = word(x0, t); w1[t] = word(x1, t); }
+            } else {
+              const uint2 x0 = load8(a.first + factor + r0 * a.rank + col, in_rank && r0 < a.depth), x1 = load8(a.first + factor + (r0 + 2) * a.rank + col, in_rank && r0 + 2 < a.depth);
+              w0[0] = x0.x; w0[1] = x0.y; w1[0] = x1.x; w1[1] = x1.y;
+            }
+#pragma unroll
+            for (int t = 0; t < V / 2; ++t) {
+              const uint32_t b0 = transpose8(w0[t]), b1 = transpose8(w1[t]);
+#pragma unroll
+              for (int m = 0; m < MT; ++m) {
+                const uint32_t av[4] = {j ? v[m][0].z : v[m][0].x, j ? v[m][1].z : v[m][1].x, j ? v[m][0].w : v[m][0].y, j ? v[m][1].w : v[m][1].y};
+                Mma<T>::run(acc[m][c * (V / 2) + t], av, b0, b1);
+              }
+            }
+          }
+        }
+      }
+    }
+    // a lane's ranks of tile n: 8 n + 2 q and the next; transposed: c * 4 V + V q + 2 t and the next
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int n = 0; n < RT; ++n) {
+        const int j = BACK ? n / (V / 2) * 4 * V + V * q + 2 * (n % (V / 2)) : 8 * n + 2 * q;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          *reinterpret_cast<float2*>(part + (warp * ROWS + m * 16 + h * 8 + g) * RP + j) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
+      }
+  }
+  __syncthreads();
+  for (int i = tid; i < ROWS * RP; i += LR_THREADS) {
+    float sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < LR_WARPS; ++w) sum += part[w * ROWS * RP + i];
+    own[i] = sum * a.first_scale;
+  }
+  if (ctas > 1) lr_cluster_sync();
+  else __syncthreads();
+  for (int i = tid; i < ROWS * RP; i += LR_THREADS) {
+    float sum = own[i];
+    if (ctas > 1) {
+      sum = 0.0f;
+      for (int c = 0; c < ctas; ++c) sum += peer_float(own + i, c);
+    }
+    inner[i] = sum;
+  }
+  __syncthreads();
+  if (Mma<T>::SCALED) {
+    if (tid < ROWS) {
+      float most = 0.0f;
+      for (int j = 0; j < RP; ++j) most = fmaxf(most, fabsf(inner[tid * RP + (j + tid) % RP]));
+      unit[tid] = power_above(most);
+    }
+    __syncthreads();
+  }
+  if (a.keep.high && rank == 0) {
+    for (int i = tid; i < ROWS * RP / 2; i += LR_THREADS) {  // two neighbouring places of a rank
+      const int block = i / (RP * 8), j = i / 8 % RP, pair = i % 8;
+      const int place = pair / 2 * 2 + (pair & 1) * 8, r0 = block * 16 + place;
+      if (r0 >= (size + 15) / 16 * 16) continue;
+      float most = 1.0f;
+      if (Mma<T>::SCALED) {
+        most = 0.0f;
+        for (int r = 0; r < 16; ++r)
+          if (block * 16 + r < size) most = fmaxf(most, unit[block * 16 + r]);
+        if (j == 0 && pair == 0) a.keep.unit[start / 16 + block] = most;
+      }
+      const float x = r0 < size ? inner[r0 * RP + j] / most : 0.0f, y = r0 + 1 < size ? inner[(r0 + 1) * RP + j] / most : 0.0f;
+      uint32_t high, low;
+      split<T>(x, y, high, low);
+      const int64_t at = (static_cast<int64_t>(start / 16 + block) * RP + j) * 8 + pair;
+      reinterpret_cast<uint32_t*>(a.keep.high)[at] = high;
+      reinterpret_cast<uint32_t*>(a.keep.low)[at] = low;
+    }
+  }
+
+  // ---- the second product: [ROWS, RP] times the factor -> [ROWS, width], 32 columns per warp and step
+  if (a.second) {
+    constexpr int KC = RP / 16;  // contraction steps
+    uint32_t high[MT][KC][4], low[MT][KC][4];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = m * 16 + (i & 1) * 8 + g;
+          const int j = V == 8 ? c / 2 * 32 + 8 * q + 4 * (c & 1) + 2 * (i >> 1) : 4 * q + 2 * (i >> 1);
+          const float2 v = *reinterpret_cast<const float2*>(inner + r * RP + j);
+          const float u = Mma<T>::SCALED ? 1.0f / unit[r] : 1.0f;  // (a power of two)
+          split<T>(v.x * u, v.y * u, high[m][c][i], low[m][c][i]);
+        }
+    const int64_t factor = static_cast<int64_t>(set) * a.rank * a.width;
+    for (int64_t n0 = (rank * LR_WARPS + warp) * 32; n0 < a.width; n0 += ctas * LR_WARPS * 32) {
+      uint32_t b[4][KC][2];  // the factor: 32 columns by RP.  Column c of tile t is n0 + 8 (c / 2) + 2 t + c % 2: a lane's results are neighbours
+      if (!BACK) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int64_t n = n0 + 8 * (g >> 1) + 2 * t + (g & 1);
+#pragma unroll
+          for (int c = 0; c < RP / (4 * V); ++c) {
+            const int j = c * 4 * V + q * V;
+            const bool there = n < a.width && j < a.rank;
+            if (V == 8) {
+              const uint4 w = load16(a.second + factor + n * a.rank + j, there);
+              b[t][(2 * c) % KC][0] = w.x; b[t][(2 * c) % KC][1] = w.y;
+              b[t][(2 * c + 1) % KC][0] = w.z; b[t][(2 * c + 1) % KC][1] = w.w;
+            } else {
+              const uint2 w = load8(a.second + factor + n * a.rank + j, there);
+              b[t][0][0] = w.x; b[t][0][1] = w.y;
+            }
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int j = (V == 8 ? c / 2 * 32 + 8 * (g >> 1) + 4 * (c & 1) : 4 * (g >> 1)) + (g & 1) + 2 * i;
+            const uint4 w = load16(a.second + factor + j * a.width + n0 + 8 * q, j < a.rank && n0 + 8 * q < a.width);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) b[t][c][i] = transpose8(word(w, t));
+          }
+      }
+      const int64_t n = n0 + 8 * q;
+#pragma unroll
+      for (int m = 0; m < MT; ++m) {
+        if (m * 16 >= size) break;
+        float d[4][4];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) d[t][i] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < KC; ++c) {
+            Mma<T>::run(d[t], low[m][c], b[t][c][0], b[t][c][1]);
+            Mma<T>::run(d[t], high[m][c], b[t][c][0], b[t][c][1]);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = m * 16 + h * 8 + g;
+          if (r >= size) continue;
+          const int64_t route = route_of[r], at = route * a.out_ld + n, from = route * a.base_ld + n;
+          const float s = Mma<T>::SCALED ? a.second_scale * unit[r] : a.second_scale;
+          float y[8];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) { y[2 * t] = s * d[t][2 * h]; y[2 * t + 1] = s * d[t][2 * h + 1]; }
+          if (a.whole) {
+            if (n >= a.width) continue;
+            float v[8] = {};
+            if (a.out32) {
+              if (a.base) load8_as_float(static_cast<const float*>(a.base) + from, v);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] += y[i];
+              store8_from_float(static_cast<float*>(a.out) + at, v);
+            } else {
+              if (a.base) load8_as_float(static_cast<const T*>(a.base) + from, v);
+#pragma unroll
+              for (int i = 0; i < 8; ++i) v[i] += y[i];
+              store8_from_float(static_cast<T*>(a.out) + at, v);
+            }
+          } else {
+            const int dtype = a.out32 ? KEEPVQ_F32 : Mma<T>::SCALED ? KEEPVQ_F16 : KEEPVQ_BF16;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (n + i < a.width) store_from_float(a.out, dtype, at + i, y[i] + (a.base ? load_as_float(a.base, dtype, from + i) : 0.0f));
+          }
+        }
+      }
+    }
+  }
+  if (ctas > 1) lr_cluster_sync();  // the others may still be reading this CTA's partial sums
+}
+
+// ---- gradients of the factors --------------------------------------------------------------------------
+
+struct FactorGradArgs {
+  const uint16_t* in;  // rows: x (for right), grad (for left)
+  int64_t in_ld;
+  int in_div;
+  int64_t width;       // in_dim, out_dim
+  int rank, row_parts; // row_parts: warps that share a set's rows, 1, 2, 4 or 8
+  float scale;
+  Plan plan;
+  Inner inner;
+  uint16_t* out;
+};
+
+// A warp has 32 columns of x (or grad) and RH ranks, and walks the set's rows 16 at a time; the warps that share
+// them add their sums up in shared memory in their order.
+//   right: D[rank][column] = inner^T rows       left: D[column][rank] = rows^T inner
+template <typename T, int RP, bool LEFT>
+__device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, int slab, int half, float* sm) {
+  constexpr int RH = RP > 64 ? 64 : RP, SUMS = RH;  // ranks of a CTA; sums of a lane: 32 columns x RH / 32 lanes
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
+  const int part = warp % a.row_parts, slabs = LR_WARPS / a.row_parts;
+  const int64_t col0 = (static_cast<int64_t>(slab) * slabs + warp / a.row_parts) * 32, col = col0 + 8 * q;
+  const int j0 = half * RH;
+  float acc[SUMS];
+#pragma unroll
+  for (int i = 0; i < SUMS; ++i) acc[i] = 0.0f;
+  const int start = a.plan.offset[set], size = a.plan.count[set], blocks = (size + 15) / 16;
+  const bool there = col < a.in_ld;
+  auto row_values = [&](int place) {
+    const int r = a.plan.order[start + place];
+    return load16(a.in + static_cast<int64_t>(r < 0 ? 0 : r / a.in_div) * a.in_ld + col, there && r >= 0);
+  };
+#pragma unroll 2
+  for (int b = part; b < blocks; b += a.row_parts) {
+    const uint4 v0 = row_values(b * 16 + g), v1 = row_values(b * 16 + 8 + g);
+    uint32_t x[4][2];  // tile t: columns col0 + 8 (c / 2) + 2 t + c % 2, the rows in pairs
+#pragma unroll
+    for (int t = 0; t < 4; ++t) { x[t][0] = transpose8(word(v0, t)); x[t][1] = transpose8(word(v1, t)); }
+    const int64_t block = (static_cast<int64_t>(start / 16) + b) * RP;
+    const float u = Mma<T>::SCALED ? a.inner.unit[start / 16 + b] : 1.0f;
+    auto inner_at = [&](const uint16_t* p, int j) { return __ldg(reinterpret_cast<const uint2*>(p + (block + j) * 16 + 4 * q)); };
+    auto add = [&](int at, const uint32_t (&m)[4], uint32_t n0, uint32_t n1, const uint32_t (&m2)[4], uint32_t k0, uint32_t k1) {
+      float d[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) d[i] = Mma<T>::SCALED ? 0.0f : acc[at + i];
+      Mma<T>::run(d, m2, k0, k1);
+      Mma<T>::run(d, m, n0, n1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[at + i] = Mma<T>::SCALED ? fmaf(u, d[i], acc[at + i]) : d[i];
+    };
+    if (!LEFT) {
+#pragma unroll
+      for (int m = 0; m < RH / 16; ++m) {
+        const int j = j0 + m * 16 + g;
+        const uint2 h0 = inner_at(a.inner.high, j), h1 = inner_at(a.inner.high, j + 8), l0 = inner_at(a.inner.low, j), l1 = inner_at(a.inner.low, j + 8);
+        const uint32_t high[4] = {h0.x, h1.x, h0.y, h1.y}, low[4] = {l0.x, l1.x, l0.y, l1.y};
+#pragma unroll
+        for (int t = 0; t < 4; ++t) add((m * 4 + t) * 4, high, x[t][0], x[t][1], low, x[t][0], x[t][1]);
+      }
+    } else {
+#pragma unroll
+      for (int n = 0; n < RH / 8; ++n) {  // column c of tile n is rank RH / 4 (c / 2) + 2 n + c % 2: a lane's ranks are neighbours
+        const int j = j0 + (g >> 1) * (RH / 4) + 2 * n + (g & 1);
+        const uint2 h = inner_at(a.inner.high, j), l = inner_at(a.inner.low, j);
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          const uint32_t rows[4] = {x[2 * m][0], x[2 * m + 1][0], x[2 * m][1], x[2 * m + 1][1]};
+          add((n * 2 + m) * 4, rows, h.x, h.y, rows, l.x, l.y);
+        }
+      }
+    }
+  }
+  if (a.row_parts > 1) {
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) sm[(warp * SUMS + i) * 32 + lane] = acc[i];
+    __syncthreads();
+    if (part != 0) return;
+    for (int p = 1; p < a.row_parts; ++p)
+#pragma unroll
+      for (int i = 0; i < SUMS; ++i) acc[i] += sm[((warp + p) * SUMS + i) * 32 + lane];
+  }
+  if (!LEFT) {
+#pragma unroll
+    for (int m = 0; m < RH / 16; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int j = j0 + m * 16 + h * 8 + g;
+        float y[8];
+#pragma unroll
+        for (int t = 0; t < 4; ++t) { y[2 * t] = a.scale * acc[(m * 4 + t) * 4 + 2 * h]; y[2 * t + 1] = a.scale * acc[(m * 4 + t) * 4 + 2 * h + 1]; }
+        if (j < a.rank && col < a.width) store8_from_float(reinterpret_cast<T*>(a.out) + (static_cast<int64_t>(set) * a.rank + j) * a.width + col, y);
+      }
+  } else {
+    constexpr int MINE = RH / 4;  // neighbouring ranks of a lane
+    const int j = j0 + q * MINE;
+#pragma unroll
+    for (int m = 0; m < 2; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {  // rows of the fragment: tile 2 m, then 2 m + 1
+        const int64_t n = col0 + 8 * (g >> 1) + 2 * (2 * m + h) + (g & 1);
+        if (n >= a.width) continue;
+        T* row = reinterpret_cast<T*>(a.out) + (static_cast<int64_t>(set) * a.width + n) * a.rank;
+        uint32_t packed[MINE / 2];
+#pragma unroll
+        for (int t = 0; t < RH / 8; ++t) packed[t] = Mma<T>::pack(a.scale * acc[(t * 2 + m) * 4 + 2 * h], a.scale * acc[(t * 2 + m) * 4 + 2 * h + 1]);
+#pragma unroll
+        for (int w = 0; w < MINE / 2; w += 2)
+          if (j + 2 * w < a.rank) *reinterpret_cast<uint2*>(row + j + 2 * w) = make_uint2(packed[w], packed[w + 1]);
+      }
+  }
+}
+
+template <typename T, int RP>
+__global__ void __launch_bounds__(LR_THREADS) factor_grad_kernel(FactorGradArgs right, FactorGradArgs left, int right_slabs) {
+  extern __shared__ __align__(16) float sm[];
+  const int slab = blockIdx.x;
+  if (slab < right_slabs) factor_grad<T, RP, false>(right, blockIdx.y, slab, blockIdx.z, sm);
+  else factor_grad<T, RP, true>(left, blockIdx.y, slab - right_slabs, blockIdx.z, sm);
+}
+
+// ---- host -------------------------------------------------------------------------------------------------
+
+static int rank_pad(int64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
+
+struct LowRankPlan {
+  int rp, mt, ctas;
+  bool solo;
+  int64_t tiles;  // at most
+};
+// One row per tile while there are no more rows than SMs: no plan to wait for, and rows that share a set
+// read it from the cache.  Else tiles of 16 rows, or of as many as 64 sums a lane allow where sets have more.
+// Clusters while there are not tiles enough for two CTAs on every SM.
+static LowRankPlan plan_low_rank(int64_t routes, int64_t sets, int64_t rank, bool grads) {
+  LowRankPlan p;
+  p.rp = rank_pad(rank);
+  p.solo = !grads && routes <= 148;
+  const int64_t used = routes < sets ? routes : sets;
+  p.mt = p.solo || routes <= 16 * used ? 1 : 128 / p.rp;
+  p.tiles = p.solo ? routes : max_tiles(routes, sets, p.mt * 16);
+  const int64_t expected = p.solo ? routes : routes / (p.mt * 16) + used / 2 + 1;
+  p.ctas = 1;
+  while (p.ctas < 8 && 2 * p.ctas * expected <= 296) p.ctas *= 2;
+  return p;
+}
+
+template <typename T, int RP, int MT, bool BACK>
+static int launch_low_rank(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
+  constexpr int SMEM = ((LR_WARPS + 2) * MT * 16 * RP + 2 * MT * 16) * 4;
+  auto kernel = low_rank_kernel<T, RP, MT, BACK>;
+  if (SMEM > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return note_cuda_error(e);
+  }
+  cudaLaunchConfig_t config = {};
+  config.gridDim = dim3(static_cast<unsigned>(p.tiles * p.ctas));
+  config.blockDim = dim3(LR_THREADS);
+  config.dynamicSmemBytes = SMEM;
+  config.stream = s;
+  cudaLaunchAttribute attribute = {};
+  attribute.id = cudaLaunchAttributeClusterDimension;
+  attribute.val.clusterDim.x = static_cast<unsigned>(p.ctas);
+  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  config.attrs = &attribute;
+  config.numAttrs = 1;
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
+  return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
+}
+template <typename T, bool BACK>
+static int launch_low_rank_of(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
+  if (p.rp == 16) return p.mt == 1 ? launch_low_rank<T, 16, 1, BACK>(a, p, s) : launch_low_rank<T, 16, 8, BACK>(a, p, s);
+  if (p.rp == 32) return p.mt == 1 ? launch_low_rank<T, 32, 1, BACK>(a, p, s) : launch_low_rank<T, 32, 4, BACK>(a, p, s);
+  if (p.rp == 64) return p.mt == 1 ? launch_low_rank<T, 64, 1, BACK>(a, p, s) : launch_low_rank<T, 64, 2, BACK>(a, p, s);
+  return launch_low_rank<T, 128, 1, BACK>(a, p, s);
+}
+static int launch_low_rank_any(int dtype, bool back, const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
+  if (dtype == KEEPVQ_BF16) return back ? launch_low_rank_of<__nv_bfloat16, true>(a, p, s) : launch_low_rank_of<__nv_bfloat16, false>(a, p, s);
+  return back ? launch_low_rank_of<__half, true>(a, p, s) : launch_low_rank_of<__half, false>(a, p, s);
+}
+
+template <typename T, int RP>
+static int launch_factor_grads(const FactorGradArgs& right, const FactorGradArgs& left, int64_t sets, cudaStream_t s) {
+  constexpr int RH = RP > 64 ? 64 : RP, SMEM = LR_WARPS * RH * 32 * 4;
+  auto kernel = factor_grad_kernel<T, RP>;
+  if (SMEM > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+    if (e != cudaSuccess) return note_cuda_error(e);
+  }
+  const int64_t cols = 32 * (LR_WARPS / right.row_parts);
+  const int64_t of_right = (right.width + cols - 1) / cols, of_left = (left.width + cols - 1) / cols;
+  const dim3 grid(static_cast<unsigned>(of_right + of_left), static_cast<unsigned>(sets), RP / RH);
+  kernel<<<grid, LR_THREADS, right.row_parts > 1 ? SMEM : 0, s>>>(right, left, static_cast<int>(of_right));
+  KEEPVQ_CHECK_LAUNCH();
+  return KEEPVQ_OK;
+}
+template <typename T>
+static int launch_factor_grads_of(int rp, const FactorGradArgs& right, const FactorGradArgs& left, int64_t sets, cudaStream_t s) {
+  if (rp == 16) return launch_factor_grads<T, 16>(right, left, sets, s);
+  if (rp == 32) return launch_factor_grads<T, 32>(right, left, sets, s);
+  if (rp == 64) return launch_factor_grads<T, 64>(right, left, sets, s);
+  return launch_factor_grads<T, 128>(right, left, sets, s);
 }
 
 struct LowRankLayout {
   Plan plan;
-  float *inner, *back;  // [routes, rank]: A x, and scale B^T grad
+  Inner inner, back;  // A x, and scale B^T grad
+  float* route_dx;    // [routes, in_dim], where a row has several picks
   int64_t bytes;
 };
-static LowRankLayout lay_out_low_rank(void* base, int64_t routes, int64_t sets, int64_t rank, bool grads) {
+static LowRankLayout lay_out_low_rank(void* base, int64_t routes, int64_t sets, int64_t in_dim, int64_t rank, int x_div, bool grads) {
   Scratch s{static_cast<char*>(base)};
+  const LowRankPlan p = plan_low_rank(routes, sets, rank, grads);
+  const int64_t blocks = max_places(routes, sets) / ROW_STEP + 1, values = grads ? blocks * ROW_STEP * p.rp : 0;
   LowRankLayout l;
-  l.plan = take_plan(s, routes, sets, 64);
-  l.inner = s.take<float>(routes * rank);
-  l.back = grads ? s.take<float>(routes * rank) : nullptr;
+  l.plan = take_plan(s, routes, sets, p.mt * 16);
+  for (Inner* i : {&l.inner, &l.back}) {
+    i->high = s.take<uint16_t>(values);
+    i->low = s.take<uint16_t>(values);
+    i->unit = s.take<float>(blocks);
+  }
+  l.route_dx = grads && x_div > 1 ? s.take<float>(routes * in_dim) : nullptr;
   l.bytes = s.used;
   return l;
 }
@@ -98,8 +624,6 @@ static int check_low_rank(const keepvq_switch_low_rank_args& a, bool grads) {
   return KEEPVQ_OK;
 }
 
-static unsigned blocks_of(int64_t n, int64_t per) { return static_cast<unsigned>((n + per - 1) / per); }
-
 }  // namespace dense
 }  // namespace keepvq
 
@@ -108,7 +632,7 @@ extern "C" {
 int64_t keepvq_switch_low_rank_workspace_bytes(int64_t routes, int64_t sets, int64_t out_dim, int64_t in_dim, int64_t rank, int32_t x_div, int32_t grads) {
   using namespace keepvq::dense;
   if (const int rc = check_low_rank_sizes(routes, sets, out_dim, in_dim, rank, x_div)) return rc;
-  return lay_out_low_rank(nullptr, routes, sets, rank, grads != 0).bytes;
+  return lay_out_low_rank(nullptr, routes, sets, in_dim, rank, x_div, grads != 0).bytes;
 }
 
 int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream) {
@@ -116,16 +640,36 @@ int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream
   if (!args) return KEEPVQ_ERR_NULL;
   const keepvq_switch_low_rank_args& a = *args;
   if (const int rc = check_low_rank(a, false)) return rc;
-  const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.rank, false);
+  const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.in_dim, a.rank, a.x_div, false);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   if (a.routes == 0) return KEEPVQ_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Indices indices{a.indices, a.index_bits};
-  inner_kernel<false><<<blocks_of(a.routes * a.rank, 8), 256, 0, s>>>(a.x, a.in_dim, a.x_div, a.right, a.in_dim, static_cast<int>(a.rank), a.dtype, indices, static_cast<int>(a.sets), a.routes, 1.0f, l.inner);
-  KEEPVQ_CHECK_LAUNCH();
-  outer_kernel<<<blocks_of(a.routes * a.out_dim, 256), 256, 0, s>>>(a, indices, l.inner);
-  KEEPVQ_CHECK_LAUNCH();
-  return KEEPVQ_OK;
+  const LowRankPlan p = plan_low_rank(a.routes, a.sets, a.rank, false);
+  LowRankArgs k = {};
+  k.indices = {a.indices, a.index_bits};
+  k.plan = l.plan;
+  if (!p.solo)
+    if (const int rc = make_plan(k.indices, a.routes, a.sets, p.mt * 16, ROW_STEP, l.plan, s)) return rc;
+  k.in = static_cast<const uint16_t*>(a.x);
+  k.in_ld = k.depth = a.in_dim;
+  k.in_div = a.x_div;
+  k.first = static_cast<const uint16_t*>(a.right);
+  k.second = static_cast<const uint16_t*>(a.left);
+  k.width = a.out_dim;
+  k.rank = static_cast<int>(a.rank);
+  k.sets = static_cast<int>(a.sets);
+  k.routes = static_cast<int>(a.routes);
+  k.first_scale = 1.0f;
+  k.second_scale = a.scale;
+  k.base = a.base;
+  k.base_ld = a.base_ld;
+  k.out = a.out;
+  k.out_ld = a.out_ld;
+  k.out32 = a.out_dtype == KEEPVQ_F32;
+  k.whole = a.out_dim % 8 == 0 && keepvq::aligned_to(a.out, 16) && a.out_ld % 8 == 0 && keepvq::aligned_to(a.base, 16) && (!a.base || a.base_ld % 8 == 0);
+  k.dead_rows = 1;
+  k.solo = p.solo;
+  return launch_low_rank_any(a.dtype, false, k, p, s);
 }
 
 int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* stream) {
@@ -133,21 +677,61 @@ int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* 
   if (!args) return KEEPVQ_ERR_NULL;
   const keepvq_switch_low_rank_args& a = *args;
   if (const int rc = check_low_rank(a, true)) return rc;
-  const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.rank, true);
+  const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.in_dim, a.rank, a.x_div, true);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const Indices indices{a.indices, a.index_bits};
-  const int rank = static_cast<int>(a.rank), sets = static_cast<int>(a.sets);
-  if (const int rc = make_plan(indices, a.routes, a.sets, 64, 16, l.plan, s)) return rc;
-  if (a.routes > 0) {
-    inner_kernel<false><<<blocks_of(a.routes * rank, 8), 256, 0, s>>>(a.x, a.in_dim, a.x_div, a.right, a.in_dim, rank, a.dtype, indices, sets, a.routes, 1.0f, l.inner);
-    inner_kernel<true><<<blocks_of(a.routes * rank, 8), 256, 0, s>>>(a.grad, a.grad_ld, 1, a.left, a.out_dim, rank, a.dtype, indices, sets, a.routes, a.scale, l.back);
-    if (a.dx) input_grad_kernel<<<blocks_of(a.routes / a.x_div * a.in_dim, 256), 256, 0, s>>>(a, indices, l.back);
+  if (a.routes == 0) {
+    for (void* p : {a.dleft, a.dright}) {
+      const cudaError_t e = p ? cudaMemsetAsync(p, 0, a.sets * a.rank * (p == a.dleft ? a.out_dim : a.in_dim) * 2, s) : cudaSuccess;
+      if (e != cudaSuccess) return keepvq::note_cuda_error(e);
+    }
+    return KEEPVQ_OK;
   }
-  if (a.dleft) factor_grad_kernel<true><<<dim3(blocks_of(a.out_dim * rank, 256), sets), 256, 0, s>>>(a.grad, a.grad_ld, 1, a.out_dim, rank, a.dtype, l.plan, l.inner, a.scale, a.dleft);
-  if (a.dright) factor_grad_kernel<false><<<dim3(blocks_of(a.in_dim * rank, 256), sets), 256, 0, s>>>(a.x, a.in_dim, a.x_div, a.in_dim, rank, a.dtype, l.plan, l.back, 1.0f, a.dright);
-  KEEPVQ_CHECK_LAUNCH();
-  return KEEPVQ_OK;
+  const LowRankPlan p = plan_low_rank(a.routes, a.sets, a.rank, true);
+  const bool weights = a.dleft || a.dright;
+  LowRankArgs k = {};
+  k.indices = {a.indices, a.index_bits};
+  k.plan = l.plan;
+  if (const int rc = make_plan(k.indices, a.routes, a.sets, p.mt * 16, ROW_STEP, l.plan, s)) return rc;
+  k.rank = static_cast<int>(a.rank);
+  k.sets = static_cast<int>(a.sets);
+  k.routes = static_cast<int>(a.routes);
+  // q = scale B^T grad, and dx = A^T q
+  k.in = static_cast<const uint16_t*>(a.grad);
+  k.in_ld = a.grad_ld;
+  k.in_div = 1;
+  k.first = static_cast<const uint16_t*>(a.left);
+  k.depth = a.out_dim;
+  k.first_scale = a.scale;
+  k.second = a.dx ? static_cast<const uint16_t*>(a.right) : nullptr;
+  k.second_scale = 1.0f;
+  k.width = k.out_ld = a.in_dim;
+  k.out = l.route_dx ? static_cast<void*>(l.route_dx) : a.dx;
+  k.out32 = l.route_dx != nullptr;
+  k.whole = 1;
+  k.dead_rows = a.dx && !l.route_dx;
+  if (weights) k.keep = l.back;
+  if (a.dx || a.dright)
+    if (const int rc = launch_low_rank_any(a.dtype, true, k, p, s)) return rc;
+  if (a.dx && l.route_dx)
+    if (const int rc = sum_picks(l.route_dx, k.indices, a.sets, a.routes / a.x_div, a.x_div, a.in_dim, a.dx, a.dtype, s)) return rc;
+  if (!weights) return KEEPVQ_OK;
+  if (a.dleft) {  // p = A x
+    k.in = static_cast<const uint16_t*>(a.x);
+    k.in_ld = k.depth = a.in_dim;
+    k.in_div = a.x_div;
+    k.first = static_cast<const uint16_t*>(a.right);
+    k.first_scale = 1.0f;
+    k.second = nullptr;
+    k.dead_rows = 0;
+    k.keep = l.inner;
+    if (const int rc = launch_low_rank_any(a.dtype, false, k, p, s)) return rc;
+  }
+  const int64_t mean = a.routes / (a.routes < a.sets ? a.routes : a.sets);
+  const int row_parts = mean <= 16 ? 1 : mean <= 64 ? 2 : mean <= 256 ? 4 : 8;  // a part keeps four blocks of 16 rows or more
+  FactorGradArgs right{static_cast<const uint16_t*>(a.x), a.in_dim, a.x_div, a.dright ? a.in_dim : 0, static_cast<int>(a.rank), row_parts, 1.0f, l.plan, l.back, static_cast<uint16_t*>(a.dright)};
+  FactorGradArgs left{static_cast<const uint16_t*>(a.grad), a.grad_ld, 1, a.dleft ? a.out_dim : 0, static_cast<int>(a.rank), row_parts, a.scale, l.plan, l.inner, static_cast<uint16_t*>(a.dleft)};
+  return a.dtype == KEEPVQ_BF16 ? launch_factor_grads_of<__nv_bfloat16>(p.rp, right, left, a.sets, s) : launch_factor_grads_of<__half>(p.rp, right, left, a.sets, s);
 }
 
 }  // extern "C"
