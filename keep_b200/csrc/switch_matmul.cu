@@ -36,8 +36,8 @@ using fast::smem_addr;
 
 enum { FORWARD = 0, INPUT_GRAD = 1, WEIGHT_GRAD = 2 };
 constexpr int M_TILE = 128, K_BLOCK = 64, N_STEP = 16, BOX_ROWS = 32;  // M_TILE: of a CTA.  // K_BLOCK: 128 bytes, a swizzled row
-constexpr int MM_THREADS = 256;
-enum { WARP_M = 0, WARP_N = 1, WARP_MMA = 2, WARP_OUT = 4 };  // loaders of the two operands, the issuer, four warps of the epilogue
+constexpr int OUT_WARPS = 8, MM_THREADS = 128 + OUT_WARPS * 32;
+enum { WARP_M = 0, WARP_N = 1, WARP_MMA = 2, WARP_OUT = 4 };  // loaders of the two operands, the issuer; the warps of the epilogue
 constexpr uint64_t MM_WAIT_NS = 2000000000ull;
 
 // ---- instructions ---------------------------------------------------------------------------------
@@ -114,6 +114,18 @@ __device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&v)[32]) {
                : "r"(taddr) : "memory");
 }
 
+// 16 lanes by 32 columns as fragments: of every 8 lanes x 8 columns a thread has lane thread / 4, columns
+// 2 (thread % 4) and the next; v[4 c] .. v[4 c + 1] are those of columns 8 c .. 8 c + 7, + 2 the lanes 8 further.
+__device__ __forceinline__ void tmem_ld_fragments(uint32_t taddr, uint32_t (&v)[16]) {
+  asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]), "=r"(v[9]), "=r"(v[10]),
+                 "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]) : "r"(taddr) : "memory");
+}
+// Four 8 x 8 matrices of 16-bit values to shared memory, transposed; a lane has the address of one row.
+__device__ __forceinline__ void store_transposed(uint32_t row, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(row), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+
 // Operand tiles with the 128-byte swizzle.  K-major: rows of 128 bytes along the contraction, groups of
 // eight 1024 bytes apart.  MN-major: 64 values of M or N in 128 bytes, a row per step of the contraction,
 // groups of eight 1024 bytes apart, the next 64 values one box (64 rows) on.
@@ -147,7 +159,7 @@ struct Shape {
   static constexpr int PAD = MANY ? 32 : N_STEP;                           // what the number of result rows is rounded up to
   static constexpr uint32_t A_BYTES = M_TILE * K_BLOCK * 2, STAGE_BYTES = A_BYTES + N_CTA * K_BLOCK * 2;
   static constexpr uint32_t STAGES = 192 * 1024 / STAGE_BYTES;  // 6 or 8
-  static constexpr uint32_t OUT_BYTES = 4 * 32 * 32 * 2;        // a 32 x 32 piece of the result for each warp of the epilogue
+  static constexpr uint32_t OUT_BYTES = OUT_WARPS * 32 * 32 * 2;        // a 32 x 32 piece of the result for each warp of the epilogue
   static constexpr uint32_t SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + OUT_BYTES;
   static constexpr uint32_t TMEM_COLS = 2 * N_MAX;              // two accumulators: one is written while the other is drained
 };
@@ -160,12 +172,14 @@ struct MatmulArgs {
   Plan plan;
 };
 
-template <typename T>
-__device__ __forceinline__ uint16_t bits_of(float v);
-template <>
-__device__ __forceinline__ uint16_t bits_of<__half>(float v) { return __half_as_ushort(__float2half_rn(v)); }
-template <>
-__device__ __forceinline__ uint16_t bits_of<__nv_bfloat16>(float v) { return __bfloat16_as_ushort(__float2bfloat16_rn(v)); }
+__device__ __forceinline__ uint32_t round_pair(uint32_t x, uint32_t y, bool bf16) {
+  if (bf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(__uint_as_float(x), __uint_as_float(y));
+    return *reinterpret_cast<const uint32_t*>(&v);
+  }
+  const __half2 v = __floats2half2_rn(__uint_as_float(x), __uint_as_float(y));
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
 
 // One tile of the result, or a CTA's half of it.
 struct Item {
@@ -196,7 +210,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
   if (tid == 0) {
     abort_flag = 0;
     for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 2 * CTAS); mbar_init(empty + 8 * s, 1); }
-    for (uint32_t s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, 4 * CTAS); }
+    for (uint32_t s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, OUT_WARPS * CTAS); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == WARP_MMA) tmem_alloc<MANY>(smem_addr(&tmem_slot), S::TMEM_COLS);
@@ -213,18 +227,18 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
 
   const int cols = static_cast<int>(MODE == FORWARD ? a.out_dim : a.in_dim);  // of a result row
   const int m_tiles = (cols + CTAS * M_TILE - 1) / (CTAS * M_TILE);
-  const int n_tiles = MODE == WEIGHT_GRAD ? static_cast<int>((a.out_dim + N_MAX - 1) / N_MAX) : 0;
+  const int n_tiles = MODE == WEIGHT_GRAD ? static_cast<int>((a.out_dim + N_MAX - 1) / N_MAX) : 1;
   const int depth_blocks = static_cast<int>(((MODE == FORWARD ? a.in_dim : a.out_dim) + K_BLOCK - 1) / K_BLOCK);
-  const int64_t items = static_cast<int64_t>(m_tiles) * (MODE == WEIGHT_GRAD ? static_cast<int64_t>(n_tiles) * a.sets : *a.plan.tiles);
+  const int items = m_tiles * (MODE == WEIGHT_GRAD ? n_tiles * a.sets : *a.plan.tiles);  // (below 2^31, check_sizes)
   const int first_item = blockIdx.x / CTAS, item_step = gridDim.x / CTAS;
   // Every role walks the same items on its own clock.
-  auto item_at = [&](int64_t i) {
+  auto item_at = [&](int i) {
     Item it;
-    const int64_t outer = i / m_tiles;
-    it.m0 = (static_cast<int>(i - outer * m_tiles) * CTAS + rank) * M_TILE;
+    const int outer = static_cast<int>(static_cast<uint32_t>(i) / static_cast<uint32_t>(m_tiles));
+    it.m0 = ((i - outer * m_tiles) * CTAS + rank) * M_TILE;
     if (MODE == WEIGHT_GRAD) {
-      it.set = static_cast<int>(outer / n_tiles);
-      it.n0 = static_cast<int>(outer - static_cast<int64_t>(it.set) * n_tiles) * N_MAX;
+      it.set = static_cast<int>(static_cast<uint32_t>(outer) / static_cast<uint32_t>(n_tiles));
+      it.n0 = (outer - it.set * n_tiles) * N_MAX;
       it.start = a.plan.offset[it.set];
       it.size = a.plan.count[it.set];
       it.n = min(N_MAX, static_cast<int>(a.out_dim) - it.n0);
@@ -246,7 +260,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     Ring<STAGES> r;
     const uint32_t tile = ring + (warp == WARP_N ? S::A_BYTES : 0);
     const CUtensorMap* map = warp == WARP_M ? &m_map : &n_map;
-    for (int64_t i = first_item; i < items && ok; i += item_step) {
+    for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       const int half = it.n_pad / CTAS;  // of the N operand, in this CTA
       int4 rows;
@@ -290,7 +304,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     // fp32 accumulator, fp16 or bf16 operands
     const uint32_t format = a.dtype == KEEPVQ_BF16 ? 1u : 0u;
     const uint32_t idesc0 = (1u << 4) | (format << 7) | (format << 10) | (static_cast<uint32_t>(M_MN) << 15) | (static_cast<uint32_t>(N_MN) << 16) | ((CTAS * M_TILE >> 4) << 24);
-    for (int64_t i = first_item; i < items && ok; i += item_step) {
+    for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks == 0) continue;  // (an expert without routes: the epilogue writes zeros)
       ok = wait_for(acc_empty + 8 * acc.index, acc.phase ^ 1u, deadline, aborted);
@@ -316,13 +330,17 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     }
   } else if (warp >= WARP_OUT) {
     // ================= the epilogue ================================================================
-    const int quadrant = warp & 3;
+    // a warp reaches a quarter of the accumulators' lanes; two share it, 32 result rows in turn (one warp alone took longer
+    // to drain 256 of them, 530 cycles for 32, than the products of six K blocks)
+    const int quadrant = warp & 3, turn = (warp - WARP_OUT) >> 2;
+    constexpr int TURN = OUT_WARPS / 4 * 32;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quadrant * 32) << 16);
-    uint16_t* piece = reinterpret_cast<uint16_t*>(smem_raw + (ring - smem_addr(smem_raw)) + STAGES * S::STAGE_BYTES) + quadrant * 32 * 32;  // [result row][32 values]
+    const uint32_t piece = ring + STAGES * S::STAGE_BYTES + (warp - WARP_OUT) * 32 * 64;
+    const bool bf16 = a.dtype == KEEPVQ_BF16;
     const bool whole = cols % 8 == 0;
     Ring<2> acc;
     if (MODE == FORWARD || (MODE == INPUT_GRAD && !a.route_dx)) {  // rows of dead routes
-      for (int64_t p = blockIdx.x * 4 + quadrant; p < *a.plan.dead_count; p += gridDim.x * 4) {
+      for (int p = blockIdx.x * OUT_WARPS + warp - WARP_OUT; p < *a.plan.dead_count; p += gridDim.x * OUT_WARPS) {
         uint16_t* row = static_cast<uint16_t*>(a.out) + static_cast<int64_t>(a.plan.dead[p]) * cols;
         if (whole)
           for (int c = lane * 8; c < cols; c += 256) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
@@ -330,7 +348,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
           for (int c = lane; c < cols; c += 32) row[c] = 0;
       }
     }
-    for (int64_t i = first_item; i < items && ok; i += item_step) {
+    for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks > 0) {
         ok = wait_for(acc_full + 8 * acc.index, acc.phase, deadline, aborted);
@@ -338,52 +356,72 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
       const int col = it.m0 + quadrant * 32;
-      for (int c0 = 0; c0 < it.n; c0 += 32) {
-        uint32_t v[32];
-        if (it.k_blocks > 0) {
+      if (MODE == INPUT_GRAD && a.route_dx) {  // fp32, to be summed over the picks
+        for (int c0 = turn * 32; c0 < it.n; c0 += TURN) {
+          uint32_t v[32];
+          const int n = min(32, it.n - c0), row = lane < n ? a.plan.order[it.start + c0 + lane] : 0;
           tmem_ld32(lanes + acc.index * N_MAX + c0, v);
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0;
-        }
-        const int n = min(32, it.n - c0);
-        // the row that result row c0 + lane is
-        const int64_t row = lane >= n ? 0 : MODE == WEIGHT_GRAD ? it.set * a.out_dim + it.n0 + c0 + lane : a.plan.order[it.start + c0 + lane];
-        if (MODE == INPUT_GRAD && a.route_dx) {
 #pragma unroll
           for (int j = 0; j < 32; ++j) {
-            const int64_t to = __shfl_sync(0xFFFFFFFFu, static_cast<int>(row), j);
+            const int64_t to = __shfl_sync(0xFFFFFFFFu, row, j);
             if (j < n && col + lane < cols) a.route_dx[to * cols + col + lane] = __uint_as_float(v[j]);
           }
-          continue;
         }
-        if (a.dtype == KEEPVQ_BF16) {
+      } else {
+        // 32 result rows at a time: fragments of tensor memory, rounded, transposed by the store to shared memory, where
+        // a result row's 32 values of this warp become 64 bytes in four pieces (piece c of row r at c ^ (r / 2) % 4: no
+        // bank twice); the next 32 rows' fragments are on their way meanwhile
+        const uint32_t from = lanes + acc.index * N_MAX;
+        const int row8 = lane >> 2, c = col + (lane & 3) * 8;
+        const uint32_t st_row = piece + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4), ld_row = piece + row8 * 64 + (((lane & 3) ^ ((row8 >> 1) & 3)) << 4);
+        uint32_t low[16], high[16];
+        auto load = [&](int c0) {
+          if (it.k_blocks > 0) {
+            tmem_ld_fragments(from + c0, low);
+            tmem_ld_fragments(from + (16u << 16) + c0, high);
+          } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) piece[j * 32 + lane] = bits_of<__nv_bfloat16>(__uint_as_float(v[j]));
-        } else {
+            for (int i = 0; i < 16; ++i) low[i] = high[i] = 0;
+          }
+        };
+        if (turn * 32 < it.n) load(turn * 32);
+        for (int c0 = turn * 32; c0 < it.n; c0 += TURN) {
+          int64_t to[4];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) piece[j * 32 + lane] = bits_of<__half>(__uint_as_float(v[j]));
-        }
-        __syncwarp();
+          for (int u = 0; u < 4; ++u) {
+            const int j = c0 + u * 8 + row8;
+            to[u] = j >= it.n ? -1 : MODE == WEIGHT_GRAD ? it.set * a.out_dim + it.n0 + j : a.plan.order[it.start + j];
+          }
+          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+          uint32_t pair[4][4];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {  // eight result rows of 64 bytes at a time
-          const int j = u * 8 + (lane >> 2), c = col + (lane & 3) * 8;
-          const int64_t to = __shfl_sync(0xFFFFFFFFu, row, j);
-          const uint4 eight = *reinterpret_cast<const uint4*>(piece + j * 32 + (lane & 3) * 8);
-          uint16_t* dst = static_cast<uint16_t*>(a.out) + to * cols + c;
-          if (j < n) {
+          for (int u = 0; u < 4; ++u) {
+            pair[u][0] = round_pair(low[4 * u], low[4 * u + 1], bf16);
+            pair[u][1] = round_pair(low[4 * u + 2], low[4 * u + 3], bf16);
+            pair[u][2] = round_pair(high[4 * u], high[4 * u + 1], bf16);
+            pair[u][3] = round_pair(high[4 * u + 2], high[4 * u + 3], bf16);
+          }
+          if (c0 + TURN < it.n) load(c0 + TURN);
+#pragma unroll
+          for (int u = 0; u < 4; ++u) store_transposed(st_row + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);
+          __syncwarp();
+#pragma unroll
+          for (int u = 0; u < 4; ++u) {
+            uint32_t w[4];
+            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(ld_row + u * 512) : "memory");
+            uint16_t* dst = static_cast<uint16_t*>(a.out) + to[u] * cols + c;
+            if (to[u] < 0) continue;
             if (whole) {
-              if (c < cols) *reinterpret_cast<uint4*>(dst) = eight;
+              if (c < cols) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
             } else {
-              const uint32_t pair[4] = {eight.x, eight.y, eight.z, eight.w};
 #pragma unroll
               for (int d = 0; d < 8; ++d)
-                if (c + d < cols) dst[d] = static_cast<uint16_t>(pair[d >> 1] >> (16 * (d & 1)));
+                if (c + d < cols) dst[d] = static_cast<uint16_t>(w[d >> 1] >> (16 * (d & 1)));
             }
           }
+          __syncwarp();
         }
-        __syncwarp();
       }
       if (it.k_blocks > 0) {
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -458,6 +496,9 @@ static Layout lay_out(void* base, int64_t routes, int64_t experts, int64_t out_d
 static int check_sizes(int64_t routes, int64_t experts, int64_t out_dim, int64_t in_dim, int32_t x_div) {
   if (routes < 0 || experts <= 0 || out_dim <= 0 || in_dim <= 0 || x_div <= 0 || in_dim % 8 != 0 || routes % x_div != 0) return KEEPVQ_ERR_SHAPE;
   if (routes > MAX_ROUTES || experts > MAX_SETS || out_dim > (1 << 24) || in_dim > (1 << 24)) return KEEPVQ_ERR_CAPACITY;
+  // tiles are numbered in 32 bits, with room for a step beyond the last
+  const int64_t most = (routes / 64 + experts + 1) * ((out_dim > in_dim ? out_dim : in_dim) / 128 + 1), of_weights = experts * (out_dim / 256 + 1) * (in_dim / 256 + 1);
+  if (most > (int64_t{1} << 30) || of_weights > (int64_t{1} << 30)) return KEEPVQ_ERR_CAPACITY;
   return KEEPVQ_OK;
 }
 
