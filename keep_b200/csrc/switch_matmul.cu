@@ -54,6 +54,15 @@ __device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* map, 
   asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
                ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar) : "memory");
 }
+// A box from shared memory to the matrix; what lies outside it is not written.
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t src) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(src) : "memory");
+  asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// At most N of this thread's stores still have to read their source.
+template <int N>
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory"); }
 template <bool PAIR>
 __device__ __forceinline__ void mma_16bit(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
   if (PAIR) asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
@@ -159,7 +168,7 @@ struct Shape {
   static constexpr int PAD = MANY ? 32 : N_STEP;                           // what the number of result rows is rounded up to
   static constexpr uint32_t A_BYTES = M_TILE * K_BLOCK * 2, STAGE_BYTES = A_BYTES + N_CTA * K_BLOCK * 2;
   static constexpr uint32_t STAGES = 192 * 1024 / STAGE_BYTES;  // 6 or 8
-  static constexpr uint32_t OUT_BYTES = OUT_WARPS * 32 * 32 * 2;        // a 32 x 32 piece of the result for each warp of the epilogue
+  static constexpr uint32_t OUT_BYTES = (MANY ? 2 : 1) * OUT_WARPS * 32 * 32 * 2;  // 32 x 32 pieces of the result for each warp of the epilogue
   static constexpr uint32_t SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + OUT_BYTES;
   static constexpr uint32_t TMEM_COLS = 2 * N_MAX;              // two accumulators: one is written while the other is drained
 };
@@ -190,7 +199,8 @@ struct Item {
 };
 
 template <int MODE, bool MANY>
-__global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs a, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map) {
+__global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs a, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map,
+                                                                      const __grid_constant__ CUtensorMap out_map) {
   using S = Shape<MANY>;
   static_assert(MANY || MODE != WEIGHT_GRAD, "the rows of dweight's operands are copied first");
   constexpr uint32_t STAGES = S::STAGES;
@@ -335,7 +345,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     const int quadrant = warp & 3, turn = (warp - WARP_OUT) >> 2;
     constexpr int TURN = OUT_WARPS / 4 * 32;
     const uint32_t lanes = tmem + (static_cast<uint32_t>(quadrant * 32) << 16);
-    const uint32_t piece = ring + STAGES * S::STAGE_BYTES + (warp - WARP_OUT) * 32 * 64;
+    const uint32_t piece = ring + STAGES * S::STAGE_BYTES + (warp - WARP_OUT) * (S::OUT_BYTES / OUT_WARPS);
+    uint32_t flip = 0;  // which of this warp's two pieces is next (dweight)
     const bool bf16 = a.dtype == KEEPVQ_BF16;
     const bool whole = cols % 8 == 0;
     Ring<2> acc;
@@ -371,7 +382,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
       } else {
         // 32 result rows at a time: fragments of tensor memory, rounded, transposed by the store to shared memory, where
         // a result row's 32 values of this warp become 64 bytes in four pieces (piece c of row r at c ^ (r / 2) % 4: no
-        // bank twice); the next 32 rows' fragments are on their way meanwhile
+        // bank twice); the next 32 rows' fragments are on their way meanwhile.  dweight's rows are neighbours: a store of the
+        // whole piece by TMA, which has the same swizzle, from two pieces in turn
         const uint32_t from = lanes + acc.index * N_MAX;
         const int row8 = lane >> 2, c = col + (lane & 3) * 8;
         const uint32_t st_row = piece + (lane & 7) * 64 + (((lane >> 3) ^ ((lane >> 1) & 3)) << 4), ld_row = piece + row8 * 64 + (((lane & 3) ^ ((row8 >> 1) & 3)) << 4);
@@ -391,7 +403,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
 #pragma unroll
           for (int u = 0; u < 4; ++u) {
             const int j = c0 + u * 8 + row8;
-            to[u] = j >= it.n ? -1 : MODE == WEIGHT_GRAD ? it.set * a.out_dim + it.n0 + j : a.plan.order[it.start + j];
+            to[u] = MODE == WEIGHT_GRAD || j >= it.n ? -1 : a.plan.order[it.start + j];
           }
           asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
           uint32_t pair[4][4];
@@ -403,6 +415,17 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
             pair[u][3] = round_pair(high[4 * u + 2], high[4 * u + 3], bf16);
           }
           if (c0 + TURN < it.n) load(c0 + TURN);
+          if (MODE == WEIGHT_GRAD) {
+            if (lane == 0) tma_stores_read<1>();
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) store_transposed(st_row + flip + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0 && col < cols) tma_store_3d(&out_map, col, it.n0 + c0, it.set, piece + flip);
+            flip ^= 32 * 64;
+            continue;
+          }
 #pragma unroll
           for (int u = 0; u < 4; ++u) store_transposed(st_row + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);
           __syncwarp();
@@ -430,6 +453,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
         acc.advance();
       }
     }
+    if (MODE == WEIGHT_GRAD && lane == 0) tma_stores_read<0>();  // (also of a warp that gave up)
   }
 
   __syncthreads();  // every role has left its loop
@@ -449,8 +473,8 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
 // ---- host ------------------------------------------------------------------------------------------
 
 // A tensor map of 16-bit values in this GPU's own memory: `sets` matrices [rows, width], boxes of 64 values
-// by box_rows rows of one of them (0: single rows, to be gathered).
-static int value_map(CUtensorMap* map, const void* base, int dtype, int64_t width, int64_t row_values, int64_t rows, int64_t sets, uint32_t box_rows) {
+// by box_rows rows of one of them (0: single rows, to be gathered), or of 32 values with the swizzle that goes with it.
+static int value_map(CUtensorMap* map, const void* base, int dtype, int64_t width, int64_t row_values, int64_t rows, int64_t sets, uint32_t box_rows, uint32_t box_cols = K_BLOCK) {
   typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*, const cuuint32_t*,
                                   CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
   static EncodeTiled encode = nullptr;
@@ -464,9 +488,9 @@ static int value_map(CUtensorMap* map, const void* base, int dtype, int64_t widt
   }
   const cuuint64_t dims[3] = {static_cast<cuuint64_t>(width), static_cast<cuuint64_t>(rows), static_cast<cuuint64_t>(sets)};
   const cuuint64_t strides[2] = {static_cast<cuuint64_t>(row_values * 2), static_cast<cuuint64_t>(row_values * 2 * rows)};
-  const cuuint32_t box[3] = {K_BLOCK, box_rows ? box_rows : 1, 1}, steps[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {box_cols, box_rows ? box_rows : 1, 1}, steps[3] = {1, 1, 1};
   const CUresult r = encode(map, dtype == KEEPVQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, box_rows ? 3 : 2, const_cast<void*>(base), dims, strides, box,
-                            steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                            steps, CU_TENSOR_MAP_INTERLEAVE_NONE, box_cols == K_BLOCK ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   return r == CUDA_SUCCESS ? KEEPVQ_OK : KEEPVQ_ERR_LAUNCH;
 }
 
@@ -507,7 +531,7 @@ static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cud
   using S = Shape<MANY>;
   MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.routes, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan};
   const int64_t places = max_places(a.routes, a.experts), grad_ld = MANY ? align_up(a.out_dim, 8) : a.grad_ld;
-  CUtensorMap m_map, n_map;
+  CUtensorMap m_map, n_map, out_map;
   int rc = MODE == WEIGHT_GRAD ? value_map(&m_map, l.x, a.dtype, a.in_dim, a.in_dim, places, 1, K_BLOCK)
                                : value_map(&m_map, a.weight, a.dtype, a.in_dim, a.in_dim, a.out_dim, a.experts, MODE == FORWARD ? M_TILE : K_BLOCK);
   if (rc) return rc;
@@ -515,6 +539,9 @@ static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cud
   rc = MODE == FORWARD ? value_map(&n_map, MANY ? l.x : a.x, a.dtype, a.in_dim, a.in_dim, MANY ? places : a.routes / a.x_div, 1, box)
                        : value_map(&n_map, MANY ? l.grad : a.grad, a.dtype, a.out_dim, grad_ld, MANY ? places : a.routes, 1, box);
   if (rc) return rc;
+  out_map = m_map;
+  if (MODE == WEIGHT_GRAD)
+    if ((rc = value_map(&out_map, a.dweight, a.dtype, a.in_dim, a.in_dim, a.out_dim, a.experts, 32, 32))) return rc;
   auto kernel = switch_matmul_kernel<MODE, MANY>;
   static uint64_t configured = 0;  // one bit per device: the shared-memory opt-in is a per-device attribute of the function
   int dev = 0, sms = 148;
@@ -541,7 +568,7 @@ static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cud
   }
   config.attrs = &attribute;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, m, m_map, n_map);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, m, m_map, n_map, out_map);
   return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
 }
 
