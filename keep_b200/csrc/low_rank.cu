@@ -4,8 +4,10 @@
 //   dA = sum q x^T,  dB = scale sum grad p^T
 //
 // The rank is 8 to 128, so all of it is bound by reading x, grad, base and the factors once; what there
-// is to multiply stays on mma.sync, whose fragments come straight from global memory in 16-byte loads
-// (the order of a contraction is free, so a lane's eight neighbouring values serve two instructions).
+// is to multiply stays on mma.sync, whose fragments are made of 16-byte pieces as they lie in memory (the
+// order of a contraction is free, so a lane's eight neighbouring values serve two instructions).  Every lane
+// copies the pieces that it will want itself to a queue of its own in shared memory, some steps ahead:
+// bytes in flight that cost no registers, and nobody to wait for but the copies.
 //
 // Two products with a vector in between (low_rank_kernel): a cluster of CTAs takes the rows of one set, up
 // to MT * 16, and splits the first contraction over its CTAs and their warps; the partial inner vectors meet in
@@ -28,7 +30,7 @@ struct Mma;
 template <>
 struct Mma<__nv_bfloat16> {
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -41,7 +43,7 @@ struct Mma<__nv_bfloat16> {
 template <>
 struct Mma<__half> {
   static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
   static __device__ __forceinline__ uint32_t pack(float x, float y) {
@@ -61,12 +63,28 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t
 // An 8 x 8 matrix of 16-bit values, a row's pairs in four lanes, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t t;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(t) : "r"(v));
   return t;
 }
 __device__ __forceinline__ uint4 load16(const uint16_t* p, bool there) { return there ? __ldg(reinterpret_cast<const uint4*>(p)) : make_uint4(0, 0, 0, 0); }
 __device__ __forceinline__ uint2 load8(const uint16_t* p, bool there) { return there ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0); }
 __device__ __forceinline__ uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
+
+// A lane's queue: pieces of up to 16 bytes, those of a step in one group of copies.  A piece that is not there is zeros.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy8(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(dst), "l"(src), "r"(there ? 8 : 0) : "memory");
+}
+__device__ __forceinline__ void step_issued() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int STEPS>
+__device__ __forceinline__ void all_but() { asm volatile("cp.async.wait_group %0;" ::"n"(STEPS) : "memory"); }
+__device__ __forceinline__ uint4 piece16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at) : "memory");
+  return v;
+}
 
 // A power of two not below `most`, within what has a reciprocal; 1 for zero and for what is not finite.
 __device__ __forceinline__ float power_above(float most) {
@@ -118,24 +136,49 @@ struct LowRankArgs {
 };
 
 // RP: the rank rounded up (zeros).  MT: 16-row tiles.  BACK: both factors are used transposed.
+template <int RP, int MT, bool BACK>
+struct LowRankShape {
+  static constexpr int ROWS = MT * 16, RT = RP / 8, KC = RP / 16, V = RP >= 32 ? 8 : 4, CC = RP / (4 * V);  // V: neighbouring ranks a lane holds
+  static constexpr int FACTOR1 = BACK ? 4 * CC : RT, FACTOR2 = BACK ? 2 * KC : 4 * CC;  // pieces of a step: the factor's, and 2 MT of the rows
+  static constexpr int PIECES = 2 * MT + (FACTOR1 > FACTOR2 ? FACTOR1 : FACTOR2), STEP_BYTES = PIECES * 32 * 16;
+  static constexpr bool SMALL = MT == 1 && RP <= 16;  // three CTAs on an SM instead of two: calls of many sets with a few rows each
+  static constexpr int BUDGET = SMALL ? 9 * 1024 : 12 * 1024, STEPS = BUDGET / STEP_BYTES < 2 ? 2 : BUDGET / STEP_BYTES;  // per warp; some 200 KB in flight on an SM
+  static constexpr int QUEUES = LR_WARPS * STEPS * STEP_BYTES;
+  static constexpr int BYTES = QUEUES + 2 * ROWS * RP * 4 + 2 * ROWS * 4;  // (the warps' partial sums lie where the queues were)
+  static constexpr int CTAS = SMALL ? 3 : BYTES + 1024 <= 114 * 1024 ? 2 : 1;  // on an SM
+  static_assert(CTAS * (BYTES + 1024) <= 228 * 1024, "");
+  static_assert(LR_WARPS * ROWS * RP * 4 <= QUEUES, "");
+};
+
 template <typename T, int RP, int MT, bool BACK>
-__global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) {
-  constexpr int ROWS = MT * 16, RT = RP / 8, V = RP >= 32 ? 8 : 4;  // V: neighbouring ranks a lane holds
+__global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, MT, BACK>::CTAS) low_rank_kernel(LowRankArgs a) {
+  grid_wait();
+  using S = LowRankShape<RP, MT, BACK>;
+  constexpr int ROWS = S::ROWS, RT = S::RT, V = S::V, KC = S::KC, CC = S::CC, STEPS = S::STEPS;
   extern __shared__ __align__(16) float sm[];
-  float* part = sm;                                     // [warps][ROWS][RP]
-  float* own = part + LR_WARPS * ROWS * RP;             // [ROWS][RP] of this CTA; then of the cluster
+  float* part = sm;                                     // [warps][ROWS][RP], behind the queues of the first product
+  float* own = sm + S::QUEUES / 4;                      // [ROWS][RP] of this CTA; then of the cluster
   float* unit = own + 2 * ROWS * RP;                    // [ROWS]
   int* route_of = reinterpret_cast<int*>(unit + ROWS);  // [ROWS]
   float* inner = own + ROWS * RP;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int ctas = static_cast<int>(lr_cluster_size()), rank = static_cast<int>(lr_cluster_rank());
   const int tile = blockIdx.x / ctas;
+  const uint32_t queue = static_cast<uint32_t>(__cvta_generic_to_shared(sm)) + warp * (STEPS * S::STEP_BYTES) + lane * 16;
+  auto slot = [&](int step, int piece) { return queue + static_cast<uint32_t>((step * S::PIECES + piece) * 512); };
 
-  auto plain_row = [&](int64_t r) {  // a route without a set
-    const int64_t step = a.out32 ? 4 : 2;
-    for (int64_t n = tid; n < a.width; n += LR_THREADS) {
-      if (step == 4) static_cast<uint32_t*>(a.out)[r * a.out_ld + n] = a.base ? static_cast<const uint32_t*>(a.base)[r * a.base_ld + n] : 0u;
-      else static_cast<uint16_t*>(a.out)[r * a.out_ld + n] = a.base ? static_cast<const uint16_t*>(a.base)[r * a.base_ld + n] : static_cast<uint16_t>(0);
+  auto plain_row = [&](int64_t r) {  // a route without a set: its base, bit for bit
+    const int size = a.out32 ? 4 : 2;
+    char* to = static_cast<char*>(a.out) + r * a.out_ld * size;
+    const char* from = a.base ? static_cast<const char*>(a.base) + r * a.base_ld * size : nullptr;
+    if (a.whole) {
+      const int n = static_cast<int>(a.width * size / 16);
+#pragma unroll 4
+      for (int i = tid; i < n; i += LR_THREADS) reinterpret_cast<uint4*>(to)[i] = from ? reinterpret_cast<const uint4*>(from)[i] : make_uint4(0, 0, 0, 0);
+    } else if (size == 4) {
+      for (int i = tid; i < a.width; i += LR_THREADS) reinterpret_cast<uint32_t*>(to)[i] = from ? reinterpret_cast<const uint32_t*>(from)[i] : 0u;
+    } else {
+      for (int i = tid; i < a.width; i += LR_THREADS) reinterpret_cast<uint16_t*>(to)[i] = from ? reinterpret_cast<const uint16_t*>(from)[i] : static_cast<uint16_t>(0);
     }
   };
   int set, start = 0, size = 1;
@@ -170,21 +213,62 @@ __global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) 
     for (int m = 0; m < MT; ++m)
 #pragma unroll
       for (int h = 0; h < 2; ++h) row[m][h] = route_of[m * 16 + h * 8 + g] / a.in_div;
-    const int64_t factor = static_cast<int64_t>(set) * a.rank * a.depth;
-#pragma unroll 2
-    for (int64_t k0 = (rank * LR_WARPS + warp) * CHUNK; k0 < a.depth; k0 += ctas * LR_WARPS * CHUNK) {
-      const int64_t k = k0 + q * 8;
-      const bool there = k < a.in_ld;  // (values of `in` between depth and in_ld are zeros)
+    // (rows and ranks times row lengths in bytes are 32 x 32 bit products: one instruction an address)
+    const int depth = static_cast<int>(a.depth), in_ld = static_cast<int>(a.in_ld), in_bytes = in_ld * 2, stride = ctas * LR_WARPS * CHUNK, k_first = (rank * LR_WARPS + warp) * CHUNK;
+    const char* in_k = reinterpret_cast<const char*>(a.in + k_first + q * 8);
+    const int factor_bytes = BACK ? a.rank * 2 : depth * 2;
+    const char* factor_k = reinterpret_cast<const char*>(a.first + static_cast<int64_t>(set) * a.rank * depth) +
+                           (BACK ? static_cast<int64_t>(k_first + 8 * (g >> 1) + (g & 1)) * factor_bytes + q * V * 2 : static_cast<int64_t>(g) * factor_bytes + (k_first + q * 8) * 2);
+    int k_fill = k_first;
+    // the pieces of the next 32 values of the contraction, to the queue's step `at`
+    auto fill = [&](int at) {
+      const bool there = k_fill + q * 8 < in_ld;  // (values of `in` between depth and in_ld are zeros)
+#pragma unroll
+      for (int m = 0; m < MT; ++m)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) copy16(slot(at, 2 * m + h), in_k + static_cast<int64_t>(row[m][h]) * in_bytes, there);
+      if (!BACK) {
+#pragma unroll
+        for (int n = 0; n < RT; ++n) copy16(slot(at, 2 * MT + n), factor_k + static_cast<int64_t>(n * 8) * factor_bytes, there && n * 8 + g < a.rank);
+        factor_k += stride * 2;
+      } else {
+        // the factor's rows lie along the contraction: 8 x 8 blocks of it are transposed in registers.  Row i of a
+        // block is the contraction index that the other operand's lane order wants there.
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int more = 4 * (i >> 1) + 2 * (i & 1);
+          const bool is = k_fill + 8 * (g >> 1) + (g & 1) + more < depth;
+#pragma unroll
+          for (int c = 0; c < CC; ++c) {
+            const char* from = factor_k + static_cast<int64_t>(more) * factor_bytes + c * 4 * V * 2;
+            if (V == 8) copy16(slot(at, 2 * MT + i * CC + c), from, is && c * 4 * V + q * V < a.rank);
+            else copy8(slot(at, 2 * MT + i * CC + c), from, is && c * 4 * V + q * V < a.rank);
+          }
+        }
+        factor_k += static_cast<int64_t>(stride) * factor_bytes;
+      }
+      in_k += stride * 2;
+      k_fill += stride;
+    };
+#pragma unroll
+    for (int i = 0; i < STEPS - 1; ++i) {
+      if (k_fill < depth) fill(i);
+      step_issued();
+    }
+    int at = 0;
+    for (int k0 = k_first; k0 < depth; k0 += stride) {
+      if (k_fill < depth) fill(at == 0 ? STEPS - 1 : at - 1);
+      step_issued();
+      all_but<STEPS - 1>();
       uint4 v[MT][2];
 #pragma unroll
       for (int m = 0; m < MT; ++m)
 #pragma unroll
-        for (int h = 0; h < 2; ++h) v[m][h] = load16(a.in + row[m][h] * a.in_ld + k, there);
+        for (int h = 0; h < 2; ++h) v[m][h] = piece16(slot(at, 2 * m + h));
       if (!BACK) {
 #pragma unroll
         for (int n = 0; n < RT; ++n) {
-          const int j = n * 8 + g;
-          const uint4 w = load16(a.first + factor + j * a.depth + k, j < a.rank && there);
+          const uint4 w = piece16(slot(at, 2 * MT + n));
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
             const uint32_t a0[4] = {v[m][0].x, v[m][1].x, v[m][0].y, v[m][1].y}, a1[4] = {v[m][0].z, v[m][1].z, v[m][0].w, v[m][1].w};
@@ -193,27 +277,14 @@ __global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) 
           }
         }
       } else {
-        // the factor's rows lie along the contraction: 8 x 8 blocks of it are transposed in registers.  Row i of a
-        // block is the contraction index that the other operand's lane order wants there.
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const int64_t r0 = k0 + 8 * (g >> 1) + 4 * j + (g & 1);
 #pragma unroll
-          for (int c = 0; c < RP / (4 * V); ++c) {
-            uint32_t w0[V / 2], w1[V / 2];
-            const int col = c * 4 * V + q * V;
-            const bool in_rank = col < a.rank;
-            if (V == 8) {
-              const uint4 x0 = load16(a.first + factor + r0 * a.rank + col, in_rank && r0 < a.depth), x1 = load16(a.first + factor + (r0 + 2) * a.rank + col, in_rank && r0 + 2 < a.depth);
-#pragma unroll
-              for (int t = 0; t < V / 2; ++t) { w0[t] = word(x0, t); w1[t] = word(x1, t); }
-            } else {
-              const uint2 x0 = load8(a.first + factor + r0 * a.rank + col, in_rank && r0 < a.depth), x1 = load8(a.first + factor + (r0 + 2) * a.rank + col, in_rank && r0 + 2 < a.depth);
-              w0[0] = x0.x; w0[1] = x0.y; w1[0] = x1.x; w1[1] = x1.y;
-            }
+          for (int c = 0; c < CC; ++c) {
+            const uint4 w0 = piece16(slot(at, 2 * MT + 2 * j * CC + c)), w1 = piece16(slot(at, 2 * MT + (2 * j + 1) * CC + c));
 #pragma unroll
             for (int t = 0; t < V / 2; ++t) {
-              const uint32_t b0 = transpose8(w0[t]), b1 = transpose8(w1[t]);
+              const uint32_t b0 = transpose8(word(w0, t)), b1 = transpose8(word(w1, t));
 #pragma unroll
               for (int m = 0; m < MT; ++m) {
                 const uint32_t av[4] = {j ? v[m][0].z : v[m][0].x, j ? v[m][1].z : v[m][1].x, j ? v[m][0].w : v[m][0].y, j ? v[m][1].w : v[m][1].y};
@@ -223,7 +294,10 @@ __global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) 
           }
         }
       }
+      if (++at == STEPS) at = 0;
     }
+    all_but<0>();
+    __syncthreads();  // the queues make room for the partial sums
     // a lane's ranks of tile n: 8 n + 2 q and the next; transposed: c * 4 V + V q + 2 t and the next
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -284,7 +358,59 @@ __global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) 
 
   // ---- the second product: [ROWS, RP] times the factor -> [ROWS, width], 32 columns per warp and step
   if (a.second) {
-    constexpr int KC = RP / 16;  // contraction steps
+    const bool queued_base = a.base && a.whole && !a.out32;
+    const int width = static_cast<int>(a.width), stride = ctas * LR_WARPS * 32, n_first = (rank * LR_WARPS + warp) * 32, size_of = a.out32 ? 4 : 2;
+    const int factor_bytes = BACK ? width * 2 : a.rank * 2, base_bytes = static_cast<int>(a.base_ld) * size_of, out_bytes = static_cast<int>(a.out_ld) * size_of;
+    const char* factor_n = reinterpret_cast<const char*>(a.second + static_cast<int64_t>(set) * a.rank * width) +
+                           (BACK ? static_cast<int64_t>((V == 8 ? 8 : 4) * (g >> 1) + (g & 1)) * factor_bytes + (n_first + 8 * q) * 2 : static_cast<int64_t>(n_first + 8 * (g >> 1) + (g & 1)) * factor_bytes + q * V * 2);
+    const char* base_n = static_cast<const char*>(a.base) + (n_first + 8 * q) * 2;
+    char* out_n = static_cast<char*>(a.out) + (n_first + 8 * q) * size_of;
+    int route[MT][2];
+#pragma unroll
+    for (int m = 0; m < MT; ++m)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) route[m][h] = route_of[m * 16 + h * 8 + g];
+    int n_fill = n_first;
+    // the pieces of the next 32 columns: the factor by RP, whose column c of tile t is 8 (c / 2) + 2 t + c % 2, so that a
+    // lane's results are neighbours; and the base of all rows
+    auto fill = [&](int at) {
+      if (!BACK) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const bool is = n_fill + 8 * (g >> 1) + 2 * t + (g & 1) < width;
+#pragma unroll
+          for (int c = 0; c < CC; ++c) {
+            const char* src = factor_n + static_cast<int64_t>(2 * t) * factor_bytes + c * 4 * V * 2;
+            if (V == 8) copy16(slot(at, t * CC + c), src, is && c * 4 * V + q * V < a.rank);
+            else copy8(slot(at, t * CC + c), src, is && c * 4 * V + q * V < a.rank);
+          }
+        }
+        factor_n += static_cast<int64_t>(stride) * factor_bytes;
+      } else {
+        const bool is = n_fill + 8 * q < width;
+#pragma unroll
+        for (int c = 0; c < KC; ++c)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int more = (V == 8 ? c / 2 * 32 + 4 * (c & 1) : 0) + 2 * i;
+            copy16(slot(at, 2 * c + i), factor_n + static_cast<int64_t>(more) * factor_bytes, is && (V == 8 ? 8 : 4) * (g >> 1) + (g & 1) + more < a.rank);
+          }
+        factor_n += stride * 2;
+      }
+      if (queued_base) {
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) copy16(slot(at, S::FACTOR2 + 2 * m + h), base_n + static_cast<int64_t>(route[m][h]) * base_bytes, m * 16 + h * 8 + g < size && n_fill + 8 * q < width);
+        base_n += stride * 2;
+      }
+      n_fill += stride;
+    };
+#pragma unroll
+    for (int i = 0; i < STEPS - 1; ++i) {
+      if (n_fill < width) fill(i);
+      step_issued();
+    }
     uint32_t high[MT][KC][4], low[MT][KC][4];
 #pragma unroll
     for (int m = 0; m < MT; ++m)
@@ -298,39 +424,32 @@ __global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) 
           const float u = Mma<T>::SCALED ? 1.0f / unit[r] : 1.0f;  // (a power of two)
           split<T>(v.x * u, v.y * u, high[m][c][i], low[m][c][i]);
         }
-    const int64_t factor = static_cast<int64_t>(set) * a.rank * a.width;
-    for (int64_t n0 = (rank * LR_WARPS + warp) * 32; n0 < a.width; n0 += ctas * LR_WARPS * 32) {
-      uint32_t b[4][KC][2];  // the factor: 32 columns by RP.  Column c of tile t is n0 + 8 (c / 2) + 2 t + c % 2: a lane's results are neighbours
+    int at = 0;
+    for (int n0 = n_first; n0 < width; n0 += stride, out_n += stride * size_of) {
+      if (n_fill < width) fill(at == 0 ? STEPS - 1 : at - 1);
+      step_issued();
+      all_but<STEPS - 1>();
+      uint32_t b[4][KC][2];
       if (!BACK) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int64_t n = n0 + 8 * (g >> 1) + 2 * t + (g & 1);
+        for (int t = 0; t < 4; ++t)
 #pragma unroll
-          for (int c = 0; c < RP / (4 * V); ++c) {
-            const int j = c * 4 * V + q * V;
-            const bool there = n < a.width && j < a.rank;
-            if (V == 8) {
-              const uint4 w = load16(a.second + factor + n * a.rank + j, there);
-              b[t][(2 * c) % KC][0] = w.x; b[t][(2 * c) % KC][1] = w.y;
-              b[t][(2 * c + 1) % KC][0] = w.z; b[t][(2 * c + 1) % KC][1] = w.w;
-            } else {
-              const uint2 w = load8(a.second + factor + n * a.rank + j, there);
-              b[t][0][0] = w.x; b[t][0][1] = w.y;
-            }
+          for (int c = 0; c < CC; ++c) {
+            const uint4 w = piece16(slot(at, t * CC + c));
+            b[t][(2 * c) % KC][0] = w.x; b[t][(2 * c) % KC][1] = w.y;
+            if (V == 8) { b[t][(2 * c + 1) % KC][0] = w.z; b[t][(2 * c + 1) % KC][1] = w.w; }
           }
-        }
       } else {
 #pragma unroll
         for (int c = 0; c < KC; ++c)
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const int j = (V == 8 ? c / 2 * 32 + 8 * (g >> 1) + 4 * (c & 1) : 4 * (g >> 1)) + (g & 1) + 2 * i;
-            const uint4 w = load16(a.second + factor + j * a.width + n0 + 8 * q, j < a.rank && n0 + 8 * q < a.width);
+            const uint4 w = piece16(slot(at, 2 * c + i));
 #pragma unroll
             for (int t = 0; t < 4; ++t) b[t][c][i] = transpose8(word(w, t));
           }
       }
-      const int64_t n = n0 + 8 * q;
+      const int n = n0 + 8 * q;
 #pragma unroll
       for (int m = 0; m < MT; ++m) {
         if (m * 16 >= size) break;
@@ -339,44 +458,54 @@ __global__ void __launch_bounds__(LR_THREADS, 2) low_rank_kernel(LowRankArgs a) 
         for (int t = 0; t < 4; ++t) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) d[t][i] = 0.0f;
+        }
 #pragma unroll
-          for (int c = 0; c < KC; ++c) {
-            Mma<T>::run(d[t], low[m][c], b[t][c][0], b[t][c][1]);
-            Mma<T>::run(d[t], high[m][c], b[t][c][0], b[t][c][1]);
-          }
+        for (int c = 0; c < KC; ++c) {
+#pragma unroll
+          for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], low[m][c], b[t][c][0], b[t][c][1]);
+#pragma unroll
+          for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], high[m][c], b[t][c][0], b[t][c][1]);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int r = m * 16 + h * 8 + g;
           if (r >= size) continue;
-          const int64_t route = route_of[r], at = route * a.out_ld + n, from = route * a.base_ld + n;
+          char* to = out_n + static_cast<int64_t>(route[m][h]) * out_bytes;
           const float s = Mma<T>::SCALED ? a.second_scale * unit[r] : a.second_scale;
           float y[8];
 #pragma unroll
           for (int t = 0; t < 4; ++t) { y[2 * t] = s * d[t][2 * h]; y[2 * t + 1] = s * d[t][2 * h + 1]; }
           if (a.whole) {
-            if (n >= a.width) continue;
-            float v[8] = {};
+            if (n >= width) continue;
             if (a.out32) {
-              if (a.base) load8_as_float(static_cast<const float*>(a.base) + from, v);
+              float v[8] = {};
+              if (a.base) load8_as_float(static_cast<const float*>(a.base) + route[m][h] * a.base_ld + n, v);
 #pragma unroll
               for (int i = 0; i < 8; ++i) v[i] += y[i];
-              store8_from_float(static_cast<float*>(a.out) + at, v);
+              store8_from_float(reinterpret_cast<float*>(to), v);
             } else {
-              if (a.base) load8_as_float(static_cast<const T*>(a.base) + from, v);
+              if (a.base) {
+                const uint4 rest = piece16(slot(at, S::FACTOR2 + 2 * m + h));
 #pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] += y[i];
-              store8_from_float(static_cast<T*>(a.out) + at, v);
+                for (int i = 0; i < 4; ++i) {
+                  const float2 v = Mma<T>::unpack(word(rest, i));
+                  y[2 * i] += v.x;
+                  y[2 * i + 1] += v.y;
+                }
+              }
+              store8_from_float(reinterpret_cast<T*>(to), y);
             }
           } else {
             const int dtype = a.out32 ? KEEPVQ_F32 : Mma<T>::SCALED ? KEEPVQ_F16 : KEEPVQ_BF16;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
-              if (n + i < a.width) store_from_float(a.out, dtype, at + i, y[i] + (a.base ? load_as_float(a.base, dtype, from + i) : 0.0f));
+              if (n + i < width) store_from_float(to, dtype, i, y[i] + (a.base ? load_as_float(a.base, dtype, route[m][h] * a.base_ld + n + i) : 0.0f));
           }
         }
       }
+      if (++at == STEPS) at = 0;
     }
+    all_but<0>();
   }
   if (ctas > 1) lr_cluster_sync();  // the others may still be reading this CTA's partial sums
 }
@@ -512,14 +641,14 @@ struct LowRankPlan {
   int64_t tiles;  // at most
 };
 // One row per tile while there are no more rows than SMs: no plan to wait for, and rows that share a set
-// read it from the cache.  Else tiles of 16 rows, or of as many as 64 sums a lane allow where sets have more.
+// read it from the cache.  Else tiles of 16 rows, or of more where sets have them and registers allow.
 // Clusters while there are not tiles enough for two CTAs on every SM.
 static LowRankPlan plan_low_rank(int64_t routes, int64_t sets, int64_t rank, bool grads) {
   LowRankPlan p;
   p.rp = rank_pad(rank);
   p.solo = !grads && routes <= 148;
   const int64_t used = routes < sets ? routes : sets;
-  p.mt = p.solo || routes <= 16 * used ? 1 : 128 / p.rp;
+  p.mt = p.solo || routes <= 16 * used ? 1 : p.rp <= 16 ? 4 : p.rp <= 64 ? 2 : 1;
   p.tiles = p.solo ? routes : max_tiles(routes, sets, p.mt * 16);
   const int64_t expected = p.solo ? routes : routes / (p.mt * 16) + used / 2 + 1;
   p.ctas = 1;
@@ -529,7 +658,7 @@ static LowRankPlan plan_low_rank(int64_t routes, int64_t sets, int64_t rank, boo
 
 template <typename T, int RP, int MT, bool BACK>
 static int launch_low_rank(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
-  constexpr int SMEM = ((LR_WARPS + 2) * MT * 16 * RP + 2 * MT * 16) * 4;
+  constexpr int SMEM = LowRankShape<RP, MT, BACK>::BYTES;
   auto kernel = low_rank_kernel<T, RP, MT, BACK>;
   if (SMEM > 48 * 1024) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
@@ -541,9 +670,14 @@ static int launch_low_rank(const LowRankArgs& a, const LowRankPlan& p, cudaStrea
   config.dynamicSmemBytes = SMEM;
   config.stream = s;
   cudaLaunchAttribute attribute = {};
-  attribute.id = cudaLaunchAttributeClusterDimension;
-  attribute.val.clusterDim.x = static_cast<unsigned>(p.ctas);
-  attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  if (p.ctas > 1) {  // (no early start of clusters, switch_matmul.cu)
+    attribute.id = cudaLaunchAttributeClusterDimension;
+    attribute.val.clusterDim.x = static_cast<unsigned>(p.ctas);
+    attribute.val.clusterDim.y = attribute.val.clusterDim.z = 1;
+  } else {
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+  }
   config.attrs = &attribute;
   config.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
@@ -551,8 +685,8 @@ static int launch_low_rank(const LowRankArgs& a, const LowRankPlan& p, cudaStrea
 }
 template <typename T, bool BACK>
 static int launch_low_rank_of(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
-  if (p.rp == 16) return p.mt == 1 ? launch_low_rank<T, 16, 1, BACK>(a, p, s) : launch_low_rank<T, 16, 8, BACK>(a, p, s);
-  if (p.rp == 32) return p.mt == 1 ? launch_low_rank<T, 32, 1, BACK>(a, p, s) : launch_low_rank<T, 32, 4, BACK>(a, p, s);
+  if (p.rp == 16) return p.mt == 1 ? launch_low_rank<T, 16, 1, BACK>(a, p, s) : launch_low_rank<T, 16, 4, BACK>(a, p, s);
+  if (p.rp == 32) return p.mt == 1 ? launch_low_rank<T, 32, 1, BACK>(a, p, s) : launch_low_rank<T, 32, 2, BACK>(a, p, s);
   if (p.rp == 64) return p.mt == 1 ? launch_low_rank<T, 64, 1, BACK>(a, p, s) : launch_low_rank<T, 64, 2, BACK>(a, p, s);
   return launch_low_rank<T, 128, 1, BACK>(a, p, s);
 }
