@@ -526,7 +526,7 @@ typedef struct keepvq_switch_low_rank_args {
   void* dx;               /* [routes / x_div, in_dim] or NULL (grads only) */
   void* dleft;            /* [sets, out_dim, rank] or NULL (grads only) */
   void* dright;           /* [sets, rank, in_dim] or NULL (grads only) */
-  void* workspace;        /* keepvq_switch_low_rank_workspace_bytes(), 256-byte aligned */
+  void* workspace;        /* keepvq_switch_low_rank_workspace_bytes(), 256-byte aligned; NULL where that is 0 */
   int64_t workspace_bytes;
 } keepvq_switch_low_rank_args;
 

@@ -304,6 +304,14 @@ def stream_handle(device: torch.device) -> c_void_p:
     return c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def raw_stream(device: torch.device) -> int:
+    """The current stream of a device as a number, without a Stream object where torch offers that (3 us a call)."""
+    return _raw_stream(device.index) if _raw_stream is not None else torch.cuda.current_stream(device).cuda_stream
+
+
 def require_cuda(*tensors: torch.Tensor) -> torch.device:
     """All tensors on one CUDA device; that device is returned.  CPU tensors are refused: the
     operators never compute on the host."""

@@ -927,7 +927,8 @@ struct LowRankPlan {
 };
 // One row per tile while there are no more rows than SMs: no plan to wait for, and rows that share a set
 // read it from the cache.  Else tiles of 16 rows, or of 64 where sets have more than 16 on average.
-// Clusters while there are not tiles enough for two CTAs on every SM.
+// Clusters while there are not tiles enough for two CTAs on every SM; sets that few rows name make fewer 64-row
+// tiles than this expects (rows of a prompt have one adapter): four there (4096 rows of rank 64: 57 -> 50 us).
 static LowRankPlan plan_low_rank(int64_t routes, int64_t sets, int64_t rank, bool grads) {
   LowRankPlan p;
   p.rp = rank_pad(rank);
@@ -937,14 +938,18 @@ static LowRankPlan plan_low_rank(int64_t routes, int64_t sets, int64_t rank, boo
   p.tiles = p.solo ? routes : max_tiles(routes, sets, p.rows);
   const int64_t expected = p.solo ? routes : routes / p.rows + used / 2 + 1;
   p.ctas = 1;
-  while (p.ctas < 8 && 2 * p.ctas * expected <= 296) p.ctas *= 2;
+  while (p.ctas < 8 && 2 * p.ctas * expected <= (p.rows == TILE_ROWS ? 592 : 296)) p.ctas *= 2;
   return p;
 }
 
-static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
-  if (bytes > 48 * 1024) {
+// `configured`: a bit per device, the shared-memory opt-in is a per-device attribute of the function.
+static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, uint64_t& configured, const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !((configured >> dev) & 1ull)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return note_cuda_error(e);
+    if (dev >= 0 && dev < 64) configured |= 1ull << dev;
   }
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(static_cast<unsigned>(p.tiles * p.ctas));
@@ -967,8 +972,9 @@ static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, const 
 }
 template <typename T, int RP, bool BACK>
 static int launch_low_rank(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
-  if (p.rows == TILE_ROWS) return launch_low_rank_kernel(low_rank_tile_kernel<T, RP, BACK>, TileShape<RP>::BYTES, a, p, s);
-  return launch_low_rank_kernel(low_rank_kernel<T, RP, BACK>, LowRankShape<RP, BACK>::BYTES, a, p, s);
+  static uint64_t configured[2] = {0, 0};
+  if (p.rows == TILE_ROWS) return launch_low_rank_kernel(low_rank_tile_kernel<T, RP, BACK>, TileShape<RP>::BYTES, configured[0], a, p, s);
+  return launch_low_rank_kernel(low_rank_kernel<T, RP, BACK>, LowRankShape<RP, BACK>::BYTES, configured[1], a, p, s);
 }
 template <typename T, bool BACK>
 static int launch_low_rank_of(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
@@ -1015,7 +1021,8 @@ static LowRankLayout lay_out_low_rank(void* base, int64_t routes, int64_t sets, 
   Scratch s{static_cast<char*>(base)};
   const LowRankPlan p = plan_low_rank(routes, sets, rank, grads);
   const int64_t blocks = max_places(routes, sets) / ROW_STEP + 1, values = grads ? blocks * ROW_STEP * p.rp : 0;
-  LowRankLayout l;
+  LowRankLayout l = {};
+  if (p.solo) return l;  // (nothing to keep: 0 bytes)
   l.plan = take_plan(s, routes, sets, p.rows);
   for (Inner* i : {&l.inner, &l.back}) {
     i->high = s.take<uint16_t>(values);
@@ -1038,7 +1045,7 @@ static int check_low_rank(const keepvq_switch_low_rank_args& a, bool grads) {
   if (!valid_16bit(a.dtype) || (a.index_bits != 32 && a.index_bits != 64) || (!grads && a.out_dtype != a.dtype && a.out_dtype != KEEPVQ_F32)) return KEEPVQ_ERR_DTYPE;
   if (const int rc = check_low_rank_sizes(a.routes, a.sets, a.out_dim, a.in_dim, a.rank, a.x_div)) return rc;
   if (grads ? a.grad_ld < a.out_dim || a.grad_ld % 8 != 0 : a.out_ld < a.out_dim || (a.base && a.base_ld < a.out_dim)) return KEEPVQ_ERR_SHAPE;
-  if (!a.workspace || (a.routes > 0 && (!a.x || !a.left || !a.right || !a.indices || (grads ? !a.grad : !a.out)))) return KEEPVQ_ERR_NULL;
+  if (a.routes > 0 && (!a.x || !a.left || !a.right || !a.indices || (grads ? !a.grad : !a.out))) return KEEPVQ_ERR_NULL;
   for (const void* p : {a.x, a.left, a.right, a.grad, static_cast<const void*>(a.dx), static_cast<const void*>(a.dleft), static_cast<const void*>(a.dright)})
     if (!aligned_to(p, 16)) return KEEPVQ_ERR_ALIGN;
   if (!aligned_to(a.workspace, 256) || !aligned_to(a.indices, a.index_bits / 8) || !aligned_to(a.base, dtype_size(a.out_dtype)) || !aligned_to(a.out, dtype_size(a.out_dtype))) return KEEPVQ_ERR_ALIGN;
@@ -1063,6 +1070,7 @@ int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream
   if (const int rc = check_low_rank(a, false)) return rc;
   const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.in_dim, a.rank, a.x_div, false);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
+  if (l.bytes > 0 && !a.workspace) return KEEPVQ_ERR_NULL;
   if (a.routes == 0) return KEEPVQ_OK;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   const LowRankPlan p = plan_low_rank(a.routes, a.sets, a.rank, false);
@@ -1100,6 +1108,7 @@ int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* 
   if (const int rc = check_low_rank(a, true)) return rc;
   const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.in_dim, a.rank, a.x_div, true);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
+  if (l.bytes > 0 && !a.workspace) return KEEPVQ_ERR_NULL;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (a.routes == 0) {
     for (void* p : {a.dleft, a.dright}) {

@@ -32,29 +32,30 @@ _DTYPES = (torch.float16, torch.bfloat16)
 
 
 def _indices(indices, device) -> torch.Tensor:
-    indices = as_device(indices, device)
-    if indices.dtype.is_floating_point or indices.dtype.is_complex or indices.dtype == torch.bool:
-        raise ValueError(f"indices must use an integer dtype, found {indices.dtype}")
-    if indices.ndim < 1:
-        raise ValueError("indices must have at least one dimension")
-    if indices.dtype == torch.uint32:  # 0xFFFFFFFF, a pick without an expert, becomes -1: same bits
-        indices = indices.view(torch.int32)
-    elif indices.dtype not in (torch.int32, torch.int64):
-        indices = indices.to(torch.int64)
+    if not (isinstance(indices, torch.Tensor) and indices.dtype in (torch.int32, torch.int64) and indices.device == device):
+        indices = as_device(indices, device)
+        if indices.dtype.is_floating_point or indices.dtype.is_complex or indices.dtype == torch.bool:
+            raise ValueError(f"indices must use an integer dtype, found {indices.dtype}")
+        if indices.dtype == torch.uint32:  # 0xFFFFFFFF, a pick without an expert, becomes -1: same bits
+            indices = indices.view(torch.int32)
+        elif indices.dtype not in (torch.int32, torch.int64):
+            indices = indices.to(torch.int64)
     return indices.contiguous()
 
 
-def _x_div(x: torch.Tensor, indices: torch.Tensor, in_dim: int) -> int:
-    """Routes per row of x: 1, or the picks of a token."""
-    if x.ndim < 1 or int(x.shape[-1]) != in_dim:
-        raise ValueError(f"x trailing dimension must be {in_dim}, found {tuple(x.shape)}")
-    if tuple(x.shape[:-1]) == tuple(indices.shape):
-        return 1
-    if tuple(x.shape[:-1]) == tuple(indices.shape[:-1]):
-        return int(indices.shape[-1])
+def _x_div(x_shape, indices_shape, in_dim: int) -> tuple[int, int]:
+    """Routes per row of x (1, or the picks of a token), and routes."""
+    if len(indices_shape) < 1:
+        raise ValueError("indices must have at least one dimension")
+    if len(x_shape) < 1 or x_shape[-1] != in_dim:
+        raise ValueError(f"x trailing dimension must be {in_dim}, found {tuple(x_shape)}")
+    if x_shape[:-1] == indices_shape:
+        return 1, indices_shape.numel()
+    if x_shape[:-1] == indices_shape[:-1]:
+        return indices_shape[-1], indices_shape.numel()
     raise ValueError(
         "x leading shape must either match indices leading shape for "
-        f"token routing or the full indices shape for per-route routing; found x {tuple(x.shape)} and indices {tuple(indices.shape)}")
+        f"token routing or the full indices shape for per-route routing; found x {tuple(x_shape)} and indices {tuple(indices_shape)}")
 
 
 def _dense(t: torch.Tensor) -> torch.Tensor:
@@ -76,7 +77,22 @@ def _no_capture(what: str, grads: str) -> None:
         raise _lib.KeepVQError(f"{what}: a recorded gradient cannot be captured; capture the call under torch.no_grad() and {grads}")
 
 
-@lru_cache(maxsize=256)
+@lru_cache(maxsize=1024)
+def _problem(x_shape, weight_shape, indices_shape, x_dtype, weight_dtype) -> tuple:
+    """What follows from shapes and types alone, checked once for each: (routes per row of x, routes, experts, out, in, dtype tag,
+    result's shape)."""
+    if x_dtype not in _DTYPES or weight_dtype != x_dtype:
+        raise ValueError(f"x and weight must share one of fp16 / bf16, found {x_dtype} and {weight_dtype}")
+    if len(weight_shape) != 3 or 0 in weight_shape:
+        raise ValueError(f"weight must be [experts, out, in], found {tuple(weight_shape)}")
+    experts, out_dim, in_dim = weight_shape
+    if in_dim % 8 != 0:
+        raise ValueError("the input dimension must be divisible by 8")
+    x_div, routes = _x_div(x_shape, indices_shape, in_dim)
+    return max(x_div, 1), routes, experts, out_dim, in_dim, _lib.dtype_tag(x_dtype), (*indices_shape, out_dim)
+
+
+@lru_cache(maxsize=1024)
 def _scratch_bytes(routes: int, experts: int, out_dim: int, in_dim: int, x_div: int, grads: bool) -> int:
     nbytes = int(_lib.load().keepvq_switch_matmul_workspace_bytes(routes, experts, out_dim, in_dim, x_div, int(grads)))
     if nbytes < 0:
@@ -85,36 +101,29 @@ def _scratch_bytes(routes: int, experts: int, out_dim: int, in_dim: int, x_div: 
 
 
 def _check(x: torch.Tensor, weight: torch.Tensor, indices):
-    if x.dtype not in _DTYPES or weight.dtype != x.dtype:
-        raise ValueError(f"x and weight must share one of fp16 / bf16, found {x.dtype} and {weight.dtype}")
-    if weight.ndim != 3 or 0 in weight.shape:
-        raise ValueError(f"weight must be [experts, out, in], found {tuple(weight.shape)}")
-    if int(weight.shape[2]) % 8 != 0:
-        raise ValueError("the input dimension must be divisible by 8")
+    shape = indices.shape if isinstance(indices, torch.Tensor) else torch.as_tensor(indices).shape
+    problem = _problem(x.shape, weight.shape, shape, x.dtype, weight.dtype)
     device = _lib.require_cuda(x, weight)
-    indices = _indices(indices, device)
-    x_div = _x_div(x, indices, int(weight.shape[2]))
-    return device, indices, x_div, tuple(indices.shape) + (int(weight.shape[1]),)
+    return device, _indices(indices, device), problem
 
 
-def _call(name: str, device, x, weight, grad, indices, x_div, grad_ld, out, dx, dweight):
-    experts, out_dim, in_dim = (int(s) for s in weight.shape)
-    routes = indices.numel()
-    nbytes = _scratch_bytes(routes, experts, out_dim, in_dim, max(x_div, 1), grad is not None)
+def _call(name: str, device, x, weight, grad, indices, problem, grad_ld, out, dx, dweight):
+    x_div, routes, experts, out_dim, in_dim, tag, _ = problem
+    nbytes = _scratch_bytes(routes, experts, out_dim, in_dim, x_div, grad is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device)  # of this call alone, as every scratch of the operators
-    address = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
     args = _lib.pack_switch_matmul_args(
-        x.data_ptr(), weight.data_ptr(), address(grad), _lib.dtype_tag(x.dtype), indices.data_ptr(), 8 * indices.element_size(), max(x_div, 1), routes,
-        experts, out_dim, in_dim, grad_ld, address(out), address(dx), address(dweight), ws.data_ptr(), nbytes)
+        x.data_ptr(), weight.data_ptr(), 0 if grad is None else grad.data_ptr(), tag, indices.data_ptr(), 64 if indices.dtype == torch.int64 else 32, x_div, routes,
+        experts, out_dim, in_dim, grad_ld, 0 if out is None else out.data_ptr(), 0 if dx is None else dx.data_ptr(), 0 if dweight is None else dweight.data_ptr(),
+        ws.data_ptr(), nbytes)
     with _lib.on_device(device):
-        _lib.check(getattr(_lib.load(), name)(args, _lib.stream_handle(device)), name)
+        _lib.check(getattr(_lib.load(), name)(args, _lib.raw_stream(device)), name)
 
 
 def _forward(x, weight, indices) -> torch.Tensor:
-    device, indices, x_div, out_shape = _check(x, weight, indices)
-    out = torch.empty(out_shape, dtype=x.dtype, device=device)
-    if out.numel():
-        _call("keepvq_switch_matmul", device, _dense(x), _dense(weight), None, indices, x_div, 0, out, None, None)
+    device, indices, problem = _check(x, weight, indices)
+    out = torch.empty(problem[6], dtype=x.dtype, device=device)
+    if problem[1]:
+        _call("keepvq_switch_matmul", device, _dense(x), _dense(weight), None, indices, problem, 0, out, None, None)
     return out
 
 
@@ -123,15 +132,15 @@ def switch_matmul_grads(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     """The gradients of ``x`` and ``weight`` where ``grad`` is that of ``switch_matmul(x, weight, indices)``,
     in their dtype; None for one that is not wanted.  A row's gradient is the fp32 sum over its picks,
     rounded once; experts without routes get zeros."""
-    device, indices, x_div, out_shape = _check(x, weight, indices)
+    device, indices, problem = _check(x, weight, indices)
     _lib.require_cuda(x, grad)
-    grad, grad_ld = _grad_rows(grad, out_shape, x.dtype)
+    grad, grad_ld = _grad_rows(grad, problem[6], x.dtype)
     dx = torch.empty(x.shape, dtype=x.dtype, device=device) if x_grad else None
     dweight = torch.empty(weight.shape, dtype=x.dtype, device=device) if weight_grad else None
     if indices.numel() == 0:
         return dx.zero_() if x_grad else None, dweight.zero_() if weight_grad else None
     if x_grad or weight_grad:
-        _call("keepvq_switch_matmul_grads", device, _dense(x), _dense(weight), grad, indices, x_div, grad_ld, None, dx, dweight)
+        _call("keepvq_switch_matmul_grads", device, _dense(x), _dense(weight), grad, indices, problem, grad_ld, None, dx, dweight)
     return dx, dweight
 
 

@@ -37,32 +37,41 @@ class LowRank:
     scale: float = 1.0
 
     def __post_init__(self):
-        _check_pair(self.left, self.right)
+        _check_pair(self.left.shape, self.right.shape, self.left.dtype, self.right.dtype)
 
     def add(self, base: torch.Tensor, x: torch.Tensor, indices) -> torch.Tensor:
         """``base`` plus the correction of the set that each route names."""
         return switch_low_rank(x, self.left, self.right, indices, base=base, scale=self.scale)
 
 
-def _check_pair(left, right) -> None:
-    if left.dtype not in _DTYPES or right.dtype != left.dtype:
-        raise ValueError(f"left and right must share one of fp16 / bf16, found {left.dtype} and {right.dtype}")
-    if left.ndim != 3 or right.ndim != 3 or left.shape[0] != right.shape[0] or left.shape[2] != right.shape[1] or 0 in left.shape or 0 in right.shape:
-        raise ValueError(f"left must be [sets, out, rank] and right [sets, rank, in], found {tuple(left.shape)} and {tuple(right.shape)}")
-    if int(left.shape[2]) > MAX_RANK:
-        raise ValueError(f"rank must be at most {MAX_RANK}, found {int(left.shape[2])}")
-    if int(right.shape[2]) % 8 != 0:
+def _check_pair(left_shape, right_shape, left_dtype, right_dtype) -> None:
+    if left_dtype not in _DTYPES or right_dtype != left_dtype:
+        raise ValueError(f"left and right must share one of fp16 / bf16, found {left_dtype} and {right_dtype}")
+    if len(left_shape) != 3 or len(right_shape) != 3 or left_shape[0] != right_shape[0] or left_shape[2] != right_shape[1] or 0 in left_shape or 0 in right_shape:
+        raise ValueError(f"left must be [sets, out, rank] and right [sets, rank, in], found {tuple(left_shape)} and {tuple(right_shape)}")
+    if left_shape[2] > MAX_RANK:
+        raise ValueError(f"rank must be at most {MAX_RANK}, found {left_shape[2]}")
+    if right_shape[2] % 8 != 0:
         raise ValueError("the input dimension must be divisible by 8")
 
 
+@lru_cache(maxsize=1024)
+def _problem(x_shape, left_shape, right_shape, indices_shape, x_dtype, left_dtype, right_dtype) -> tuple:
+    """What follows from shapes and types alone, checked once for each: (routes per row of x, routes, sets, out, in, rank rounded
+    up, dtype tag, result's shape)."""
+    _check_pair(left_shape, right_shape, left_dtype, right_dtype)
+    if x_dtype != left_dtype:
+        raise ValueError(f"x must be {left_dtype} as left and right, found {x_dtype}")
+    sets, out_dim, rank = left_shape
+    x_div, routes = _x_div(x_shape, indices_shape, right_shape[2])
+    return max(x_div, 1), routes, sets, out_dim, right_shape[2], -(-rank // 8) * 8, _lib.dtype_tag(x_dtype), (*indices_shape, out_dim)
+
+
 def _check(x, left, right, indices):
-    _check_pair(left, right)
-    if x.dtype != left.dtype:
-        raise ValueError(f"x must be {left.dtype} as left and right, found {x.dtype}")
+    shape = indices.shape if isinstance(indices, torch.Tensor) else torch.as_tensor(indices).shape
+    problem = _problem(x.shape, left.shape, right.shape, shape, x.dtype, left.dtype, right.dtype)
     device = _lib.require_cuda(x, left, right)
-    indices = _indices(indices, device)
-    x_div = _x_div(x, indices, int(right.shape[2]))
-    return device, indices, x_div, tuple(indices.shape) + (int(left.shape[1]),)
+    return device, _indices(indices, device), problem
 
 
 def _whole_ranks(left, right):
@@ -73,7 +82,7 @@ def _whole_ranks(left, right):
     return _dense(left), _dense(right)
 
 
-@lru_cache(maxsize=256)
+@lru_cache(maxsize=1024)
 def _scratch_bytes(routes: int, sets: int, out_dim: int, in_dim: int, rank: int, x_div: int, grads: bool) -> int:
     nbytes = int(_lib.load().keepvq_switch_low_rank_workspace_bytes(routes, sets, out_dim, in_dim, rank, x_div, int(grads)))
     if nbytes < 0:
@@ -81,34 +90,40 @@ def _scratch_bytes(routes: int, sets: int, out_dim: int, in_dim: int, rank: int,
     return nbytes
 
 
-def _call(name, device, x, left, right, grad, indices, x_div, grad_ld, scale, out_dtype, base, base_ld, out, dx, dleft, dright):
-    (sets, out_dim, rank), in_dim, routes = (int(s) for s in left.shape), int(right.shape[2]), indices.numel()
-    nbytes = _scratch_bytes(routes, sets, out_dim, in_dim, rank, max(x_div, 1), grad is not None)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    address = lambda t: 0 if t is None else t.data_ptr()  # noqa: E731
+def _call(name, device, x, left, right, grad, indices, problem, grad_ld, scale, out_tag, base, base_ld, out, dx, dleft, dright):
+    x_div, routes, sets, out_dim, in_dim, rank, tag, _ = problem
+    nbytes = _scratch_bytes(routes, sets, out_dim, in_dim, rank, x_div, grad is not None)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     args = _lib.pack_switch_low_rank_args(
-        x.data_ptr(), left.data_ptr(), right.data_ptr(), address(grad), _lib.dtype_tag(x.dtype), indices.data_ptr(), 8 * indices.element_size(), max(x_div, 1),
-        routes, sets, out_dim, in_dim, rank, grad_ld, float(scale), _lib.dtype_tag(out_dtype), address(base), base_ld, address(out), out_dim,
-        address(dx), address(dleft), address(dright), ws.data_ptr(), nbytes)
+        x.data_ptr(), left.data_ptr(), right.data_ptr(), 0 if grad is None else grad.data_ptr(), tag, indices.data_ptr(), 64 if indices.dtype == torch.int64 else 32,
+        x_div, routes, sets, out_dim, in_dim, rank, grad_ld, scale, out_tag, 0 if base is None else base.data_ptr(), base_ld, 0 if out is None else out.data_ptr(), out_dim,
+        0 if dx is None else dx.data_ptr(), 0 if dleft is None else dleft.data_ptr(), 0 if dright is None else dright.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes)
     with _lib.on_device(device):
-        _lib.check(getattr(_lib.load(), name)(args, _lib.stream_handle(device)), name)
+        _lib.check(getattr(_lib.load(), name)(args, _lib.raw_stream(device)), name)
 
 
 def _forward(x, left, right, indices, base, scale) -> torch.Tensor:
-    device, indices, x_div, out_shape = _check(x, left, right, indices)
-    out_dtype, base_ld, rows = x.dtype, 0, None
-    if base is not None:
-        _lib.require_cuda(x, base)
-        if tuple(base.shape) != out_shape or base.dtype not in (x.dtype, torch.float32):
+    device, indices, problem = _check(x, left, right, indices)
+    out_shape, out_tag, base_ld = problem[7], problem[6], 0
+    if base is None:
+        out = torch.empty(out_shape, dtype=x.dtype, device=device)
+    else:
+        if base.shape != out_shape or base.dtype not in (x.dtype, torch.float32):
             raise ValueError(f"base must be {out_shape} in {x.dtype} or fp32, found {tuple(base.shape)} {base.dtype}")
-        out_dtype = base.dtype
-        # rows may lie apart (one of several projections of a wider product), a row's values may not
-        rows = base if base.ndim == 2 and base.stride(1) == 1 and base.stride(0) >= out_shape[-1] else base.contiguous()
-        base_ld = rows.stride(0) if rows.ndim == 2 and rows.shape[0] > 1 else out_shape[-1]
-    out = torch.empty(out_shape, dtype=out_dtype, device=device)
-    if out.numel():
+        _lib.require_cuda(x, base)
+        out = torch.empty(out_shape, dtype=base.dtype, device=device)
+        if base.dtype != x.dtype:
+            out_tag = _lib.F32
+        base_ld = out_shape[-1]
+        if not base.is_contiguous():
+            # rows may lie apart (one of several projections of a wider product), a row's values may not
+            if base.ndim == 2 and base.stride(1) == 1 and base.stride(0) >= base_ld:
+                base_ld = base.stride(0) if base.shape[0] > 1 else base_ld
+            else:
+                base = base.contiguous()
+    if problem[1]:
         left, right = _whole_ranks(left, right)
-        _call("keepvq_switch_low_rank", device, _dense(x), left, right, None, indices, x_div, 0, scale, out_dtype, rows, base_ld, out, None, None, None)
+        _call("keepvq_switch_low_rank", device, _dense(x), left, right, None, indices, problem, 0, scale, out_tag, base, base_ld, out, None, None, None)
     return out
 
 
@@ -116,9 +131,9 @@ def switch_low_rank_grads(grad: torch.Tensor, x: torch.Tensor, left: torch.Tenso
                           x_grad: bool = True, weight_grad: bool = True):
     """The gradients of ``x``, ``left`` and ``right`` where ``grad`` (in x's dtype) is that of
     ``switch_low_rank(x, left, right, indices, base=..., scale=scale)``; None for those not wanted."""
-    device, indices, x_div, out_shape = _check(x, left, right, indices)
+    device, indices, problem = _check(x, left, right, indices)
     _lib.require_cuda(x, grad)
-    grad, grad_ld = _grad_rows(grad, out_shape, x.dtype)
+    grad, grad_ld = _grad_rows(grad, problem[7], x.dtype)
     rank = int(left.shape[2])
     left, right = _whole_ranks(left, right)
     empty = lambda t, wanted: torch.empty(t.shape, dtype=x.dtype, device=device) if wanted else None  # noqa: E731
@@ -128,7 +143,7 @@ def switch_low_rank_grads(grad: torch.Tensor, x: torch.Tensor, left: torch.Tenso
             if t is not None:
                 t.zero_()
     elif x_grad or weight_grad:
-        _call("keepvq_switch_low_rank_grads", device, _dense(x), left, right, grad, indices, x_div, grad_ld, scale, x.dtype, None, 0, None, dx, dleft, dright)
+        _call("keepvq_switch_low_rank_grads", device, _dense(x), left, right, grad, indices, problem, grad_ld, float(scale), problem[6], None, 0, None, dx, dleft, dright)
     if weight_grad and int(left.shape[2]) != rank:
         dleft, dright = dleft[:, :, :rank].contiguous(), dright[:, :rank].contiguous()
     return dx, dleft, dright

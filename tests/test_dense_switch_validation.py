@@ -64,14 +64,14 @@ def matmul_args(**change):
 
 
 def low_rank_args(**change):
-    a = _lib.SwitchLowRankArgs(x=256, left=256, right=256, grad=256, dtype=1, indices=256, index_bits=32, x_div=2, routes=8, sets=3, out_dim=24, in_dim=16, rank=8,
+    a = _lib.SwitchLowRankArgs(x=256, left=256, right=256, grad=256, dtype=1, indices=256, index_bits=32, x_div=2, routes=800, sets=3, out_dim=24, in_dim=16, rank=8,
                                grad_ld=24, scale=1.0, out_dtype=1, base=256, base_ld=24, out=256, out_ld=24, dx=256, dleft=256, dright=256, workspace=256, workspace_bytes=1 << 30)
     for name, value in change.items():
         setattr(a, name, value)
     return a
 
 
-BOTH = [(dict(dtype=0), DTYPE), (dict(dtype=7), DTYPE), (dict(index_bits=16), DTYPE), (dict(routes=-1), SHAPE), (dict(routes=7), SHAPE), (dict(x_div=0), SHAPE),
+BOTH = [(dict(dtype=0), DTYPE), (dict(dtype=7), DTYPE), (dict(index_bits=16), DTYPE), (dict(routes=-1), SHAPE), (dict(routes=801), SHAPE), (dict(x_div=0), SHAPE),
         (dict(in_dim=12), SHAPE), (dict(out_dim=0), SHAPE), (dict(routes=1 << 25), CAPACITY), (dict(workspace=None), NULL), (dict(workspace=264), ALIGN),
         (dict(workspace_bytes=64), CAPACITY), (dict(x=None), NULL), (dict(indices=None), NULL), (dict(x=258), ALIGN), (dict(indices=258), ALIGN)]
 
@@ -113,6 +113,8 @@ def test_scratch_sizes():
     assert lib.keepvq_switch_matmul_workspace_bytes(8, 3, 24, 12, 2, 0) == SHAPE
     assert lib.keepvq_switch_matmul_workspace_bytes(8, 1 << 15, 24, 16, 2, 0) == CAPACITY
     assert lib.keepvq_switch_low_rank_workspace_bytes(8, 3, 24, 16, 136, 2, 0) == UNSUPPORTED
+    assert lib.keepvq_switch_low_rank_workspace_bytes(8, 3, 24, 16, 8, 2, 0) == 0  # a few rows need none
+    assert lib.keepvq_switch_low_rank_workspace_bytes(8, 3, 24, 16, 8, 2, 1) > 0
     # a row's gradient is summed over its picks in fp32
     assert lib.keepvq_switch_matmul_workspace_bytes(4096, 8, 512, 1024, 2, 1) >= 4096 * 1024 * 4
     assert lib.keepvq_switch_matmul_workspace_bytes(0, 1, 8, 8, 1, 0) > 0
