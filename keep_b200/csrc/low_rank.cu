@@ -10,7 +10,7 @@
 // bytes in flight that cost no registers, and nobody to wait for but the copies.
 //
 // Two products with a vector in between (low_rank_kernel): a cluster of CTAs takes the rows of one set, up
-// to MT * 16, and splits the first contraction over its CTAs and their warps; the partial inner vectors meet in
+// to 16, and splits the first contraction over its CTAs and their warps; the partial inner vectors meet in
 // shared memory, once per CTA and once over the cluster; the CTAs then split the width of the result.  So
 // the inner vectors never leave the SMs, and one row of one set still has a whole cluster's loads in
 // flight.  Forward: A, then B.  Input gradient: B^T, then A^T, whose fragments are transposed in registers.
@@ -523,7 +523,6 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
   }
   if (ctas > 1) lr_cluster_sync();  // the others may still be reading this CTA's partial sums
 }
-
 // ---- the same for many rows of a set -------------------------------------------------------------------
 // 64 rows of a set per cluster, whose CTAs split the first contraction and then the width of the result.
 // Here the warps share what is loaded: stages of 64 values of a contraction (or columns), rows of 128 bytes
@@ -794,7 +793,6 @@ __global__ void __launch_bounds__(LR_THREADS, TileShape<RP>::CTAS) low_rank_tile
   }
   if (ctas > 1) lr_cluster_sync();  // the others may still be reading this CTA's partial sums
 }
-
 // ---- gradients of the factors --------------------------------------------------------------------------
 
 struct FactorGradArgs {
@@ -824,47 +822,72 @@ __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, in
   for (int i = 0; i < SUMS; ++i) acc[i] = 0.0f;
   const int start = a.plan.offset[set], size = a.plan.count[set], blocks = (size + 15) / 16;
   const bool there = col < a.in_ld;
-  auto row_values = [&](int place) {
-    const int r = a.plan.order[start + place];
-    return load16(a.in + static_cast<int64_t>(r < 0 ? 0 : r / a.in_div) * a.in_ld + col, there && r >= 0);
+  // BATCH blocks' rows and inner vectors on their way together, the places of the next ones read meanwhile: what counts is
+  // that no load waits for another one's use (8192 rows of rank 16: 47 us a block at a time)
+  constexpr int BATCH = RP <= 16 ? 4 : RP <= 32 ? 2 : 1, PIECES = RH / 8;  // of the inner vectors, high and low, for a block
+  int route[BATCH][2];
+  auto look_up = [&](int b0) {
+#pragma unroll
+    for (int u = 0; u < BATCH; ++u)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) route[u][h] = b0 + u * a.row_parts < blocks ? __ldg(a.plan.order + start + (b0 + u * a.row_parts) * 16 + h * 8 + g) : -1;
   };
-#pragma unroll 2
-  for (int b = part; b < blocks; b += a.row_parts) {
-    const uint4 v0 = row_values(b * 16 + g), v1 = row_values(b * 16 + 8 + g);
-    uint32_t x[4][2];  // tile t: columns col0 + 8 (c / 2) + 2 t + c % 2, the rows in pairs
+  look_up(part);
+  for (int b0 = part; b0 < blocks; b0 += BATCH * a.row_parts) {
+    uint4 values[BATCH][2];
+    uint2 high[BATCH][PIECES], low[BATCH][PIECES];
+    float block_unit[BATCH];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) { x[t][0] = transpose8(word(v0, t)); x[t][1] = transpose8(word(v1, t)); }
-    const int64_t block = (static_cast<int64_t>(start / 16) + b) * RP;
-    const float u = Mma<T>::SCALED ? a.inner.unit[start / 16 + b] : 1.0f;
-    auto inner_at = [&](const uint16_t* p, int j) { return __ldg(reinterpret_cast<const uint2*>(p + (block + j) * 16 + 4 * q)); };
-    auto add = [&](int at, const uint32_t (&m)[4], uint32_t n0, uint32_t n1, const uint32_t (&m2)[4], uint32_t k0, uint32_t k1) {
-      float d[4];
+    for (int u = 0; u < BATCH; ++u) {
+      const int b = b0 + u * a.row_parts;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) d[i] = Mma<T>::SCALED ? 0.0f : acc[at + i];
-      Mma<T>::run(d, m2, k0, k1);
-      Mma<T>::run(d, m, n0, n1);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[at + i] = Mma<T>::SCALED ? fmaf(u, d[i], acc[at + i]) : d[i];
-    };
-    if (!LEFT) {
-#pragma unroll
-      for (int m = 0; m < RH / 16; ++m) {
-        const int j = j0 + m * 16 + g;
-        const uint2 h0 = inner_at(a.inner.high, j), h1 = inner_at(a.inner.high, j + 8), l0 = inner_at(a.inner.low, j), l1 = inner_at(a.inner.low, j + 8);
-        const uint32_t high[4] = {h0.x, h1.x, h0.y, h1.y}, low[4] = {l0.x, l1.x, l0.y, l1.y};
-#pragma unroll
-        for (int t = 0; t < 4; ++t) add((m * 4 + t) * 4, high, x[t][0], x[t][1], low, x[t][0], x[t][1]);
+      for (int h = 0; h < 2; ++h) {
+        const int r = route[u][h];
+        values[u][h] = load16(a.in + static_cast<int64_t>(r < 0 ? 0 : r / a.in_div) * a.in_ld + col, there && r >= 0);
       }
-    } else {
+      const int64_t block = (static_cast<int64_t>(start / 16) + b) * RP;
 #pragma unroll
-      for (int n = 0; n < RH / 8; ++n) {  // column c of tile n is rank RH / 4 (c / 2) + 2 n + c % 2: a lane's ranks are neighbours
-        const int j = j0 + (g >> 1) * (RH / 4) + 2 * n + (g & 1);
-        const uint2 h = inner_at(a.inner.high, j), l = inner_at(a.inner.low, j);
+      for (int i = 0; i < PIECES; ++i) {
+        // right: ranks of the rows of fragment i / 2, then 8 further.  left: column c of tile i is rank RH / 4 (c / 2) + 2 i + c % 2, so
+        // that a lane's ranks are neighbours
+        const int j = j0 + (LEFT ? (g >> 1) * (RH / 4) + 2 * i + (g & 1) : i * 8 + g);
+        high[u][i] = load8(a.inner.high + (block + j) * 16 + 4 * q, b < blocks);
+        low[u][i] = load8(a.inner.low + (block + j) * 16 + 4 * q, b < blocks);
+      }
+      block_unit[u] = Mma<T>::SCALED && b < blocks ? __ldg(a.inner.unit + start / 16 + b) : 1.0f;
+    }
+    look_up(b0 + BATCH * a.row_parts);
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
-          const uint32_t rows[4] = {x[2 * m][0], x[2 * m + 1][0], x[2 * m][1], x[2 * m + 1][1]};
-          add((n * 2 + m) * 4, rows, h.x, h.y, rows, l.x, l.y);
+    for (int u = 0; u < BATCH; ++u) {
+      uint32_t x[4][2];  // tile t: columns col0 + 8 (c / 2) + 2 t + c % 2, the rows in pairs
+#pragma unroll
+      for (int t = 0; t < 4; ++t) { x[t][0] = transpose8(word(values[u][0], t)); x[t][1] = transpose8(word(values[u][1], t)); }
+      // D += M (low + high), by way of the block's unit
+      auto add = [&](int at, const uint32_t (&m_low)[4], uint32_t l0, uint32_t l1, const uint32_t (&m_high)[4], uint32_t h0, uint32_t h1) {
+        float d[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[i] = Mma<T>::SCALED ? 0.0f : acc[at + i];
+        Mma<T>::run(d, m_low, l0, l1);
+        Mma<T>::run(d, m_high, h0, h1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[at + i] = Mma<T>::SCALED ? fmaf(block_unit[u], d[i], acc[at + i]) : d[i];
+      };
+      if (!LEFT) {
+#pragma unroll
+        for (int m = 0; m < RH / 16; ++m) {
+          const uint32_t hi[4] = {high[u][2 * m].x, high[u][2 * m + 1].x, high[u][2 * m].y, high[u][2 * m + 1].y};
+          const uint32_t lo[4] = {low[u][2 * m].x, low[u][2 * m + 1].x, low[u][2 * m].y, low[u][2 * m + 1].y};
+#pragma unroll
+          for (int t = 0; t < 4; ++t) add((m * 4 + t) * 4, lo, x[t][0], x[t][1], hi, x[t][0], x[t][1]);
         }
+      } else {
+#pragma unroll
+        for (int n = 0; n < RH / 8; ++n)
+#pragma unroll
+          for (int m = 0; m < 2; ++m) {
+            const uint32_t rows[4] = {x[2 * m][0], x[2 * m + 1][0], x[2 * m][1], x[2 * m + 1][1]};
+            add((n * 2 + m) * 4, rows, low[u][n].x, low[u][n].y, rows, high[u][n].x, high[u][n].y);
+          }
       }
     }
   }
@@ -943,7 +966,8 @@ static LowRankPlan plan_low_rank(int64_t routes, int64_t sets, int64_t rank, boo
 }
 
 // `configured`: a bit per device, the shared-memory opt-in is a per-device attribute of the function.
-static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, uint64_t& configured, const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
+template <typename... Params>
+static int launch_low_rank_kernel(void (*kernel)(Params...), int bytes, uint64_t& configured, int64_t clusters, const LowRankPlan& p, cudaStream_t s, Params... args) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !((configured >> dev) & 1ull)) {
@@ -952,7 +976,7 @@ static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, uint64
     if (dev >= 0 && dev < 64) configured |= 1ull << dev;
   }
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(p.tiles * p.ctas));
+  config.gridDim = dim3(static_cast<unsigned>(clusters * p.ctas));
   config.blockDim = dim3(LR_THREADS);
   config.dynamicSmemBytes = bytes;
   config.stream = s;
@@ -967,14 +991,14 @@ static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, uint64
   }
   config.attrs = &attribute;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
   return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
 }
 template <typename T, int RP, bool BACK>
 static int launch_low_rank(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
   static uint64_t configured[2] = {0, 0};
-  if (p.rows == TILE_ROWS) return launch_low_rank_kernel(low_rank_tile_kernel<T, RP, BACK>, TileShape<RP>::BYTES, configured[0], a, p, s);
-  return launch_low_rank_kernel(low_rank_kernel<T, RP, BACK>, LowRankShape<RP, BACK>::BYTES, configured[1], a, p, s);
+  if (p.rows == TILE_ROWS) return launch_low_rank_kernel(low_rank_tile_kernel<T, RP, BACK>, TileShape<RP>::BYTES, configured[0], p.tiles, p, s, a);
+  return launch_low_rank_kernel(low_rank_kernel<T, RP, BACK>, LowRankShape<RP, BACK>::BYTES, configured[1], p.tiles, p, s, a);
 }
 template <typename T, bool BACK>
 static int launch_low_rank_of(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
@@ -1141,22 +1165,22 @@ int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* 
   k.whole = 1;
   k.dead_rows = a.dx && !l.route_dx;
   if (weights) k.keep = l.back;
+  LowRankArgs inner = k;  // p = A x
+  inner.in = static_cast<const uint16_t*>(a.x);
+  inner.in_ld = inner.depth = a.in_dim;
+  inner.in_div = a.x_div;
+  inner.first = static_cast<const uint16_t*>(a.right);
+  inner.first_scale = 1.0f;
+  inner.second = nullptr;
+  inner.dead_rows = 0;
+  inner.keep = l.inner;
   if (a.dx || a.dright)
     if (const int rc = launch_low_rank_any(a.dtype, true, k, p, s)) return rc;
+  if (a.dleft)
+    if (const int rc = launch_low_rank_any(a.dtype, false, inner, p, s)) return rc;
   if (a.dx && l.route_dx)
     if (const int rc = sum_picks(l.route_dx, k.indices, a.sets, a.routes / a.x_div, a.x_div, a.in_dim, a.dx, a.dtype, s)) return rc;
   if (!weights) return KEEPVQ_OK;
-  if (a.dleft) {  // p = A x
-    k.in = static_cast<const uint16_t*>(a.x);
-    k.in_ld = k.depth = a.in_dim;
-    k.in_div = a.x_div;
-    k.first = static_cast<const uint16_t*>(a.right);
-    k.first_scale = 1.0f;
-    k.second = nullptr;
-    k.dead_rows = 0;
-    k.keep = l.inner;
-    if (const int rc = launch_low_rank_any(a.dtype, false, k, p, s)) return rc;
-  }
   const int64_t mean = a.routes / (a.routes < a.sets ? a.routes : a.sets);
   const int row_parts = mean <= 16 ? 1 : mean <= 64 ? 2 : mean <= 256 ? 4 : 8;  // a part keeps four blocks of 16 rows or more
   FactorGradArgs right{static_cast<const uint16_t*>(a.x), a.in_dim, a.x_div, a.dright ? a.in_dim : 0, static_cast<int>(a.rank), row_parts, 1.0f, l.plan, l.back, static_cast<uint16_t*>(a.dright)};

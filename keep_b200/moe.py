@@ -20,6 +20,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
+from .low_rank import LowRank
 from .router import Routing
 from .vq import as_device, table_on
 
@@ -56,6 +57,10 @@ class SharedExpert:
     GEMM over the stacked weights.  The reference's shared expert runs on oMLX's MXFP4 / MXFP8 /
     affine kernels, a third-party package that is not part of it: a caller holding such weights
     expands them to 16 bits first, and no parity with those kernels is claimed.
+
+    Requests may bring low-rank adapters: ``shared(x, adapters={"w1": ..., "w3": ..., "w2": ...},
+    adapter_indices=indices)`` adds those of ``low_rank.LowRank`` stacks to the products (in fp32, before
+    anything is rounded), row by row: ``indices[t]`` is the adapter of token ``t``, -1 for none.
     """
 
     def __init__(self, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, *, swiglu_limit: float = 0.0):
@@ -69,15 +74,20 @@ class SharedExpert:
         self.down = w2.t().contiguous()                          # [inter, hidden]
         self.swiglu_limit = float(swiglu_limit)
 
-    def __call__(self, x: torch.Tensor) -> torch.Tensor:
+    def __call__(self, x: torch.Tensor, *, adapters: dict[str, LowRank] | None = None, adapter_indices: torch.Tensor | None = None) -> torch.Tensor:
         """``x`` [tokens, hidden] in the weights' dtype -> fp32 ``[tokens, hidden]``."""
+        adapters = adapters or {}
+        if not set(adapters) <= {"w1", "w3", "w2"} or (adapters and adapter_indices is None):
+            raise ValueError("adapters go to 'w1', 'w3' and 'w2' and need adapter_indices [tokens]")
+        add = lambda name, base, rows: adapters[name].add(base, rows, adapter_indices) if name in adapters else base  # noqa: E731
         if x.ndim != 2 or int(x.shape[1]) != self.hidden or x.dtype != self.down.dtype:
             raise ValueError(f"x must be [tokens, {self.hidden}] {self.down.dtype}, found {tuple(x.shape)} {x.dtype}")
         gate, up = torch.mm(x, self.gate_up, out_dtype=torch.float32).split(self.inter, dim=1)
+        gate, up = add("w1", gate, x), add("w3", up, x)
         if self.swiglu_limit > 0:
             gate, up = gate.clamp(max=self.swiglu_limit), up.clamp(-self.swiglu_limit, self.swiglu_limit)
         h = (torch.nn.functional.silu(gate) * up).to(x.dtype)   # the hidden row in 16 bits, as the routed experts keep theirs
-        return torch.mm(h, self.down, out_dtype=torch.float32)
+        return add("w2", torch.mm(h, self.down, out_dtype=torch.float32), h)
 
 
 class RoutedMoELayer:

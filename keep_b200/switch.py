@@ -1,4 +1,5 @@
-"""Holders for stacked VQ experts: one switch projection, and the gate/up/down trio of a routed MLP.
+"""Holders for stacked experts: one switch projection (E8P codes, or 16-bit weights), and the gate/up/down
+trio of a routed MLP.
 
 Mirrors of ``QuantizedVQSwitchLinear`` (``src/ramp/nn/switch_linear.py:93-571``) and
 ``QuantizedVQSwitchGLU`` (``src/ramp/models/glm4_moe_adapter.py:113-390``) over ``torch.Tensor``
@@ -8,6 +9,10 @@ What they hold is the hot path only: codes, scales, codebook, optional bias and 
 scale / output-bias sidecars.  The reference's other sidecars (low-rank and sparse residual rows,
 RHT signs, rotation matrices) and ``from_weights`` (the RTN encoder) belong to conversion and
 quality tooling; passing one raises ``NotImplementedError`` rather than being ignored.
+
+``HighPrecisionSwitchLinear`` is the holder of a projection that stays in fp16 or bf16 (``src/ramp/nn/``); it
+takes the place of a quantised one in ``QuantizedVQSwitchGLU``.  Either takes ``low_rank``, a
+``low_rank.LowRank`` with one correction per expert that is added to its outputs.
 """
 
 from __future__ import annotations
@@ -17,13 +22,22 @@ from typing import Callable
 import torch
 
 from . import _lib
+from .dense_switch import switch_matmul
 from .kernels import e8p_m1_per_route, e8p_m1_token_layout, should_use_e8p_m1
+from .low_rank import LowRank
 from .vq import table_on
 from .vq_switch import gather_vqmm, vq_switch_qmv
 
 _ROUTE_STRATEGIES = ("auto", "direct", "sorted_tiled", "per_route_decoded")
 _OUTSIDE = ("continuous_low_rank_left", "continuous_low_rank_right", "sparse_residual_expert_indices",
             "sparse_residual_output_indices", "sparse_residual_values", "rht_signs", "rotation_matrix")
+
+
+def _check_low_rank(low_rank: LowRank | None, num_experts: int, output_dims: int, input_dims: int) -> None:
+    if low_rank is not None:
+        found = (int(low_rank.left.shape[0]), int(low_rank.left.shape[1]), int(low_rank.right.shape[2]))
+        if found != (num_experts, output_dims, input_dims):
+            raise ValueError(f"low_rank must correct (experts, out, in) = {(num_experts, output_dims, input_dims)}, found {found}")
 
 
 class QuantizedVQSwitchLinear:
@@ -37,7 +51,7 @@ class QuantizedVQSwitchLinear:
                  codebook: torch.Tensor | None = None, bias: torch.Tensor | None = None, group_size: int = 512,
                  code_bits: int = 8, use_gather_vqmm: bool = True, route_strategy: str = "auto",
                  gather_codebook_duplication: int = 8, continuous_scale_delta: torch.Tensor | None = None,
-                 continuous_output_bias: torch.Tensor | None = None, **outside):
+                 continuous_output_bias: torch.Tensor | None = None, low_rank: LowRank | None = None, **outside):
         for name, value in outside.items():
             if name not in _OUTSIDE:
                 raise TypeError(f"unexpected keyword argument {name!r}")
@@ -63,7 +77,9 @@ class QuantizedVQSwitchLinear:
             raise ValueError(f"scales must have shape {expected_scales}, found {tuple(scales.shape)}")
         if bias is not None and tuple(bias.shape) != (num_experts, output_dims):
             raise ValueError(f"bias must have shape {(num_experts, output_dims)}, found {tuple(bias.shape)}")
+        _check_low_rank(low_rank, num_experts, output_dims, input_dims)
         _lib.require_cuda(codes, scales)
+        self.low_rank = low_rank
         self.input_dims, self.output_dims, self.num_experts = int(input_dims), int(output_dims), int(num_experts)
         self.group_size, self.code_bits = int(group_size), int(code_bits)
         self.use_gather_vqmm, self.route_strategy = bool(use_gather_vqmm), route_strategy
@@ -122,11 +138,46 @@ class QuantizedVQSwitchLinear:
             y = y.reshape(tuple(indices.shape) + (self.output_dims,))
         else:
             y = vq_switch_qmv(x, self.codes, scales, self.codebook, indices, **common)
+        if self.low_rank is not None:
+            y = self.low_rank.add(y, x, indices)
         gather = indices.long().clamp(min=0)
         if self.bias is not None:
             y = y + self.bias[gather].to(y.dtype)
         if self.continuous_output_bias is not None:
             y = y + self.continuous_output_bias[gather].to(y.dtype)
+        return y
+
+
+class HighPrecisionSwitchLinear:
+    """Switch-linear layer over 16-bit expert weights ``[experts, out, in]``, with the call layouts of
+    ``QuantizedVQSwitchLinear``; ``x`` has the weights' dtype.  Recorded by autograd where an input requires
+    a gradient."""
+
+    def __init__(self, *, input_dims: int, output_dims: int, num_experts: int, weight: torch.Tensor, bias: torch.Tensor | None = None,
+                 low_rank: LowRank | None = None):
+        if input_dims <= 0 or output_dims <= 0 or num_experts <= 0:
+            raise ValueError("input_dims, output_dims, and num_experts must be positive")
+        if input_dims % 8 != 0:
+            raise ValueError("input_dims must be divisible by 8")
+        expected = (num_experts, output_dims, input_dims)
+        if tuple(weight.shape) != expected:
+            raise ValueError(f"weight must have shape {expected}, found {tuple(weight.shape)}")
+        if weight.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"weight must be fp16 or bf16, found {weight.dtype}")
+        if bias is not None and tuple(bias.shape) != (num_experts, output_dims):
+            raise ValueError(f"bias must have shape {(num_experts, output_dims)}, found {tuple(bias.shape)}")
+        _check_low_rank(low_rank, num_experts, output_dims, input_dims)
+        _lib.require_cuda(weight, bias)
+        self.input_dims, self.output_dims, self.num_experts = int(input_dims), int(output_dims), int(num_experts)
+        self.weight, self.bias, self.low_rank = weight, bias, low_rank
+
+    def __call__(self, x: torch.Tensor, indices: torch.Tensor, *, sorted_indices: bool = False) -> torch.Tensor:
+        del sorted_indices  # routes may come in any order
+        y = switch_matmul(x, self.weight, indices)
+        if self.low_rank is not None:
+            y = self.low_rank.add(y, x, indices)
+        if self.bias is not None:
+            y = y + self.bias[indices.long().clamp(min=0)].to(y.dtype)
         return y
 
 
@@ -146,9 +197,10 @@ class QuantizedVQSwitchGLU:
     """``down(act(up(x), gate(x)))`` per route: ``x [tokens, hidden]``, ``indices [tokens, k]`` ->
     ``[tokens, k, hidden]`` (``glm4_moe_adapter.py:367-372``).
 
-    With 16-bit E8P codes, no bias or sidecars and plain or limited SwiGLU, a call runs the fused
-    layer kernels (activation quantisation, gate + up + SwiGLU in one launch, down in another);
-    any other configuration composes the three projections as the reference does.
+    With 16-bit E8P codes, no bias, sidecars or low-rank corrections and plain or limited SwiGLU, a call
+    runs the fused layer kernels (activation quantisation, gate + up + SwiGLU in one launch, down in
+    another); any other configuration (a projection in 16 bits among them) composes the three
+    projections as the reference does.
     """
 
     def __init__(self, *, gate_proj: QuantizedVQSwitchLinear, up_proj: QuantizedVQSwitchLinear, down_proj: QuantizedVQSwitchLinear,
@@ -181,9 +233,10 @@ class QuantizedVQSwitchGLU:
             from .moe import Projection, RoutedMoELayer
 
             projs = (self.gate_proj, self.up_proj, self.down_proj)
-            plain = all(p.code_bits == 16 and p.bias is None and not p.has_continuous_sidecar and p.use_gather_vqmm for p in projs)
+            plain = all(isinstance(p, QuantizedVQSwitchLinear) and p.code_bits == 16 and p.bias is None and p.low_rank is None
+                        and not p.has_continuous_sidecar and p.use_gather_vqmm for p in projs)
             act_ok = self.activation is None or hasattr(self.activation, "limit")
-            same_book = all(p.codebook is self.gate_proj.codebook or (p.codebook is not None and self.gate_proj.codebook is not None
+            same_book = plain and all(p.codebook is self.gate_proj.codebook or (p.codebook is not None and self.gate_proj.codebook is not None
                                                                      and torch.equal(p.codebook, self.gate_proj.codebook)) for p in projs)
             self._fused[top_k] = None
             if plain and act_ok and same_book:

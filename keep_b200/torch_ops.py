@@ -17,12 +17,15 @@ op                              reference interface it stands in for
 ``gather_vqmm_sorted_routes``   ``src/ramp/ops/vq_switch.py:620-640``
 ``routed_topk``                 ``scripts/v41_build/omlx_lattice.py:77-104,333-338``
 ``moe_decode_layer``            ``scripts/v41_build/omlx_lattice.py:327-371``
+``switch_matmul``               the 16-bit ``HighPrecisionSwitchLinear`` (``src/ramp/nn/``)
+``switch_low_rank``             -- (``low_rank.switch_low_rank``)
 ==============================  ==========================================================
 
 Arguments are tensors and plain scalars only (what a schema can carry): tables are passed
 explicitly, tuples of the nested operators are flattened, keyword-only arguments keep their names.
-None of the ops mutates an argument; outputs are fresh tensors.  There is no autograd formula:
-this is an inference path.
+None of the ops mutates an argument; outputs are fresh tensors.  The operators over codes have no autograd
+formula: they are an inference path.  ``switch_matmul`` and ``switch_low_rank`` have one, whose work is done by
+``switch_matmul_grads`` and ``switch_low_rank_grads`` (empty tensors for gradients that are not wanted).
 """
 
 from __future__ import annotations
@@ -33,7 +36,7 @@ import torch
 from torch import Tensor
 from torch.library import custom_op
 
-from . import kernels, moe, router, vq_switch
+from . import dense_switch, kernels, low_rank, moe, router, vq_switch
 
 __all__ = ["OPS"]
 
@@ -237,6 +240,84 @@ def _(x, router_w, w1_codes, w1_scales, w3_codes, w3_scales, w2_codes, w2_scales
     return (torch.empty_like(x),) + _routing_shapes(x, top_k)
 
 
+# ---- 16-bit experts and low-rank adapters ---------------------------------------------------------------
+
+def _wanted(grads, like):
+    return tuple(like.new_empty((0,)) if g is None else g for g in grads)
+
+
+@custom_op("keepvq::switch_matmul", mutates_args=(), device_types=_CUDA)
+def switch_matmul(x: Tensor, weight: Tensor, indices: Tensor) -> Tensor:
+    return dense_switch._forward(x, weight, indices)
+
+
+@switch_matmul.register_fake
+def _(x, weight, indices):
+    return x.new_empty((*indices.shape, weight.shape[1]))
+
+
+@custom_op("keepvq::switch_matmul_grads", mutates_args=(), device_types=_CUDA)
+def switch_matmul_grads(grad: Tensor, x: Tensor, weight: Tensor, indices: Tensor, x_grad: bool, weight_grad: bool) -> Tuple[Tensor, Tensor]:
+    return _wanted(dense_switch.switch_matmul_grads(grad, x, weight, indices, x_grad=x_grad, weight_grad=weight_grad), x)
+
+
+@switch_matmul_grads.register_fake
+def _(grad, x, weight, indices, x_grad, weight_grad):
+    return tuple(t.new_empty(t.shape if wanted else (0,)) for t, wanted in ((x, x_grad), (weight, weight_grad)))
+
+
+def _matmul_context(ctx, inputs, output):
+    ctx.save_for_backward(*inputs)
+
+
+def _matmul_backward(ctx, grad):
+    x, weight, indices = ctx.saved_tensors
+    of_x, of_weight = ctx.needs_input_grad[:2]
+    dx, dweight = torch.ops.keepvq.switch_matmul_grads(grad, x, weight, indices, of_x, of_weight)
+    return dx if of_x else None, dweight if of_weight else None, None
+
+
+switch_matmul.register_autograd(_matmul_backward, setup_context=_matmul_context)
+
+
+@custom_op("keepvq::switch_low_rank", mutates_args=(), device_types=_CUDA)
+def switch_low_rank(x: Tensor, left: Tensor, right: Tensor, indices: Tensor, base: Optional[Tensor], scale: float) -> Tensor:
+    return low_rank._forward(x, left, right, indices, base, scale)
+
+
+@switch_low_rank.register_fake
+def _(x, left, right, indices, base, scale):
+    return x.new_empty((*indices.shape, left.shape[1]), dtype=x.dtype if base is None else base.dtype)
+
+
+@custom_op("keepvq::switch_low_rank_grads", mutates_args=(), device_types=_CUDA)
+def switch_low_rank_grads(grad: Tensor, x: Tensor, left: Tensor, right: Tensor, indices: Tensor, scale: float, x_grad: bool,
+                          weight_grad: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    return _wanted(low_rank.switch_low_rank_grads(grad, x, left, right, indices, scale=scale, x_grad=x_grad, weight_grad=weight_grad), x)
+
+
+@switch_low_rank_grads.register_fake
+def _(grad, x, left, right, indices, scale, x_grad, weight_grad):
+    return tuple(t.new_empty(t.shape if wanted else (0,)) for t, wanted in ((x, x_grad), (left, weight_grad), (right, weight_grad)))
+
+
+def _low_rank_context(ctx, inputs, output):
+    x, left, right, indices, _, ctx.scale = inputs
+    ctx.save_for_backward(x, left, right, indices)
+
+
+def _low_rank_backward(ctx, grad):
+    x, left, right, indices = ctx.saved_tensors
+    of_x, of_left, of_right, _, of_base, _ = ctx.needs_input_grad
+    dx = dleft = dright = None
+    if of_x or of_left or of_right:
+        dx, dleft, dright = torch.ops.keepvq.switch_low_rank_grads(grad.to(x.dtype), x, left, right, indices, ctx.scale, of_x, of_left or of_right)
+    return dx if of_x else None, dleft if of_left else None, dright if of_right else None, None, grad if of_base else None, None
+
+
+switch_low_rank.register_autograd(_low_rank_backward, setup_context=_low_rank_context)
+
+
 OPS = ("vq_qmv", "vq_qmm", "e8p_m1_token_layout", "e8p_m1_per_route", "e8_1bit_m1_token_layout", "e8_1bit_m1_per_route",
        "e8p_nested_m1_token_layout", "e8p_nested_m1_per_route", "vq_switch_qmv", "gather_vqmm", "gather_vqmm_sorted_routes", "routed_topk",
-       "moe_decode_layer")
+       "moe_decode_layer", "switch_matmul", "switch_matmul_grads", "switch_low_rank", "switch_low_rank_grads")

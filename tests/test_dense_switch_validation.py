@@ -118,3 +118,16 @@ def test_scratch_sizes():
     # a row's gradient is summed over its picks in fp32
     assert lib.keepvq_switch_matmul_workspace_bytes(4096, 8, 512, 1024, 2, 1) >= 4096 * 1024 * 4
     assert lib.keepvq_switch_matmul_workspace_bytes(0, 1, 8, 8, 1, 0) > 0
+
+
+def test_the_sixteen_bit_holder_refuses():
+    from keep_b200.switch import HighPrecisionSwitchLinear
+
+    ok = dict(input_dims=16, output_dims=8, num_experts=3, weight=rows(3, 8, 16))
+    for change, message in ((dict(num_experts=0), "must be positive"), (dict(input_dims=12, weight=rows(3, 8, 12)), "divisible by 8"), (dict(output_dims=9), "weight must have shape"),
+                            (dict(weight=rows(3, 8, 16, dtype=torch.float32)), "fp16 or bf16"), (dict(bias=rows(3, 7)), "bias must have shape"),
+                            (dict(low_rank=LowRank(rows(3, 8, 4), rows(3, 4, 24))), "low_rank must correct")):
+        with pytest.raises(ValueError, match=message):
+            HighPrecisionSwitchLinear(**{**ok, **change})
+    with pytest.raises(_lib.KeepVQError, match="no CPU path"):
+        HighPrecisionSwitchLinear(**ok)
