@@ -233,6 +233,20 @@ def test_calls_on_two_streams_at_once(cuda):
             assert all(torch.equal(a, b) for a, b in zip(result, want[n]))
 
 
+def test_many_tiles_of_a_block_and_calls_that_follow_one_another_at_once(cuda):
+    """Several tiles of both gradients for every block, ragged experts, and calls enqueued without a wait between them."""
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    x, weight, indices, grad = make(cuda, 1500, 2, 5, 2048, 4096, dead=0.1, seed=5)
+    indices[:900, 0] = 1  # one expert with most of the routes
+    indices[:, 1][indices[:, 1] == 3] = 4  # one without any
+    ref.close(switch_matmul(x, weight, indices), ref.matmul(x, weight, indices))
+    want = ref.matmul_grads(grad, x, weight, indices)
+    for got in [switch_matmul_grads(grad, x, weight, indices) for _ in range(40)][::13]:
+        ref.close(got[0], want[0])
+        ref.close(got[1], want[1])
+
+
 def test_weights_beyond_32_bit_offsets(cuda):
     from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
 
