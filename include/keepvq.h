@@ -462,7 +462,9 @@ int keepvq_grouped_projection_bytes_served(int64_t routes, int64_t slots, int64_
  *
  * An index outside [0, experts) is a dead route: its output row is zero and it adds nothing to a
  * gradient; experts without routes get zero gradients.  All sums are held in fp32 and rounded once;
- * an expert's routes are added up in their order, so a call gives the same bits every time.  Rows
+ * an expert's routes are added up in their order, so a call gives the same bits every time.  The first
+ * int32 of the workspace is 1 after a call one of whose bounded waits expired (2 s, on a device that has
+ * stopped making progress): its outputs are then invalid.  Rows
  * are dense, in_dim is a multiple of 8, pointers are aligned to 16 bytes; a row of `grad` is
  * grad_ld >= out_dim values long, a multiple of 8, and those behind out_dim are zero.
  * ------------------------------------------------------------------------------------------ */
@@ -500,10 +502,11 @@ int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stre
  *                                 dright[e] = sum over e's routes of q x^T
  *
  * A dead route (see above) leaves out[r] = base[r].  The inner vectors A x and q are sums in fp32
- * and enter the second product as the sum of two 16-bit values (16 bits of them, 22 for fp16),
- * scaled by a power of two per row so that fp16 neither overflows nor loses small ones.  out and
- * base have the type out_dtype: the activations', or fp32.  base may be out.  rank is a multiple
- * of 8 up to 128; in_dim and pointers as above, grad as above.
+ * and enter the second product as the sum of two 16-bit values: 16 bits of every value for bf16; for
+ * fp16, whose range they may leave, 22 bits of the row's largest (a power of two per row is taken out and
+ * put back).  The factors' gradients take them as the sum of two bf16 values.  out and base have the
+ * type out_dtype: the activations', or fp32.  base may be out.  rank is a multiple of 8 up to 128;
+ * in_dim, pointers and grad as above; base_ld and out_ld are at most 2^28.
  * ------------------------------------------------------------------------------------------ */
 typedef struct keepvq_switch_low_rank_args {
   const void* x;          /* [routes / x_div, in_dim] */

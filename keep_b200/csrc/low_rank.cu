@@ -22,6 +22,7 @@
 namespace keepvq {
 namespace dense {
 
+constexpr int64_t LR_MAX_PITCH = int64_t{1} << 28;  // of a row, in values: its bytes stay within 32 bits
 constexpr int LR_MAX_RANK = 128, LR_WARPS = 8, LR_THREADS = LR_WARPS * 32, CHUNK = 32;
 
 // ---- fragments ------------------------------------------------------------------------------------
@@ -106,11 +107,11 @@ __device__ __forceinline__ float peer_float(const float* p, uint32_t rank) {
 // ---- one product after the other ---------------------------------------------------------------------
 
 // Inner vectors as the gradients of the factors take them: per block of 16 places, [rank][16 places] of
-// 16-bit values, the two whose sum they are apart; a lane's four places of a fragment (2q, 2q + 1, 2q + 8,
-// 2q + 9) side by side.  `unit`: the power of two a block is divided by (fp16).
+// bf16, the two whose sum they are apart; a lane's four places of a fragment (2q, 2q + 1, 2q + 8,
+// 2q + 9) side by side.  bf16 for fp16 operands too: the rows of a set are summed over, so no power of two
+// of a row's own could be taken out again, and one for several rows would lose the smallest.
 struct Inner {
   uint16_t *high, *low;
-  float* unit;
 };
 
 struct LowRankArgs {
@@ -152,27 +153,19 @@ __device__ __forceinline__ void low_rank_plain_row(const LowRankArgs& a, int64_t
   }
 }
 // The inner vectors of a tile for the gradients of the factors.
-template <typename T, int RP, int ROWS>
-__device__ __forceinline__ void keep_inner(const LowRankArgs& a, const float* inner, const float* unit, int start, int size) {
+template <int RP, int ROWS>
+__device__ __forceinline__ void keep_inner(const LowRankArgs& a, const float* inner, int start, int size) {
   for (int i = threadIdx.x; i < ROWS * RP / 2; i += LR_THREADS) {  // two neighbouring places of a rank
     const int block = i / (RP * 8), j = i / 8 % RP, pair = i % 8;
-    const int place = pair / 2 * 2 + (pair & 1) * 8, r0 = block * 16 + place;
+    const int r0 = block * 16 + pair / 2 * 2 + (pair & 1) * 8;
     if (r0 >= (size + 15) / 16 * 16) continue;
-    float most = 1.0f;
-    if (Mma<T>::SCALED) {
-      most = 0.0f;
-      for (int r = 0; r < 16; ++r)
-        if (block * 16 + r < size) most = fmaxf(most, unit[block * 16 + r]);
-      if (j == 0 && pair == 0) a.keep.unit[start / 16 + block] = most;
-    }
-    const float x = r0 < size ? inner[r0 * RP + j] / most : 0.0f, y = r0 + 1 < size ? inner[(r0 + 1) * RP + j] / most : 0.0f;
     uint32_t high, low;
-    split<T>(x, y, high, low);
+    split<__nv_bfloat16>(r0 < size ? inner[r0 * RP + j] : 0.0f, r0 + 1 < size ? inner[(r0 + 1) * RP + j] : 0.0f, high, low);
     const int64_t at = (static_cast<int64_t>(start / 16 + block) * RP + j) * 8 + pair;
     reinterpret_cast<uint32_t*>(a.keep.high)[at] = high;
     reinterpret_cast<uint32_t*>(a.keep.low)[at] = low;
   }
-  }
+}
 // `own`, this CTA's part of the sums of all rows, becomes `inner`, the cluster's (in the order of its CTAs), with a
 // power of two per row for fp16.
 template <typename T, int RP, int ROWS>
@@ -368,7 +361,7 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
     own[i] = sum * a.first_scale;
   }
   meet<T, RP, ROWS>(own, inner, unit, ctas);
-  if (a.keep.high && rank == 0) keep_inner<T, RP, ROWS>(a, inner, unit, start, size);
+  if (a.keep.high && rank == 0) keep_inner<RP, ROWS>(a, inner, start, size);
 
   // ---- the second product: [ROWS, RP] times the factor -> [ROWS, width], 32 columns per warp and step
   if (a.second) {
@@ -693,7 +686,7 @@ __global__ void __launch_bounds__(LR_THREADS, TileShape<RP>::CTAS) low_rank_tile
     step_issued();
   }
   meet<T, RP, TILE_ROWS>(own, inner, unit, ctas);
-  if (a.keep.high && rank == 0) keep_inner<T, RP, TILE_ROWS>(a, inner, unit, start, size);
+  if (a.keep.high && rank == 0) keep_inner<RP, TILE_ROWS>(a, inner, start, size);
   if (a.second) {
     uint32_t high[KC][4], low[KC][4];
 #pragma unroll
@@ -812,14 +805,15 @@ struct FactorGradArgs {
 //   right: D[rank][column] = inner^T rows       left: D[column][rank] = rows^T inner
 template <typename T, int RP, bool LEFT>
 __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, int slab, int half, float* sm) {
+  constexpr bool SPLIT = Mma<T>::SCALED;  // fp16
   constexpr int RH = RP > 64 ? 64 : RP, SUMS = RH;  // ranks of a CTA; sums of a lane: 32 columns x RH / 32 lanes
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
   const int part = warp % a.row_parts, slabs = LR_WARPS / a.row_parts;
   const int64_t col0 = (static_cast<int64_t>(slab) * slabs + warp / a.row_parts) * 32, col = col0 + 8 * q;
   const int j0 = half * RH;
-  float acc[SUMS];
+  float acc[SUMS / 4][4];
 #pragma unroll
-  for (int i = 0; i < SUMS; ++i) acc[i] = 0.0f;
+  for (int i = 0; i < SUMS; ++i) acc[i / 4][i % 4] = 0.0f;
   const int start = a.plan.offset[set], size = a.plan.count[set], blocks = (size + 15) / 16;
   const bool there = col < a.in_ld;
   // BATCH blocks' rows and inner vectors on their way together, the places of the next ones read meanwhile: what counts is
@@ -836,7 +830,6 @@ __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, in
   for (int b0 = part; b0 < blocks; b0 += BATCH * a.row_parts) {
     uint4 values[BATCH][2];
     uint2 high[BATCH][PIECES], low[BATCH][PIECES];
-    float block_unit[BATCH];
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
       const int b = b0 + u * a.row_parts;
@@ -854,51 +847,62 @@ __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, in
         high[u][i] = load8(a.inner.high + (block + j) * 16 + 4 * q, b < blocks);
         low[u][i] = load8(a.inner.low + (block + j) * 16 + 4 * q, b < blocks);
       }
-      block_unit[u] = Mma<T>::SCALED && b < blocks ? __ldg(a.inner.unit + start / 16 + b) : 1.0f;
     }
     look_up(b0 + BATCH * a.row_parts);
 #pragma unroll
     for (int u = 0; u < BATCH; ++u) {
-      uint32_t x[4][2];  // tile t: columns col0 + 8 (c / 2) + 2 t + c % 2, the rows in pairs
+      // tile t: columns col0 + 8 (c / 2) + 2 t + c % 2, the rows in pairs; fp16 values as the sum of two bf16 ones (exactly)
+      uint32_t x[4][2], x_low[SPLIT ? 4 : 1][2];
 #pragma unroll
-      for (int t = 0; t < 4; ++t) { x[t][0] = transpose8(word(values[u][0], t)); x[t][1] = transpose8(word(values[u][1], t)); }
-      // D += M (low + high), by way of the block's unit
-      auto add = [&](int at, const uint32_t (&m_low)[4], uint32_t l0, uint32_t l1, const uint32_t (&m_high)[4], uint32_t h0, uint32_t h1) {
-        float d[4];
+      for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[i] = Mma<T>::SCALED ? 0.0f : acc[at + i];
-        Mma<T>::run(d, m_low, l0, l1);
-        Mma<T>::run(d, m_high, h0, h1);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[at + i] = Mma<T>::SCALED ? fmaf(block_unit[u], d[i], acc[at + i]) : d[i];
-      };
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t v = transpose8(word(values[u][h], t));
+          if (SPLIT) {
+            const float2 f = Mma<T>::unpack(v);
+            split<__nv_bfloat16>(f.x, f.y, x[t][h], x_low[t][h]);
+          } else x[t][h] = v;
+        }
+      using M = Mma<__nv_bfloat16>;
       if (!LEFT) {
 #pragma unroll
         for (int m = 0; m < RH / 16; ++m) {
           const uint32_t hi[4] = {high[u][2 * m].x, high[u][2 * m + 1].x, high[u][2 * m].y, high[u][2 * m + 1].y};
           const uint32_t lo[4] = {low[u][2 * m].x, low[u][2 * m + 1].x, low[u][2 * m].y, low[u][2 * m + 1].y};
 #pragma unroll
-          for (int t = 0; t < 4; ++t) add((m * 4 + t) * 4, lo, x[t][0], x[t][1], hi, x[t][0], x[t][1]);
+          for (int t = 0; t < 4; ++t) {
+            float(&d)[4] = acc[m * 4 + t];
+            M::run(d, lo, x[t][0], x[t][1]);
+            if (SPLIT) M::run(d, hi, x_low[t % (SPLIT ? 4 : 1)][0], x_low[t % (SPLIT ? 4 : 1)][1]);
+            M::run(d, hi, x[t][0], x[t][1]);
+          }
         }
       } else {
 #pragma unroll
         for (int n = 0; n < RH / 8; ++n)
 #pragma unroll
           for (int m = 0; m < 2; ++m) {
+            float(&d)[4] = acc[n * 2 + m];
             const uint32_t rows[4] = {x[2 * m][0], x[2 * m + 1][0], x[2 * m][1], x[2 * m + 1][1]};
-            add((n * 2 + m) * 4, rows, low[u][n].x, low[u][n].y, rows, high[u][n].x, high[u][n].y);
+            M::run(d, rows, low[u][n].x, low[u][n].y);
+            if (SPLIT) {
+              constexpr int L = SPLIT ? 4 : 1;
+              const uint32_t rest[4] = {x_low[2 * m % L][0], x_low[(2 * m + 1) % L][0], x_low[2 * m % L][1], x_low[(2 * m + 1) % L][1]};
+              M::run(d, rest, high[u][n].x, high[u][n].y);
+            }
+            M::run(d, rows, high[u][n].x, high[u][n].y);
           }
       }
     }
   }
   if (a.row_parts > 1) {
 #pragma unroll
-    for (int i = 0; i < SUMS; ++i) sm[(warp * SUMS + i) * 32 + lane] = acc[i];
+    for (int i = 0; i < SUMS; ++i) sm[(warp * SUMS + i) * 32 + lane] = acc[i / 4][i % 4];
     __syncthreads();
     if (part != 0) return;
     for (int p = 1; p < a.row_parts; ++p)
 #pragma unroll
-      for (int i = 0; i < SUMS; ++i) acc[i] += sm[((warp + p) * SUMS + i) * 32 + lane];
+      for (int i = 0; i < SUMS; ++i) acc[i / 4][i % 4] += sm[((warp + p) * SUMS + i) * 32 + lane];
   }
   if (!LEFT) {
 #pragma unroll
@@ -908,7 +912,7 @@ __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, in
         const int j = j0 + m * 16 + h * 8 + g;
         float y[8];
 #pragma unroll
-        for (int t = 0; t < 4; ++t) { y[2 * t] = a.scale * acc[(m * 4 + t) * 4 + 2 * h]; y[2 * t + 1] = a.scale * acc[(m * 4 + t) * 4 + 2 * h + 1]; }
+        for (int t = 0; t < 4; ++t) { y[2 * t] = a.scale * acc[m * 4 + t][2 * h]; y[2 * t + 1] = a.scale * acc[m * 4 + t][2 * h + 1]; }
         if (j < a.rank && col < a.width) store8_from_float(reinterpret_cast<T*>(a.out) + (static_cast<int64_t>(set) * a.rank + j) * a.width + col, y);
       }
   } else {
@@ -923,7 +927,7 @@ __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, in
         T* row = reinterpret_cast<T*>(a.out) + (static_cast<int64_t>(set) * a.width + n) * a.rank;
         uint32_t packed[MINE / 2];
 #pragma unroll
-        for (int t = 0; t < RH / 8; ++t) packed[t] = Mma<T>::pack(a.scale * acc[(t * 2 + m) * 4 + 2 * h], a.scale * acc[(t * 2 + m) * 4 + 2 * h + 1]);
+        for (int t = 0; t < RH / 8; ++t) packed[t] = Mma<T>::pack(a.scale * acc[t * 2 + m][2 * h], a.scale * acc[t * 2 + m][2 * h + 1]);
 #pragma unroll
         for (int w = 0; w < MINE / 2; w += 2)
           if (j + 2 * w < a.rank) *reinterpret_cast<uint2*>(row + j + 2 * w) = make_uint2(packed[w], packed[w + 1]);
@@ -1051,7 +1055,6 @@ static LowRankLayout lay_out_low_rank(void* base, int64_t routes, int64_t sets, 
   for (Inner* i : {&l.inner, &l.back}) {
     i->high = s.take<uint16_t>(values);
     i->low = s.take<uint16_t>(values);
-    i->unit = s.take<float>(blocks);
   }
   l.route_dx = grads && x_div > 1 ? s.take<float>(routes * in_dim) : nullptr;
   l.bytes = s.used;
@@ -1069,6 +1072,7 @@ static int check_low_rank(const keepvq_switch_low_rank_args& a, bool grads) {
   if (!valid_16bit(a.dtype) || (a.index_bits != 32 && a.index_bits != 64) || (!grads && a.out_dtype != a.dtype && a.out_dtype != KEEPVQ_F32)) return KEEPVQ_ERR_DTYPE;
   if (const int rc = check_low_rank_sizes(a.routes, a.sets, a.out_dim, a.in_dim, a.rank, a.x_div)) return rc;
   if (grads ? a.grad_ld < a.out_dim || a.grad_ld % 8 != 0 : a.out_ld < a.out_dim || (a.base && a.base_ld < a.out_dim)) return KEEPVQ_ERR_SHAPE;
+  if (a.grad_ld > LR_MAX_PITCH || a.out_ld > LR_MAX_PITCH || a.base_ld > LR_MAX_PITCH) return KEEPVQ_ERR_CAPACITY;
   if (a.routes > 0 && (!a.x || !a.left || !a.right || !a.indices || (grads ? !a.grad : !a.out))) return KEEPVQ_ERR_NULL;
   for (const void* p : {a.x, a.left, a.right, a.grad, static_cast<const void*>(a.dx), static_cast<const void*>(a.dleft), static_cast<const void*>(a.dright)})
     if (!aligned_to(p, 16)) return KEEPVQ_ERR_ALIGN;

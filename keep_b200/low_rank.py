@@ -9,7 +9,8 @@ Layouts, indices and the rules for captures are those of ``dense_switch``; a dea
 adapter) leaves its base as it is.  ``left`` is ``[sets, out, rank]``, ``right`` ``[sets, rank, in]``, both in x's
 dtype (fp16 or bf16), rank 1 to 128: ranks that are not a multiple of 8 are padded on every call, so a caller
 who keeps such adapters pads them once instead.  ``base`` has x's dtype or is fp32, and so has the result.
-Inner vectors are fp32 sums and enter the second product with 16 (bf16) or 22 (fp16) bits.
+Inner vectors are fp32 sums and enter the second product with 16 bits each (bf16), or with 22 bits of a row's
+largest (fp16: their range does not matter).
 """
 
 from __future__ import annotations
@@ -26,6 +27,7 @@ from .vq import as_device
 __all__ = ["LowRank", "switch_low_rank", "switch_low_rank_grads"]
 
 MAX_RANK = 128
+_MAX_PITCH = 1 << 28  # values from one row of a base to the next
 
 
 @dataclass
@@ -117,7 +119,7 @@ def _forward(x, left, right, indices, base, scale) -> torch.Tensor:
         base_ld = out_shape[-1]
         if not base.is_contiguous():
             # rows may lie apart (one of several projections of a wider product), a row's values may not
-            if base.ndim == 2 and base.stride(1) == 1 and base.stride(0) >= base_ld:
+            if base.ndim == 2 and base.stride(1) == 1 and base_ld <= base.stride(0) <= _MAX_PITCH:
                 base_ld = base.stride(0) if base.shape[0] > 1 else base_ld
             else:
                 base = base.contiguous()

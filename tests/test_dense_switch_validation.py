@@ -101,6 +101,8 @@ def test_what_only_one_direction_looks_at():
     assert lib.keepvq_switch_low_rank(low_rank_args(out_dtype=2), None) == DTYPE
     assert lib.keepvq_switch_low_rank(low_rank_args(base_ld=23), None) == SHAPE
     assert lib.keepvq_switch_low_rank(low_rank_args(out_ld=23), None) == SHAPE
+    for pitch in ("base_ld", "out_ld"):
+        assert lib.keepvq_switch_low_rank(low_rank_args(**{pitch: 1 << 29}), None) == CAPACITY
     assert lib.keepvq_switch_low_rank_grads(low_rank_args(grad_ld=16), None) == SHAPE
     for name, args in (("keepvq_switch_matmul", matmul_args), ("keepvq_switch_low_rank", low_rank_args)):
         assert getattr(lib, name)(args(routes=0), None) == 0  # nothing to do, nothing launched

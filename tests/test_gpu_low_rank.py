@@ -92,6 +92,21 @@ def test_inner_vectors_beyond_the_range_of_fp16(cuda):
     ref.close(switch_low_rank(small, left, right, indices, scale=2.0 ** 14), ref.low_rank(small, left, right, indices, None, 2.0 ** 14))
 
 
+def test_gradients_of_rows_of_very_different_size(cuda):
+    """Rows of one set whose gradients lie 2^-18 apart (fp16), the large ones zero where the small ones are not: what the small
+    rows give a factor's gradient is not lost beside them."""
+    from keep_b200.low_rank import switch_low_rank_grads
+
+    for size in ((24, 1, 1, 64, 48, 16), (200, 1, 2, 128, 72, 8)):
+        x, left, right, indices, _, grad = make(cuda, *size, dtype=FP16, seed=6)
+        odd = torch.arange(size[0], device=cuda) % 2 == 1
+        grad[odd] *= 2.0 ** -9
+        grad[~odd] *= 2.0 ** 9
+        x[odd, :32], x[~odd, 32:] = 0, 0
+        for a, b in zip(switch_low_rank_grads(grad, x, left, right, indices), ref.low_rank_grads(grad, x, left, right, indices, 1.0)):
+            ref.close(a, b)
+
+
 def test_values_that_are_not_finite_stay_where_they_belong(cuda):
     from keep_b200.low_rank import switch_low_rank, switch_low_rank_grads
 
