@@ -19,12 +19,8 @@
 //   FEW   few routes per set, the time is reading weights: one CTA per tile, up to 64 result rows, the
 //         set's rows gathered by TMA, four at a time by their index, straight from the caller's matrix
 //   MANY  two CTAs (of one TPC) per tile of 256 x 256, whose tensor cores work as one: each loads half of
-//         both operands.  TMA's row gather takes 7 cycles a row from warps of its own (20 when one warp issues
-//         from its lanes' registers), a box of 32 neighbouring rows next to nothing: where experts have
-//         hundreds of routes, and for dweight, rows are first copied into the sets' order
-// Measured on a B200 (the listed sizes stand for what a rule covers): 32 experts of 4096 x 2048, 768 routes each, 278 us of
-// products = 1.48 PFLOP/s, 0.90 of cuBLAS's rate on a large matrix; 192 experts of 2304 x 5120, 32 routes each, 717 us =
-// 6.3 TB/s of weights; a token's six experts 24 us = 4.2 TB/s (the tiles of 96 CTAs, each as fast as its loads in flight allow).
+//         both operands.  TMA's row gather is too slow here (about 80 cycles for four rows, measured: 229
+//         TFLOP/s at 768 routes a set), so rows are first copied into the sets' order
 #include "async_copy.cuh"
 #include "switch_plan.cuh"
 
@@ -40,8 +36,8 @@ using fast::smem_addr;
 
 enum { FORWARD = 0, INPUT_GRAD = 1, WEIGHT_GRAD = 2 };
 constexpr int M_TILE = 128, K_BLOCK = 64, N_STEP = 16, BOX_ROWS = 32;  // M_TILE: of a CTA.  // K_BLOCK: 128 bytes, a swizzled row
-constexpr int OUT_WARPS = 8, GATHER_WARPS = 4;
-enum { WARP_M = 0, WARP_N = 1, WARP_MMA = 2, WARP_OUT = 4, WARP_GATHER = WARP_OUT + OUT_WARPS };  // loaders of the two operands, the issuer; the warps of the epilogue
+constexpr int OUT_WARPS = 8, MM_THREADS = 128 + OUT_WARPS * 32;
+enum { WARP_M = 0, WARP_N = 1, WARP_MMA = 2, WARP_OUT = 4 };  // loaders of the two operands, the issuer; the warps of the epilogue
 constexpr uint64_t MM_WAIT_NS = 2000000000ull;
 
 // ---- instructions ---------------------------------------------------------------------------------
@@ -54,15 +50,10 @@ __device__ __forceinline__ void tma_box_3d(uint32_t dst, const CUtensorMap* map,
                     ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
 }
 // Four rows of a matrix, 128 bytes of each from column x on.  The map's box is one row high.
-template <bool PAIR>
-__device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* map, int32_t x, int r0, int r1, int r2, int r3, uint32_t bar) {
-  if (PAIR) asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar) : "memory");
-  else asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
-                    ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3), "r"(bar) : "memory");
+__device__ __forceinline__ void tma_rows4(uint32_t dst, const CUtensorMap* map, int32_t x, const int4& rows, uint32_t bar) {
+  asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];"
+               ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w), "r"(bar) : "memory");
 }
-// A value that is the same in every lane, in a form that the compiler knows to be: operands of copies live in uniform registers.
-__device__ __forceinline__ int uniform(int v) { return static_cast<int>(__reduce_or_sync(0xFFFFFFFFu, static_cast<uint32_t>(v))); }
 // A box from shared memory to the matrix; what lies outside it is not written.
 __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int32_t x, int32_t y, int32_t z, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%1, %2, %3}], [%4];"
@@ -207,11 +198,8 @@ struct Item {
   int k_blocks;
 };
 
-// GATHER (MANY): warps of their own gather the rows of the N operand
-constexpr int threads_of(bool gather) { return 128 + OUT_WARPS * 32 + (gather ? GATHER_WARPS * 32 : 0); }
-
-template <int MODE, bool MANY, bool GATHER>
-__global__ void __launch_bounds__(threads_of(GATHER), 1) switch_matmul_kernel(MatmulArgs a, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map,
+template <int MODE, bool MANY>
+__global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs a, const __grid_constant__ CUtensorMap m_map, const __grid_constant__ CUtensorMap n_map,
                                                                       const __grid_constant__ CUtensorMap out_map) {
   using S = Shape<MANY>;
   static_assert(MANY || MODE != WEIGHT_GRAD, "the rows of dweight's operands are copied first");
@@ -231,7 +219,7 @@ __global__ void __launch_bounds__(threads_of(GATHER), 1) switch_matmul_kernel(Ma
   const uint32_t full = smem_addr(bars), empty = full + 8 * STAGES, acc_full = empty + 8 * STAGES, acc_empty = acc_full + 16;
   if (tid == 0) {
     abort_flag = 0;
-    for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, (GATHER ? 1 + GATHER_WARPS : 2) * CTAS); mbar_init(empty + 8 * s, 1); }
+    for (uint32_t s = 0; s < STAGES; ++s) { mbar_init(full + 8 * s, 2 * CTAS); mbar_init(empty + 8 * s, 1); }
     for (uint32_t s = 0; s < 2; ++s) { mbar_init(acc_full + 8 * s, 1); mbar_init(acc_empty + 8 * s, OUT_WARPS * CTAS); }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -277,7 +265,7 @@ __global__ void __launch_bounds__(threads_of(GATHER), 1) switch_matmul_kernel(Ma
   };
   bool ok = true, mma_issued = false;
 
-  if (warp == WARP_M || (warp == WARP_N && !GATHER)) {
+  if (warp == WARP_M || warp == WARP_N) {
     // ================= the loaders ===============================================================
     Ring<STAGES> r;
     const uint32_t tile = ring + (warp == WARP_N ? S::A_BYTES : 0);
@@ -298,7 +286,7 @@ __global__ void __launch_bounds__(threads_of(GATHER), 1) switch_matmul_kernel(Ma
         if (!MANY && warp == WARP_N) {
           if (lane == 0) expect_bytes<MANY>(bar, static_cast<uint32_t>((it.size + 3) / 4 * 512));
           __syncwarp();
-          if (lane * 4 < it.size) tma_rows4<false>(dst + lane * 512, map, kb * K_BLOCK, rows.x, rows.y, rows.z, rows.w, bar);
+          if (lane * 4 < it.size) tma_rows4(dst + lane * 512, map, kb * K_BLOCK, rows, bar);
         } else if (elect_one()) {
           if (MODE == WEIGHT_GRAD) {  // 64 places of the set's routes (those behind the last are not multiplied) by 64 columns
             const int boxes = warp == WARP_M ? 2 : (half + 63) / 64, col0 = warp == WARP_M ? it.m0 : it.n0 + rank * half;
@@ -350,33 +338,7 @@ __global__ void __launch_bounds__(threads_of(GATHER), 1) switch_matmul_kernel(Ma
       }
       acc.advance();
     }
-  } else if (GATHER && warp >= WARP_GATHER) {
-    // ================= the rows of the N operand, 32 of this CTA's half per warp ==================
-    Ring<STAGES> r;
-    const int mine = (warp - WARP_GATHER) * 32;
-    for (int i = first_item; i < items && ok; i += item_step) {
-      const Item it = item_at(i);
-      const int half = it.n_pad / CTAS, begin = rank * half + mine, last = it.size - 1;
-      const int quads = uniform(max(0, min(min(half - mine, 32), it.size - begin) + 3) / 4);  // rows past the last route repeat it: nobody looks at their columns
-      const int row = a.plan.order[it.start + min(begin + lane, last)] / a.x_div;
-      int rows[32];  // in uniform registers for the whole tile: from a lane's own a copy takes 80 cycles to issue
-#pragma unroll
-      for (int j = 0; j < 32; ++j) rows[j] = uniform(lane == j ? row : 0);
-      for (int kb = 0; kb < it.k_blocks; ++kb) {
-        ok = wait_for(empty + 8 * r.index, r.phase ^ 1u, deadline, aborted);
-        if (!ok) break;
-        const uint32_t bar = full0 + 8 * r.index, dst = ring + r.index * S::STAGE_BYTES + S::A_BYTES + mine * 128;
-        if (elect_one()) {
-          expect_bytes<MANY>(bar, static_cast<uint32_t>(quads * 512));
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (j < quads) tma_rows4<MANY>(dst + j * 512, &n_map, kb * K_BLOCK, rows[4 * j], rows[4 * j + 1], rows[4 * j + 2], rows[4 * j + 3], bar);
-        }
-        __syncwarp();
-        r.advance();
-      }
-    }
-  } else if (warp >= WARP_OUT && warp < WARP_GATHER) {
+  } else if (warp >= WARP_OUT) {
     // ================= the epilogue ================================================================
     // a warp reaches a quarter of the accumulators' lanes; two share it, 32 result rows in turn (one warp alone took longer
     // to drain 256 of them, 530 cycles for 32, than the products of six K blocks)
@@ -532,12 +494,9 @@ static int value_map(CUtensorMap* map, const void* base, int dtype, int64_t widt
   return r == CUDA_SUCCESS ? KEEPVQ_OK : KEEPVQ_ERR_LAUNCH;
 }
 
-// FEW reads the weights as fast as they come up to some 32 routes of an expert; MANY wants tiles enough for its pairs.
+// FEW reads the weights as fast as they come up to some 32 routes per expert; what MANY takes beside that,
+// copying the rows into the experts' order, is two bytes in and out per value of a route.
 static bool many_routes(int64_t routes, int64_t experts) { return routes > 16 * experts && routes >= 256; }
-// MANY, forward: rows gathered by TMA cost some 7 cycles each in every K block, which the products hide up to some 200 routes
-// of an expert; beyond that copying them first is faster.  64 experts, 4096 to 2048, gathered / copied: 94 routes each
-// 203 / 216 us, 192 each 238 / 253 us; 32 experts, 768 each 385 / 354 us.
-static bool copies_rows(int64_t routes, int64_t experts) { return routes > 256 * experts; }
 
 struct Layout {
   Plan plan;
@@ -551,7 +510,7 @@ static Layout lay_out(void* base, int64_t routes, int64_t experts, int64_t out_d
   const int64_t places = max_places(routes, experts);
   Layout l;
   l.plan = take_plan(s, routes, experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX);
-  l.x = grads || (many && copies_rows(routes, experts)) ? s.take<uint16_t>(places * in_dim) : nullptr;
+  l.x = many || grads ? s.take<uint16_t>(places * in_dim) : nullptr;
   l.grad = grads ? s.take<uint16_t>(places * align_up(out_dim, 8)) : nullptr;
   l.route_dx = grads && x_div > 1 ? s.take<float>(routes * in_dim) : nullptr;
   l.bytes = s.used;
@@ -567,7 +526,7 @@ static int check_sizes(int64_t routes, int64_t experts, int64_t out_dim, int64_t
   return KEEPVQ_OK;
 }
 
-template <int MODE, bool MANY, bool GATHER = false>
+template <int MODE, bool MANY>
 static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cudaStream_t s) {
   using S = Shape<MANY>;
   MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.routes, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan};
@@ -576,15 +535,14 @@ static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cud
   int rc = MODE == WEIGHT_GRAD ? value_map(&m_map, l.x, a.dtype, a.in_dim, a.in_dim, places, 1, K_BLOCK)
                                : value_map(&m_map, a.weight, a.dtype, a.in_dim, a.in_dim, a.out_dim, a.experts, MODE == FORWARD ? M_TILE : K_BLOCK);
   if (rc) return rc;
-  constexpr bool COPIED = MANY && !GATHER;
-  const uint32_t box = MODE == WEIGHT_GRAD ? K_BLOCK : COPIED ? BOX_ROWS : 0;
-  rc = MODE == FORWARD ? value_map(&n_map, COPIED ? l.x : a.x, a.dtype, a.in_dim, a.in_dim, COPIED ? places : a.routes / a.x_div, 1, box)
+  const uint32_t box = MODE == WEIGHT_GRAD ? K_BLOCK : MANY ? BOX_ROWS : 0;
+  rc = MODE == FORWARD ? value_map(&n_map, MANY ? l.x : a.x, a.dtype, a.in_dim, a.in_dim, MANY ? places : a.routes / a.x_div, 1, box)
                        : value_map(&n_map, MANY ? l.grad : a.grad, a.dtype, a.out_dim, grad_ld, MANY ? places : a.routes, 1, box);
   if (rc) return rc;
   out_map = m_map;
   if (MODE == WEIGHT_GRAD)
     if ((rc = value_map(&out_map, a.dweight, a.dtype, a.in_dim, a.in_dim, a.out_dim, a.experts, 32, 32))) return rc;
-  auto kernel = switch_matmul_kernel<MODE, MANY, GATHER>;
+  auto kernel = switch_matmul_kernel<MODE, MANY>;
   static uint64_t configured = 0;  // one bit per device: the shared-memory opt-in is a per-device attribute of the function
   int dev = 0, sms = 148;
   cudaGetDevice(&dev);
@@ -596,7 +554,7 @@ static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cud
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   cudaLaunchConfig_t config = {};
   config.gridDim = dim3(MANY ? sms / 2 * 2 : sms);
-  config.blockDim = dim3(threads_of(GATHER));
+  config.blockDim = dim3(MM_THREADS);
   config.dynamicSmemBytes = S::SMEM_BYTES;
   config.stream = s;
   cudaLaunchAttribute attribute = {};
@@ -648,7 +606,6 @@ int keepvq_switch_matmul(const keepvq_switch_matmul_args* args, void* stream) {
   const bool many = many_routes(a.routes, a.experts);
   if (const int rc = make_plan({a.indices, a.index_bits}, a.routes, a.experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX, many ? Shape<true>::PAD : N_STEP, l.plan, s)) return rc;
   if (!many) return launch_tiles<FORWARD, false>(a, l, s);
-  if (!copies_rows(a.routes, a.experts)) return launch_tiles<FORWARD, true, true>(a, l, s);
   const RowCopy x{a.x, l.x, a.in_dim, a.in_dim, a.x_div};
   if (const int rc = copy_rows(&x, 1, a.routes, a.experts, l.plan, s)) return rc;
   return launch_tiles<FORWARD, true>(a, l, s);
