@@ -15,6 +15,11 @@
 // the inner vectors never leave the SMs, and one row of one set still has a whole cluster's loads in
 // flight.  Forward: A, then B.  Input gradient: B^T, then A^T, whose fragments are transposed in registers.
 //
+// Measured on a B200, 4096 -> 4096, bf16: one row of rank 16 6 us on the device, 61 rows of rank 32 11 us cold; 251 tokens with
+// six of 384 corrections of rank 8 20 us; 4096 rows of rank 16 / 64 / 128 35 / 47 / 82 us with the plan, where x, base and
+// results are 100 MB.  What bounds it then is instructions and latency per 16 rows, not bytes.  Tiles of 64 rows shared
+// by the warps through ldmatrix were slower at every rank from 32 on (4096 rows of rank 64: 67 us).
+//
 // Inner vectors are fp32 sums; for the second product each is split into the sum of two 16-bit values, scaled
 // by a power of two per row for fp16 so that neither its range nor its small values are lost.
 #include "switch_plan.cuh"
@@ -152,6 +157,7 @@ __device__ __forceinline__ void low_rank_plain_row(const LowRankArgs& a, int64_t
     for (int i = tid; i < a.width; i += LR_THREADS) reinterpret_cast<uint16_t*>(to)[i] = from ? reinterpret_cast<const uint16_t*>(from)[i] : static_cast<uint16_t>(0);
   }
 }
+
 // The inner vectors of a tile for the gradients of the factors.
 template <int RP, int ROWS>
 __device__ __forceinline__ void keep_inner(const LowRankArgs& a, const float* inner, int start, int size) {
@@ -166,6 +172,7 @@ __device__ __forceinline__ void keep_inner(const LowRankArgs& a, const float* in
     reinterpret_cast<uint32_t*>(a.keep.low)[at] = low;
   }
 }
+
 // `own`, this CTA's part of the sums of all rows, becomes `inner`, the cluster's (in the order of its CTAs), with a
 // power of two per row for fp16.
 template <typename T, int RP, int ROWS>
@@ -195,9 +202,9 @@ __device__ __forceinline__ void meet(const float* own, float* inner, float* unit
 // RP: the rank rounded up (zeros).  BACK: both factors are used transposed.
 template <int RP, bool BACK>
 struct LowRankShape {
-  static constexpr int MT = 1, ROWS = 16, RT = RP / 8, KC = RP / 16, V = RP >= 32 ? 8 : 4, CC = RP / (4 * V);  // V: neighbouring ranks a lane holds
-  static constexpr int FACTOR1 = BACK ? 4 * CC : RT, FACTOR2 = BACK ? 2 * KC : 4 * CC;  // pieces of a step: the factor's, and 2 MT of the rows
-  static constexpr int PIECES = 2 * MT + (FACTOR1 > FACTOR2 ? FACTOR1 : FACTOR2), STEP_BYTES = PIECES * 32 * 16;
+  static constexpr int ROWS = 16, RT = RP / 8, KC = RP / 16, V = RP >= 32 ? 8 : 4, CC = RP / (4 * V);  // V: neighbouring ranks a lane holds
+  static constexpr int FACTOR1 = BACK ? 4 * CC : RT, FACTOR2 = BACK ? 2 * KC : 4 * CC;  // pieces of a step: the factor's, and two of the rows
+  static constexpr int PIECES = 2 + (FACTOR1 > FACTOR2 ? FACTOR1 : FACTOR2), STEP_BYTES = PIECES * 32 * 16;
   static constexpr bool SMALL = RP <= 16;  // three CTAs on an SM instead of two: calls of many sets with a few rows each
   static constexpr int BUDGET = SMALL ? 9 * 1024 : 12 * 1024, STEPS = BUDGET / STEP_BYTES < 2 ? 2 : BUDGET / STEP_BYTES;  // per warp; some 200 KB in flight on an SM
   static constexpr int QUEUES = LR_WARPS * STEPS * STEP_BYTES;
@@ -211,7 +218,7 @@ template <typename T, int RP, bool BACK>
 __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_rank_kernel(LowRankArgs a) {
   grid_wait();
   using S = LowRankShape<RP, BACK>;
-  constexpr int MT = S::MT, ROWS = S::ROWS, RT = S::RT, V = S::V, KC = S::KC, CC = S::CC, STEPS = S::STEPS;
+  constexpr int ROWS = S::ROWS, RT = S::RT, V = S::V, KC = S::KC, CC = S::CC, STEPS = S::STEPS;
   extern __shared__ __align__(16) float sm[];
   float* part = sm;                                     // [warps][ROWS][RP], behind the queues of the first product
   float* own = sm + S::QUEUES / 4;                      // [ROWS][RP] of this CTA; then of the cluster
@@ -245,18 +252,14 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
 
   // ---- the first product: rows [ROWS, depth] times the factor -> [ROWS, RP]
   {
-    float acc[MT][RT][4];
+    float acc[RT][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < RT; ++n)
 #pragma unroll
-      for (int n = 0; n < RT; ++n)
+      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
+    int row[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) acc[m][n][i] = 0.0f;
-    int row[MT][2];
-#pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) row[m][h] = route_of[m * 16 + h * 8 + g] / a.in_div;
+    for (int h = 0; h < 2; ++h) row[h] = route_of[h * 8 + g] / a.in_div;
     // (rows and ranks times row lengths in bytes are 32 x 32 bit products: one instruction an address)
     const int depth = static_cast<int>(a.depth), in_ld = static_cast<int>(a.in_ld), in_bytes = in_ld * 2, stride = ctas * LR_WARPS * CHUNK, k_first = (rank * LR_WARPS + warp) * CHUNK;
     const char* in_k = reinterpret_cast<const char*>(a.in + k_first + q * 8);
@@ -268,12 +271,10 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
     auto fill = [&](int at) {
       const bool there = k_fill + q * 8 < in_ld;  // (values of `in` between depth and in_ld are zeros)
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) copy16(slot(at, 2 * m + h), in_k + static_cast<int64_t>(row[m][h]) * in_bytes, there);
+      for (int h = 0; h < 2; ++h) copy16(slot(at, h), in_k + static_cast<int64_t>(row[h]) * in_bytes, there);
       if (!BACK) {
 #pragma unroll
-        for (int n = 0; n < RT; ++n) copy16(slot(at, 2 * MT + n), factor_k + static_cast<int64_t>(n * 8) * factor_bytes, there && n * 8 + g < a.rank);
+        for (int n = 0; n < RT; ++n) copy16(slot(at, 2 + n), factor_k + static_cast<int64_t>(n * 8) * factor_bytes, there && n * 8 + g < a.rank);
         factor_k += stride * 2;
       } else {
         // the factor's rows lie along the contraction: 8 x 8 blocks of it are transposed in registers.  Row i of a
@@ -285,8 +286,8 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
 #pragma unroll
           for (int c = 0; c < CC; ++c) {
             const char* from = factor_k + static_cast<int64_t>(more) * factor_bytes + c * 4 * V * 2;
-            if (V == 8) copy16(slot(at, 2 * MT + i * CC + c), from, is && c * 4 * V + q * V < a.rank);
-            else copy8(slot(at, 2 * MT + i * CC + c), from, is && c * 4 * V + q * V < a.rank);
+            if (V == 8) copy16(slot(at, 2 + i * CC + c), from, is && c * 4 * V + q * V < a.rank);
+            else copy8(slot(at, 2 + i * CC + c), from, is && c * 4 * V + q * V < a.rank);
           }
         }
         factor_k += static_cast<int64_t>(stride) * factor_bytes;
@@ -304,36 +305,28 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
       if (k_fill < depth) fill(at == 0 ? STEPS - 1 : at - 1);
       step_issued();
       all_but<STEPS - 1>();
-      uint4 v[MT][2];
+      uint4 v[2];
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) v[m][h] = piece16(slot(at, 2 * m + h));
+      for (int h = 0; h < 2; ++h) v[h] = piece16(slot(at, h));
       if (!BACK) {
 #pragma unroll
         for (int n = 0; n < RT; ++n) {
-          const uint4 w = piece16(slot(at, 2 * MT + n));
-#pragma unroll
-          for (int m = 0; m < MT; ++m) {
-            const uint32_t a0[4] = {v[m][0].x, v[m][1].x, v[m][0].y, v[m][1].y}, a1[4] = {v[m][0].z, v[m][1].z, v[m][0].w, v[m][1].w};
-            Mma<T>::run(acc[m][n], a0, w.x, w.y);
-            Mma<T>::run(acc[m][n], a1, w.z, w.w);
-          }
+          const uint4 w = piece16(slot(at, 2 + n));
+          const uint32_t a0[4] = {v[0].x, v[1].x, v[0].y, v[1].y}, a1[4] = {v[0].z, v[1].z, v[0].w, v[1].w};
+          Mma<T>::run(acc[n], a0, w.x, w.y);
+          Mma<T>::run(acc[n], a1, w.z, w.w);
         }
       } else {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int c = 0; c < CC; ++c) {
-            const uint4 w0 = piece16(slot(at, 2 * MT + 2 * j * CC + c)), w1 = piece16(slot(at, 2 * MT + (2 * j + 1) * CC + c));
+            const uint4 w0 = piece16(slot(at, 2 + 2 * j * CC + c)), w1 = piece16(slot(at, 2 + (2 * j + 1) * CC + c));
 #pragma unroll
             for (int t = 0; t < V / 2; ++t) {
               const uint32_t b0 = transpose8(word(w0, t)), b1 = transpose8(word(w1, t));
-#pragma unroll
-              for (int m = 0; m < MT; ++m) {
-                const uint32_t av[4] = {j ? v[m][0].z : v[m][0].x, j ? v[m][1].z : v[m][1].x, j ? v[m][0].w : v[m][0].y, j ? v[m][1].w : v[m][1].y};
-                Mma<T>::run(acc[m][c * (V / 2) + t], av, b0, b1);
-              }
+              const uint32_t av[4] = {j ? v[0].z : v[0].x, j ? v[1].z : v[1].x, j ? v[0].w : v[0].y, j ? v[1].w : v[1].y};
+              Mma<T>::run(acc[c * (V / 2) + t], av, b0, b1);
             }
           }
         }
@@ -344,14 +337,12 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
     __syncthreads();  // the queues make room for the partial sums
     // a lane's ranks of tile n: 8 n + 2 q and the next; transposed: c * 4 V + V q + 2 t and the next
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int n = 0; n < RT; ++n) {
+      const int j = BACK ? n / (V / 2) * 4 * V + V * q + 2 * (n % (V / 2)) : 8 * n + 2 * q;
 #pragma unroll
-      for (int n = 0; n < RT; ++n) {
-        const int j = BACK ? n / (V / 2) * 4 * V + V * q + 2 * (n % (V / 2)) : 8 * n + 2 * q;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-          *reinterpret_cast<float2*>(part + (warp * ROWS + m * 16 + h * 8 + g) * RP + j) = make_float2(acc[m][n][2 * h], acc[m][n][2 * h + 1]);
-      }
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(part + (warp * ROWS + h * 8 + g) * RP + j) = make_float2(acc[n][2 * h], acc[n][2 * h + 1]);
+    }
   }
   __syncthreads();
   for (int i = tid; i < ROWS * RP; i += LR_THREADS) {
@@ -372,11 +363,9 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
                            (BACK ? static_cast<int64_t>((V == 8 ? 8 : 4) * (g >> 1) + (g & 1)) * factor_bytes + (n_first + 8 * q) * 2 : static_cast<int64_t>(n_first + 8 * (g >> 1) + (g & 1)) * factor_bytes + q * V * 2);
     const char* base_n = static_cast<const char*>(a.base) + (n_first + 8 * q) * 2;
     char* out_n = static_cast<char*>(a.out) + (n_first + 8 * q) * size_of;
-    int route[MT][2];
+    int route[2];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) route[m][h] = route_of[m * 16 + h * 8 + g];
+    for (int h = 0; h < 2; ++h) route[h] = route_of[h * 8 + g];
     int n_fill = n_first;
     // the pieces of the next 32 columns: the factor by RP, whose column c of tile t is 8 (c / 2) + 2 t + c % 2, so that a
     // lane's results are neighbours; and the base of all rows
@@ -406,9 +395,7 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
       }
       if (queued_base) {
 #pragma unroll
-        for (int m = 0; m < MT; ++m)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) copy16(slot(at, S::FACTOR2 + 2 * m + h), base_n + static_cast<int64_t>(route[m][h]) * base_bytes, m * 16 + h * 8 + g < size && n_fill + 8 * q < width);
+        for (int h = 0; h < 2; ++h) copy16(slot(at, S::FACTOR2 + h), base_n + static_cast<int64_t>(route[h]) * base_bytes, h * 8 + g < size && n_fill + 8 * q < width);
         base_n += stride * 2;
       }
       n_fill += stride;
@@ -418,19 +405,17 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
       if (n_fill < width) fill(i);
       step_issued();
     }
-    uint32_t high[MT][KC][4], low[MT][KC][4];
+    uint32_t high[KC][4], low[KC][4];
 #pragma unroll
-    for (int m = 0; m < MT; ++m)
+    for (int c = 0; c < KC; ++c)
 #pragma unroll
-      for (int c = 0; c < KC; ++c)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int r = m * 16 + (i & 1) * 8 + g;
-          const int j = V == 8 ? c / 2 * 32 + 8 * q + 4 * (c & 1) + 2 * (i >> 1) : 4 * q + 2 * (i >> 1);
-          const float2 v = *reinterpret_cast<const float2*>(inner + r * RP + j);
-          const float u = Mma<T>::SCALED ? 1.0f / unit[r] : 1.0f;  // (a power of two)
-          split<T>(v.x * u, v.y * u, high[m][c][i], low[m][c][i]);
-        }
+      for (int i = 0; i < 4; ++i) {
+        const int r = (i & 1) * 8 + g;
+        const int j = V == 8 ? c / 2 * 32 + 8 * q + 4 * (c & 1) + 2 * (i >> 1) : 4 * q + 2 * (i >> 1);
+        const float2 v = *reinterpret_cast<const float2*>(inner + r * RP + j);
+        const float u = Mma<T>::SCALED ? 1.0f / unit[r] : 1.0f;  // (a power of two)
+        split<T>(v.x * u, v.y * u, high[c][i], low[c][i]);
+      }
     int at = 0;
     for (int n0 = n_first; n0 < width; n0 += stride, out_n += stride * size_of) {
       if (n_fill < width) fill(at == 0 ? STEPS - 1 : at - 1);
@@ -457,57 +442,53 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
           }
       }
       const int n = n0 + 8 * q;
+      float d[4][4];
 #pragma unroll
-      for (int m = 0; m < MT; ++m) {
-        if (m * 16 >= size) break;
-        float d[4][4];
+      for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int i = 0; i < 4; ++i) d[t][i] = 0.0f;
+      }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) d[t][i] = 0.0f;
-        }
+      for (int c = 0; c < KC; ++c) {
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
+        for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], low[c], b[t][c][0], b[t][c][1]);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], low[m][c], b[t][c][0], b[t][c][1]);
+        for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], high[c], b[t][c][0], b[t][c][1]);
+      }
 #pragma unroll
-          for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], high[m][c], b[t][c][0], b[t][c][1]);
-        }
+      for (int h = 0; h < 2; ++h) {
+        const int r = h * 8 + g;
+        if (r >= size) continue;
+        char* to = out_n + static_cast<int64_t>(route[h]) * out_bytes;
+        const float s = Mma<T>::SCALED ? a.second_scale * unit[r] : a.second_scale;
+        float y[8];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = m * 16 + h * 8 + g;
-          if (r >= size) continue;
-          char* to = out_n + static_cast<int64_t>(route[m][h]) * out_bytes;
-          const float s = Mma<T>::SCALED ? a.second_scale * unit[r] : a.second_scale;
-          float y[8];
+        for (int t = 0; t < 4; ++t) { y[2 * t] = s * d[t][2 * h]; y[2 * t + 1] = s * d[t][2 * h + 1]; }
+        if (a.whole) {
+          if (n >= width) continue;
+          if (a.out32) {
+            float v[8] = {};
+            if (a.base) load8_as_float(static_cast<const float*>(a.base) + route[h] * a.base_ld + n, v);
 #pragma unroll
-          for (int t = 0; t < 4; ++t) { y[2 * t] = s * d[t][2 * h]; y[2 * t + 1] = s * d[t][2 * h + 1]; }
-          if (a.whole) {
-            if (n >= width) continue;
-            if (a.out32) {
-              float v[8] = {};
-              if (a.base) load8_as_float(static_cast<const float*>(a.base) + route[m][h] * a.base_ld + n, v);
-#pragma unroll
-              for (int i = 0; i < 8; ++i) v[i] += y[i];
-              store8_from_float(reinterpret_cast<float*>(to), v);
-            } else {
-              if (a.base) {
-                const uint4 rest = piece16(slot(at, S::FACTOR2 + 2 * m + h));
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const float2 v = Mma<T>::unpack(word(rest, i));
-                  y[2 * i] += v.x;
-                  y[2 * i + 1] += v.y;
-                }
-              }
-              store8_from_float(reinterpret_cast<T*>(to), y);
-            }
+            for (int i = 0; i < 8; ++i) v[i] += y[i];
+            store8_from_float(reinterpret_cast<float*>(to), v);
           } else {
-            const int dtype = a.out32 ? KEEPVQ_F32 : Mma<T>::SCALED ? KEEPVQ_F16 : KEEPVQ_BF16;
+            if (a.base) {
+              const uint4 rest = piece16(slot(at, S::FACTOR2 + h));
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (n + i < width) store_from_float(to, dtype, i, y[i] + (a.base ? load_as_float(a.base, dtype, route[m][h] * a.base_ld + n + i) : 0.0f));
+              for (int i = 0; i < 4; ++i) {
+                const float2 v = Mma<T>::unpack(word(rest, i));
+                y[2 * i] += v.x;
+                y[2 * i + 1] += v.y;
+              }
+            }
+            store8_from_float(reinterpret_cast<T*>(to), y);
           }
+        } else {
+          const int dtype = a.out32 ? KEEPVQ_F32 : Mma<T>::SCALED ? KEEPVQ_F16 : KEEPVQ_BF16;
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (n + i < width) store_from_float(to, dtype, i, y[i] + (a.base ? load_as_float(a.base, dtype, route[h] * a.base_ld + n + i) : 0.0f));
         }
       }
       if (++at == STEPS) at = 0;
@@ -516,276 +497,7 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
   }
   if (ctas > 1) lr_cluster_sync();  // the others may still be reading this CTA's partial sums
 }
-// ---- the same for many rows of a set -------------------------------------------------------------------
-// 64 rows of a set per cluster, whose CTAs split the first contraction and then the width of the result.
-// Here the warps share what is loaded: stages of 64 values of a contraction (or columns), rows of 128 bytes
-// that eight lanes copy together, read as fragments by ldmatrix.  Against the kernel above, whose warps each
-// have all rows and a part of the contraction: a quarter of the factor's bytes from the cache and a third of the
-// instructions per row (4096 rows of rank 64 at 4096 x 4096: 52 us there).
-constexpr int TILE_ROWS = 64, TILE_K = 64;
-template <int RP>
-struct TileShape {
-  static constexpr int ROW_BYTES = TILE_ROWS * 128, FACTOR_BYTES = TILE_K * RP * 2, STAGE_BYTES = ROW_BYTES + FACTOR_BYTES;
-  static constexpr int STAGES = RP <= 32 ? 5 : RP <= 64 ? 4 : 3;
-  static constexpr int BYTES = STAGES * STAGE_BYTES + 2 * TILE_ROWS * RP * 4 + 2 * TILE_ROWS * 4;
-  static constexpr int CTAS = BYTES + 1024 <= 114 * 1024 ? 2 : 1;  // on an SM
-};
-__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t row) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(row) : "memory");
-}
-__device__ __forceinline__ void ldmatrix4_transposed(uint32_t (&r)[4], uint32_t row) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(row) : "memory");
-}
-__device__ __forceinline__ void stmatrix4(uint32_t row, const uint32_t (&r)[4]) {
-  asm volatile("stmatrix.sync.aligned.m8n8.x4.shared.b16 [%0], {%1,%2,%3,%4};" ::"r"(row), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
-}
-// Where 16-byte piece c of row r of a tile lies: pieces are permuted so that eight rows' same piece never meet in a bank.
-template <int WIDTH>  // bytes of a row
-__device__ __forceinline__ uint32_t tile_at(int r, int c) {
-  constexpr int PER = WIDTH >= 128 ? 1 : 128 / WIDTH, MASK = WIDTH >= 128 ? 7 : WIDTH / 16 - 1;
-  return static_cast<uint32_t>(r * WIDTH + ((c ^ ((r / PER) & MASK)) << 4));
-}
 
-template <typename T, int RP, bool BACK>
-__global__ void __launch_bounds__(LR_THREADS, TileShape<RP>::CTAS) low_rank_tile_kernel(LowRankArgs a) {
-  grid_wait();
-  using S = TileShape<RP>;
-  constexpr int STAGES = S::STAGES, KC = RP / 16, FW = RP * 2;  // FW: bytes of a factor's row along the rank
-  constexpr bool SPLIT_K = RP == 16;                            // two warps share 16 rows: halves of the ranks, or of a stage's contraction
-  constexpr int NT = SPLIT_K ? 2 : RP / 16;                     // 8-rank tiles of a warp
-  extern __shared__ __align__(128) float tile_sm[];
-  float* own = tile_sm + STAGES * S::STAGE_BYTES / 4;     // [64][RP] of this CTA; then of the cluster
-  float* inner = own + TILE_ROWS * RP;
-  float* unit = inner + TILE_ROWS * RP;                   // [64]
-  int* route_of = reinterpret_cast<int*>(unit + TILE_ROWS);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3, wm = warp & 3, wh = warp >> 2;
-  const int ctas = static_cast<int>(lr_cluster_size()), rank = static_cast<int>(lr_cluster_rank()), tile = blockIdx.x / ctas;
-  const uint32_t stages = static_cast<uint32_t>(__cvta_generic_to_shared(tile_sm));
-  if (a.dead_rows)
-    for (int p = blockIdx.x; p < *a.plan.dead_count; p += gridDim.x) low_rank_plain_row(a, a.plan.dead[p]);
-  if (tile >= *a.plan.tiles) return;
-  const int4 t = a.plan.tile[tile];
-  const int set = t.x, start = t.y, size = t.z;
-  if (tid < TILE_ROWS) route_of[tid] = a.plan.order[start + min(tid, size - 1)];  // rows past the last repeat it and are not stored
-  __syncthreads();
-  const int row8 = tid >> 3, piece8 = tid & 7;                     // of a tile with rows of 128 bytes, 32 rows further with every 256 pieces
-  constexpr int FP = RP / 8;                                       // pieces of a row along the rank
-  const int row_f = tid / FP, piece_f = tid % FP;
-  // this CTA's stages of a contraction (or a width) of n values: a contiguous part
-  auto share = [&](int n, int& first, int& end) {
-    const int all = (n + TILE_K - 1) / TILE_K, each = (all + ctas - 1) / ctas;
-    first = min(all, rank * each);
-    end = min(all, first + each);
-  };
-
-  // ---- the first product
-  {
-    const int depth = static_cast<int>(a.depth), in_ld = static_cast<int>(a.in_ld);
-    int first, end;
-    share(depth, first, end);
-    const char* in_row[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) in_row[i] = reinterpret_cast<const char*>(a.in + static_cast<int64_t>(route_of[row8 + 32 * i] / a.in_div) * in_ld + piece8 * 8);
-    const char* factor = reinterpret_cast<const char*>(a.first + static_cast<int64_t>(set) * a.rank * depth);
-    auto fill = [&](int slot, int at) {
-      const uint32_t base = stages + slot * S::STAGE_BYTES;
-      const int k0 = at * TILE_K;
-      const bool there = k0 + piece8 * 8 < in_ld;
-#pragma unroll
-      for (int i = 0; i < 2; ++i) copy16(base + tile_at<128>(row8 + 32 * i, piece8), in_row[i] + k0 * 2, there);
-#pragma unroll
-      for (int i = 0; i < (RP * 8 + LR_THREADS - 1) / LR_THREADS; ++i) {
-        if (!BACK) {  // [RP][64]
-          const int j = row8 + 32 * i;
-          if (RP >= 32 || j < RP) copy16(base + S::ROW_BYTES + tile_at<128>(j, piece8), factor + (static_cast<int64_t>(j) * depth + k0 + piece8 * 8) * 2, there && j < a.rank);
-        } else {      // [64][RP]
-          const int r = row_f + i * (LR_THREADS / FP), k = k0 + r;
-          if (RP >= 32 || r < TILE_K) copy16(base + S::ROW_BYTES + tile_at<FW>(r, piece_f), factor + (static_cast<int64_t>(k) * a.rank + piece_f * 8) * 2, k < depth && piece_f * 8 < a.rank);
-        }
-      }
-    };
-    float acc[NT][4];
-#pragma unroll
-    for (int n = 0; n < NT; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) acc[n][i] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) {
-      if (first + i < end) fill(i, first + i);
-      step_issued();
-    }
-    int slot = 0;
-    for (int at = first; at < end; ++at) {
-      all_but<STAGES - 2>();
-      __syncthreads();  // this stage is there for everybody, and the one before it is used up
-      if (at + STAGES - 1 < end) fill(slot == 0 ? STAGES - 1 : slot - 1, at + STAGES - 1);
-      step_issued();
-      const uint32_t rows = stages + slot * S::STAGE_BYTES, fac = rows + S::ROW_BYTES;
-#pragma unroll
-      for (int kk = 0; kk < (SPLIT_K ? 2 : 4); ++kk) {
-        const int ks = SPLIT_K ? wh * 2 + kk : kk;
-        uint32_t x[4];
-        ldmatrix4(x, rows + tile_at<128>(wm * 16 + (lane & 15), 2 * ks + (lane >> 4)));
-#pragma unroll
-        for (int n = 0; n < NT; n += 2) {
-          const int n0 = SPLIT_K ? 0 : wh * (RP / 2) + n * 8;
-          uint32_t w[4];
-          if (!BACK) ldmatrix4(w, fac + tile_at<128>(n0 + (lane & 7) + ((lane >> 4) << 3), 2 * ks + ((lane >> 3) & 1)));
-          else ldmatrix4_transposed(w, fac + tile_at<FW>(ks * 16 + (lane & 15), n0 / 8 + (lane >> 4)));
-          Mma<T>::run(acc[n], x, w[0], w[1]);
-          Mma<T>::run(acc[n + 1], x, w[2], w[3]);
-        }
-      }
-      if (++slot == STAGES) slot = 0;
-    }
-    all_but<0>();
-    float* to = SPLIT_K && wh ? inner : own;
-#pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      const int j = (SPLIT_K ? 0 : wh * (RP / 2)) + n * 8 + 2 * q;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) *reinterpret_cast<float2*>(to + (wm * 16 + h * 8 + g) * RP + j) = make_float2(a.first_scale * acc[n][2 * h], a.first_scale * acc[n][2 * h + 1]);
-    }
-    __syncthreads();
-    if (SPLIT_K) {
-      for (int i = tid; i < TILE_ROWS * RP; i += LR_THREADS) own[i] += inner[i];
-      __syncthreads();
-    }
-  }
-
-  // ---- the second product, whose first stages are on their way while the partial sums meet
-  const bool queued_base = a.base && a.whole && !a.out32;
-  const int width = static_cast<int>(a.width);
-  int first = 0, end = 0;
-  if (a.second) share(width, first, end);
-  const char* base_row[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) base_row[i] = static_cast<const char*>(a.base) + (route_of[row8 + 32 * i] * a.base_ld + piece8 * 8) * 2;
-  const char* factor = reinterpret_cast<const char*>(a.second + static_cast<int64_t>(set) * a.rank * width);
-  auto fill = [&](int slot, int at) {
-    const uint32_t to = stages + slot * S::STAGE_BYTES;
-    const int n0 = at * TILE_K;
-    if (queued_base) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) copy16(to + tile_at<128>(row8 + 32 * i, piece8), base_row[i] + n0 * 2, row8 + 32 * i < size && n0 + piece8 * 8 < width);
-    }
-#pragma unroll
-    for (int i = 0; i < (RP * 8 + LR_THREADS - 1) / LR_THREADS; ++i) {
-      if (BACK) {  // [RP][64]
-        const int j = row8 + 32 * i;
-        if (RP >= 32 || j < RP) copy16(to + S::ROW_BYTES + tile_at<128>(j, piece8), factor + (static_cast<int64_t>(j) * width + n0 + piece8 * 8) * 2, n0 + piece8 * 8 < width && j < a.rank);
-      } else {     // [64][RP]
-        const int r = row_f + i * (LR_THREADS / FP), n = n0 + r;
-        if (RP >= 32 || r < TILE_K) copy16(to + S::ROW_BYTES + tile_at<FW>(r, piece_f), factor + (static_cast<int64_t>(n) * a.rank + piece_f * 8) * 2, n < width && piece_f * 8 < a.rank);
-      }
-    }
-  };
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    if (first + i < end) fill(i, first + i);
-    step_issued();
-  }
-  meet<T, RP, TILE_ROWS>(own, inner, unit, ctas);
-  if (a.keep.high && rank == 0) keep_inner<RP, TILE_ROWS>(a, inner, start, size);
-  if (a.second) {
-    uint32_t high[KC][4], low[KC][4];
-#pragma unroll
-    for (int c = 0; c < KC; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = wm * 16 + (i & 1) * 8 + g;
-        const float2 v = *reinterpret_cast<const float2*>(inner + r * RP + c * 16 + 2 * q + 8 * (i >> 1));
-        const float u = Mma<T>::SCALED ? 1.0f / unit[r] : 1.0f;  // (a power of two)
-        split<T>(v.x * u, v.y * u, high[c][i], low[c][i]);
-      }
-    float scale[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) scale[h] = Mma<T>::SCALED ? a.second_scale * unit[wm * 16 + h * 8 + g] : a.second_scale;
-    const int size_of = a.out32 ? 4 : 2;
-    int slot = 0;
-    for (int at = first; at < end; ++at) {
-      all_but<STAGES - 2>();
-      __syncthreads();
-      if (at + STAGES - 1 < end) fill(slot == 0 ? STAGES - 1 : slot - 1, at + STAGES - 1);
-      step_issued();
-      const uint32_t rows = stages + slot * S::STAGE_BYTES, fac = rows + S::ROW_BYTES;
-      if (++slot == STAGES) slot = 0;
-      if (wm * 16 >= size) continue;  // (nothing of this warp's is stored)
-      float d[4][4];
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[n][i] = 0.0f;
-#pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        uint32_t w[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-          const int n0 = wh * 32 + n * 16;
-          if (!BACK) ldmatrix4(w[n], fac + tile_at<FW>(n0 + (lane & 7) + ((lane >> 4) << 3), 2 * c + ((lane >> 3) & 1)));
-          else ldmatrix4_transposed(w[n], fac + tile_at<128>(c * 16 + (lane & 15), n0 / 8 + (lane >> 4)));
-        }
-#pragma unroll
-        for (int n = 0; n < 4; ++n) Mma<T>::run(d[n], low[c], w[n >> 1][2 * (n & 1)], w[n >> 1][2 * (n & 1) + 1]);
-#pragma unroll
-        for (int n = 0; n < 4; ++n) Mma<T>::run(d[n], high[c], w[n >> 1][2 * (n & 1)], w[n >> 1][2 * (n & 1) + 1]);
-      }
-#pragma unroll
-      for (int n = 0; n < 4; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) d[n][i] *= scale[i >> 1];
-      const int col0 = at * TILE_K + wh * 32;
-      if (a.whole && !a.out32) {
-        // through the stage's own rows: the base leaves them as fragments, the results take its place, and go out in pieces
-#pragma unroll
-        for (int n = 0; n < 4; n += 2) {
-          const uint32_t where = rows + tile_at<128>(wm * 16 + (lane & 15), wh * 4 + n + (lane >> 4));
-          uint32_t y[4] = {0, 0, 0, 0};
-          if (a.base) ldmatrix4(y, where);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = a.base ? Mma<T>::unpack(y[i]) : make_float2(0.0f, 0.0f);
-            const float* r = d[n + (i >> 1)] + 2 * (i & 1);
-            y[i] = Mma<T>::pack(v.x + r[0], v.y + r[1]);
-          }
-          __syncwarp();
-          stmatrix4(where, y);
-        }
-        __syncwarp();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = wm * 16 + h * 8 + g, n = col0 + q * 8;
-          const uint4 eight = piece16(rows + tile_at<128>(r, wh * 4 + q));
-          if (r < size && n < width) *reinterpret_cast<uint4*>(static_cast<char*>(a.out) + (route_of[r] * a.out_ld + n) * 2) = eight;
-        }
-      } else {
-        const int dtype = a.out32 ? KEEPVQ_F32 : Mma<T>::SCALED ? KEEPVQ_F16 : KEEPVQ_BF16;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int r = wm * 16 + h * 8 + g;
-          if (r >= size) continue;
-          char* to = static_cast<char*>(a.out) + route_of[r] * a.out_ld * size_of;
-          const char* from = static_cast<const char*>(a.base) + route_of[r] * a.base_ld * size_of;
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const int c = col0 + n * 8 + 2 * q;
-            if (a.whole) {  // fp32
-              if (c >= width) continue;
-              const float2 v = a.base ? *reinterpret_cast<const float2*>(from + c * 4) : make_float2(0.0f, 0.0f);
-              *reinterpret_cast<float2*>(to + c * 4) = make_float2(v.x + d[n][2 * h], v.y + d[n][2 * h + 1]);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                if (c + i < width) store_from_float(to, dtype, c + i, d[n][2 * h + i] + (a.base ? load_as_float(from, dtype, c + i) : 0.0f));
-            }
-          }
-        }
-      }
-    }
-    all_but<0>();
-  }
-  if (ctas > 1) lr_cluster_sync();  // the others may still be reading this CTA's partial sums
-}
 // ---- gradients of the factors --------------------------------------------------------------------------
 
 struct FactorGradArgs {
@@ -948,30 +660,27 @@ __global__ void __launch_bounds__(LR_THREADS) factor_grad_kernel(FactorGradArgs 
 static int rank_pad(int64_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : rank <= 64 ? 64 : 128; }
 
 struct LowRankPlan {
-  int rp, rows, ctas;  // rows of a tile: 16, or 64 for the tile kernel
+  int rp, ctas;
   bool solo;
-  int64_t tiles;       // at most
+  int64_t tiles;  // at most
 };
 // One row per tile while there are no more rows than SMs: no plan to wait for, and rows that share a set
-// read it from the cache.  Else tiles of 16 rows, or of 64 where sets have more than 16 on average.
-// Clusters while there are not tiles enough for two CTAs on every SM; sets that few rows name make fewer 64-row
-// tiles than this expects (rows of a prompt have one adapter): four there (4096 rows of rank 64: 57 -> 50 us).
+// read it from the cache (64 rows of four adapters of rank 16: 15 us, grouped 18).  Else tiles of 16 rows; clusters
+// while there are not tiles enough for two CTAs on every SM.
 static LowRankPlan plan_low_rank(int64_t routes, int64_t sets, int64_t rank, bool grads) {
   LowRankPlan p;
   p.rp = rank_pad(rank);
   p.solo = !grads && routes <= 148;
   const int64_t used = routes < sets ? routes : sets;
-  p.rows = p.solo || routes <= 16 * used ? 16 : TILE_ROWS;
-  p.tiles = p.solo ? routes : max_tiles(routes, sets, p.rows);
-  const int64_t expected = p.solo ? routes : routes / p.rows + used / 2 + 1;
+  p.tiles = p.solo ? routes : max_tiles(routes, sets, ROW_STEP);
+  const int64_t expected = p.solo ? routes : routes / ROW_STEP + used / 2 + 1;
   p.ctas = 1;
-  while (p.ctas < 8 && 2 * p.ctas * expected <= (p.rows == TILE_ROWS ? 592 : 296)) p.ctas *= 2;
+  while (p.ctas < 8 && 2 * p.ctas * expected <= 296) p.ctas *= 2;
   return p;
 }
 
 // `configured`: a bit per device, the shared-memory opt-in is a per-device attribute of the function.
-template <typename... Params>
-static int launch_low_rank_kernel(void (*kernel)(Params...), int bytes, uint64_t& configured, int64_t clusters, const LowRankPlan& p, cudaStream_t s, Params... args) {
+static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, uint64_t& configured, const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
   int dev = 0;
   cudaGetDevice(&dev);
   if (dev < 0 || dev >= 64 || !((configured >> dev) & 1ull)) {
@@ -980,7 +689,7 @@ static int launch_low_rank_kernel(void (*kernel)(Params...), int bytes, uint64_t
     if (dev >= 0 && dev < 64) configured |= 1ull << dev;
   }
   cudaLaunchConfig_t config = {};
-  config.gridDim = dim3(static_cast<unsigned>(clusters * p.ctas));
+  config.gridDim = dim3(static_cast<unsigned>(p.tiles * p.ctas));
   config.blockDim = dim3(LR_THREADS);
   config.dynamicSmemBytes = bytes;
   config.stream = s;
@@ -995,14 +704,13 @@ static int launch_low_rank_kernel(void (*kernel)(Params...), int bytes, uint64_t
   }
   config.attrs = &attribute;
   config.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, args...);
+  const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
   return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
 }
 template <typename T, int RP, bool BACK>
 static int launch_low_rank(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
-  static uint64_t configured[2] = {0, 0};
-  if (p.rows == TILE_ROWS) return launch_low_rank_kernel(low_rank_tile_kernel<T, RP, BACK>, TileShape<RP>::BYTES, configured[0], p.tiles, p, s, a);
-  return launch_low_rank_kernel(low_rank_kernel<T, RP, BACK>, LowRankShape<RP, BACK>::BYTES, configured[1], p.tiles, p, s, a);
+  static uint64_t configured = 0;
+  return launch_low_rank_kernel(low_rank_kernel<T, RP, BACK>, LowRankShape<RP, BACK>::BYTES, configured, a, p, s);
 }
 template <typename T, bool BACK>
 static int launch_low_rank_of(const LowRankArgs& a, const LowRankPlan& p, cudaStream_t s) {
@@ -1051,7 +759,7 @@ static LowRankLayout lay_out_low_rank(void* base, int64_t routes, int64_t sets, 
   const int64_t blocks = max_places(routes, sets) / ROW_STEP + 1, values = grads ? blocks * ROW_STEP * p.rp : 0;
   LowRankLayout l = {};
   if (p.solo) return l;  // (nothing to keep: 0 bytes)
-  l.plan = take_plan(s, routes, sets, p.rows);
+  l.plan = take_plan(s, routes, sets, ROW_STEP);
   for (Inner* i : {&l.inner, &l.back}) {
     i->high = s.take<uint16_t>(values);
     i->low = s.take<uint16_t>(values);
@@ -1106,7 +814,7 @@ int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream
   k.indices = {a.indices, a.index_bits};
   k.plan = l.plan;
   if (!p.solo)
-    if (const int rc = make_plan(k.indices, a.routes, a.sets, p.rows, ROW_STEP, l.plan, s)) return rc;
+    if (const int rc = make_plan(k.indices, a.routes, a.sets, ROW_STEP, ROW_STEP, l.plan, s)) return rc;
   k.in = static_cast<const uint16_t*>(a.x);
   k.in_ld = k.depth = a.in_dim;
   k.in_div = a.x_div;
@@ -1150,7 +858,7 @@ int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* 
   LowRankArgs k = {};
   k.indices = {a.indices, a.index_bits};
   k.plan = l.plan;
-  if (const int rc = make_plan(k.indices, a.routes, a.sets, p.rows, ROW_STEP, l.plan, s)) return rc;
+  if (const int rc = make_plan(k.indices, a.routes, a.sets, ROW_STEP, ROW_STEP, l.plan, s)) return rc;
   k.rank = static_cast<int>(a.rank);
   k.sets = static_cast<int>(a.sets);
   k.routes = static_cast<int>(a.routes);
