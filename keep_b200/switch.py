@@ -22,7 +22,7 @@ from typing import Callable
 import torch
 
 from . import _lib
-from .dense_switch import switch_matmul
+from .dense_switch import _indices, switch_matmul
 from .kernels import e8p_m1_per_route, e8p_m1_token_layout, should_use_e8p_m1
 from .low_rank import LowRank
 from .vq import table_on
@@ -173,11 +173,13 @@ class HighPrecisionSwitchLinear:
 
     def __call__(self, x: torch.Tensor, indices: torch.Tensor, *, sorted_indices: bool = False) -> torch.Tensor:
         del sorted_indices  # routes may come in any order
+        indices = _indices(indices, x.device)
         y = switch_matmul(x, self.weight, indices)
         if self.low_rank is not None:
             y = self.low_rank.add(y, x, indices)
-        if self.bias is not None:
-            y = y + self.bias[indices.long().clamp(min=0)].to(y.dtype)
+        if self.bias is not None:  # (a dead route stays zeros, whatever number it holds)
+            dead = (indices < 0) | (indices >= self.num_experts)
+            y = y + self.bias[indices.clamp(0, self.num_experts - 1).long()].to(y.dtype).masked_fill(dead[..., None], 0)
         return y
 
 

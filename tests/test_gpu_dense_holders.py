@@ -48,6 +48,20 @@ def test_high_precision_switch_linear(cuda, tokens):
     near(got, want)
 
 
+@pytest.mark.parametrize("dtype", [torch.int32, torch.int64, torch.uint32])
+def test_dead_routes_get_no_bias(cuda, dtype):
+    """Numbers below and beyond the experts: zeros, not another expert's bias, and no read outside of it."""
+    gen = torch.Generator(device=cuda).manual_seed(2)
+    weight, bias, x = rand(gen, 6, 72, 256, scale=1 / 16), rand(gen, 6, 72).requires_grad_(True), rand(gen, 4, 256)
+    indices = torch.tensor([[0, -1], [5, 6], [-7, 2], [1 << 30, -1]], device=cuda)
+    out = dense_linear(weight, bias=bias)(x, indices.to(torch.int32).view(dtype) if dtype == torch.uint32 else indices.to(dtype))
+    dead = (indices < 0) | (indices > 5)
+    assert out[dead].eq(0).all()
+    near(out[~dead], (ref.matmul(x, weight, indices)[0] + bias.double()[indices.clamp(0, 5)])[~dead], rounds=2)
+    out.sum().backward()  # sums of ones: exact
+    assert torch.equal(bias.grad[:, 0].float(), torch.tensor([1.0, 0, 1, 0, 0, 1], device=cuda))
+
+
 def test_glu_of_mixed_projections(cuda):
     """Gate and up in E8P codes, down in 16 bits, against the same products one by one."""
     from keep_b200 import vq
