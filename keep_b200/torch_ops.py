@@ -267,10 +267,12 @@ def _(grad, x, weight, indices, x_grad, weight_grad):
 
 
 def _matmul_context(ctx, inputs, output):
+    dense_switch._no_capture("switch_matmul", "switch_matmul_grads")
     ctx.save_for_backward(*inputs)
 
 
 def _matmul_backward(ctx, grad):
+    dense_switch._no_capture("switch_matmul", "switch_matmul_grads")
     x, weight, indices = ctx.saved_tensors
     of_x, of_weight = ctx.needs_input_grad[:2]
     dx, dweight = torch.ops.keepvq.switch_matmul_grads(grad, x, weight, indices, of_x, of_weight)
@@ -302,11 +304,13 @@ def _(grad, x, left, right, indices, scale, x_grad, weight_grad):
 
 
 def _low_rank_context(ctx, inputs, output):
+    dense_switch._no_capture("switch_low_rank", "switch_low_rank_grads")
     x, left, right, indices, _, ctx.scale = inputs
     ctx.save_for_backward(x, left, right, indices)
 
 
 def _low_rank_backward(ctx, grad):
+    dense_switch._no_capture("switch_low_rank", "switch_low_rank_grads")
     x, left, right, indices = ctx.saved_tensors
     of_x, of_left, of_right, _, of_base, _ = ctx.needs_input_grad
     dx = dleft = dright = None

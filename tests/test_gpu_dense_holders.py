@@ -147,3 +147,21 @@ def test_custom_ops(cuda):
     dense, thin = switch_matmul_grads(grad, x, weight, indices), switch_low_rank_grads(grad, x, low.left, low.right, indices, scale=0.5)
     assert torch.equal(leaves[1].grad, dense[1]) and torch.equal(leaves[2].grad, thin[1]) and torch.equal(leaves[3].grad, thin[2])
     near(leaves[0].grad, dense[0].double() + thin[0].double(), rounds=1)
+
+
+def test_custom_ops_refuse_recorded_captures(cuda):
+    from keep_b200 import _lib, torch_ops  # noqa: F401
+
+    gen, ops = torch.Generator(device=cuda).manual_seed(5), torch.ops.keepvq
+    x, weight, low, indices = rand(gen, 12, 64), rand(gen, 4, 48, 64), pair(gen, 4, 48, 64, 8), ref.picks(gen, 12, 2, 4)
+    leaf = x.clone().requires_grad_()
+    calls = {"switch_matmul": lambda t: ops.switch_matmul(t, weight, indices), "switch_low_rank": lambda t: ops.switch_low_rank(t, low.left, low.right, indices, None, 0.5)}
+    for name, call in calls.items():
+        want, graph = call(x), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            with pytest.raises(_lib.KeepVQError, match=f"{name}: a recorded gradient cannot be captured"):
+                call(leaf)
+            got = call(x)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
