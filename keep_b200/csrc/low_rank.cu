@@ -126,7 +126,7 @@ struct LowRankArgs {
   const uint16_t* first;   // its factor: right, or left (transposed)
   const uint16_t* second;  // left, or right (transposed); null: no second product
   int64_t depth, width;    // of the first contraction; of the result
-  int rank, sets, routes;
+  int rank, sets;
   float first_scale, second_scale;
   const void* base;        // null: zeros
   int64_t base_ld;
@@ -823,7 +823,6 @@ int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream
   k.width = a.out_dim;
   k.rank = static_cast<int>(a.rank);
   k.sets = static_cast<int>(a.sets);
-  k.routes = static_cast<int>(a.routes);
   k.first_scale = 1.0f;
   k.second_scale = a.scale;
   k.base = a.base;
@@ -861,7 +860,6 @@ int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* 
   if (const int rc = make_plan(k.indices, a.routes, a.sets, ROW_STEP, ROW_STEP, l.plan, s)) return rc;
   k.rank = static_cast<int>(a.rank);
   k.sets = static_cast<int>(a.sets);
-  k.routes = static_cast<int>(a.routes);
   // q = scale B^T grad, and dx = A^T q
   k.in = static_cast<const uint16_t*>(a.grad);
   k.in_ld = a.grad_ld;

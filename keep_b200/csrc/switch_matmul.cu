@@ -148,13 +148,16 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn_major) {
   return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (lead << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// Wait of a whole warp, bounded by time: false when the deadline passes or another warp gave up.
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, uint64_t deadline, volatile int* abort_flag) {
+// Wait of a whole warp, bounded by time: false after MM_WAIT_NS in this wait (a call as a whole may take longer), or when
+// another warp gave up.
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+  uint64_t deadline = 0;
   for (uint32_t spin = 0;; ++spin) {
     if (__all_sync(0xFFFFFFFFu, mbar_complete(bar, parity))) return true;
     if ((spin & 31u) == 31u) {
       if (__any_sync(0xFFFFFFFFu, *abort_flag)) return false;
-      if (__any_sync(0xFFFFFFFFu, global_timer_ns() > deadline)) { *abort_flag = 1; return false; }
+      if (!deadline) deadline = global_timer_ns() + MM_WAIT_NS;
+      else if (__any_sync(0xFFFFFFFFu, global_timer_ns() > deadline)) { *abort_flag = 1; return false; }
     }
   }
 }
@@ -180,7 +183,7 @@ struct Shape {
 
 struct MatmulArgs {
   int x_div, sets, dtype;
-  int64_t routes, out_dim, in_dim;
+  int64_t out_dim, in_dim;
   void* out;        // result rows
   float* route_dx;  // dx before the pick sum, or null
   Plan plan;
@@ -235,7 +238,6 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
   asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
   const uint32_t tmem = tmem_slot;
   if (!MANY) grid_wait();
-  const uint64_t deadline = global_timer_ns() + MM_WAIT_NS;
   volatile int* aborted = &abort_flag;
   // the first CTA's barriers that both CTAs of a pair arrive on
   const uint32_t full0 = MANY ? of_first_cta(full) : full, acc_empty0 = MANY ? of_first_cta(acc_empty) : acc_empty;
@@ -285,7 +287,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
         rows = make_int4(row_at(q), row_at(q + 1), row_at(q + 2), row_at(q + 3));
       }
       for (int kb = 0; kb < it.k_blocks; ++kb) {
-        ok = wait_for(empty + 8 * r.index, r.phase ^ 1u, deadline, aborted);
+        ok = wait_for(empty + 8 * r.index, r.phase ^ 1u, aborted);
         if (!ok) break;
         const uint32_t bar = full0 + 8 * r.index, dst = tile + r.index * S::STAGE_BYTES;
         if (!MANY && warp == WARP_N) {
@@ -322,10 +324,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks == 0) continue;  // (an expert without routes: the epilogue writes zeros)
-      ok = wait_for(acc_empty + 8 * acc.index, acc.phase ^ 1u, deadline, aborted);
+      ok = wait_for(acc_empty + 8 * acc.index, acc.phase ^ 1u, aborted);
       const uint32_t idesc = idesc0 | (static_cast<uint32_t>(it.n_pad >> 3) << 17);
       for (int kb = 0; kb < it.k_blocks && ok; ++kb) {
-        ok = wait_for(full + 8 * r.index, r.phase, deadline, aborted);
+        ok = wait_for(full + 8 * r.index, r.phase, aborted);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int steps = MODE == WEIGHT_GRAD ? min(4, (it.size - kb * K_BLOCK + ROW_STEP - 1) / ROW_STEP) : 4;  // of 16
@@ -367,7 +369,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks > 0) {
-        ok = wait_for(acc_full + 8 * acc.index, acc.phase, deadline, aborted);
+        ok = wait_for(acc_full + 8 * acc.index, acc.phase, aborted);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
@@ -534,7 +536,7 @@ static int check_sizes(int64_t routes, int64_t experts, int64_t out_dim, int64_t
 template <int MODE, bool MANY>
 static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cudaStream_t s) {
   using S = Shape<MANY>;
-  MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.routes, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan};
+  MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan};
   const int64_t places = max_places(a.routes, a.experts), grad_ld = MANY ? align_up(a.out_dim, 8) : a.grad_ld;
   CUtensorMap m_map, n_map, out_map;
   int rc = MODE == WEIGHT_GRAD ? value_map(&m_map, l.x, a.dtype, a.in_dim, a.in_dim, places, 1, K_BLOCK)
