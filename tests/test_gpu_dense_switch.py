@@ -266,3 +266,27 @@ def test_weights_beyond_32_bit_offsets(cuda):
     ref.close(dx, want_x)
     ref.close(dw[[0, experts - 1]], want_w)
     assert not dw[1:experts - 1].any()
+
+
+def test_rows_beyond_32_bit_offsets(cuda):
+    """2.2e9 values in the result and its gradient, 1.1e9 in x and the copies of rows; a few rows at both ends that are not zero."""
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads
+
+    tokens, out, inp = 135_000, 8192, 4096
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    rand = lambda *shape: torch.randn(shape, generator=gen, device=cuda).to(BF16)  # noqa: E731
+    ends = torch.cat([torch.arange(9, device=cuda), torch.arange(tokens - 9, tokens, device=cuda)])
+    x, grad = torch.zeros((tokens, inp), dtype=BF16, device=cuda), torch.zeros((tokens, 2, out), dtype=BF16, device=cuda)
+    x[ends], grad[ends] = rand(18, inp), rand(18, 2, out)
+    weight = rand(4, out, inp) / 64
+    first = torch.arange(tokens, device=cuda, dtype=torch.int32) % 4
+    indices = torch.stack([first, 3 - first], dim=1)
+    got = switch_matmul(x, weight, indices)
+    ref.close(got[ends], ref.matmul(x[ends], weight, indices[ends]))
+    assert not got[9:tokens - 9].any()
+    del got
+    want = ref.matmul_grads(grad[ends], x[ends], weight, indices[ends])
+    dx, dweight = switch_matmul_grads(grad, x, weight, indices)
+    ref.close(dx[ends], want[0])
+    assert not dx[9:tokens - 9].any()
+    ref.close(dweight, want[1])

@@ -263,3 +263,31 @@ def test_an_adapter_on_an_expert_projection_as_a_routed_layer_uses_them(cuda):
     ref.close(leaves[3].grad, low[2])
     both = dense[0][0] + low[0][0]
     ref.close(leaves[0].grad, (both, dense[0][1] + low[0][1] + ref.rounding(both, BF16) + 2.0 ** -8 * (dense[0][1] + low[0][1])))
+
+
+def test_rows_beyond_32_bit_offsets(cuda):
+    """2.2e9 values in x, base, grad and the results; a few rows at both ends that are not zero."""
+    from keep_b200.low_rank import switch_low_rank, switch_low_rank_grads
+
+    tokens, width, rank = 270_000, 8192, 16
+    gen = torch.Generator(device=cuda).manual_seed(3)
+    ends = torch.cat([torch.arange(9, device=cuda), torch.arange(tokens - 9, tokens, device=cuda)])
+    def rows():
+        t = torch.zeros((tokens, width), dtype=BF16, device=cuda)
+        t[ends] = torch.randn((18, width), generator=gen, device=cuda).to(BF16)
+        return t
+    left, right = (torch.randn((3, *shape), generator=gen, device=cuda).div(width ** 0.5).to(BF16) for shape in ((width, rank), (rank, width)))
+    x, base = rows(), rows()
+    indices = torch.arange(tokens, device=cuda, dtype=torch.int32) % 3
+    want = ref.low_rank(x[ends], left, right, indices[ends], base[ends], 0.5)
+    got = switch_low_rank(x, left, right, indices, base=base, scale=0.5)
+    ref.close(got[ends], want)
+    assert not got[9:tokens - 9].any()
+    del got, base
+    grad = rows()
+    want = ref.low_rank_grads(grad[ends], x[ends], left, right, indices[ends], 0.5)
+    dx, dleft, dright = switch_low_rank_grads(grad, x, left, right, indices, scale=0.5)
+    ref.close(dx[ends], want[0])
+    assert not dx[9:tokens - 9].any()
+    ref.close(dleft, want[1])
+    ref.close(dright, want[2])
