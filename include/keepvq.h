@@ -463,8 +463,8 @@ int keepvq_grouped_projection_bytes_served(int64_t routes, int64_t slots, int64_
  * An index outside [0, experts) is a dead route: its output row is zero and it adds nothing to a
  * gradient; experts without routes get zero gradients.  All sums are held in fp32 and rounded once;
  * an expert's routes are added up in their order, so a call gives the same bits every time.  The first
- * int32 of the workspace is 1 after a call one of whose bounded waits expired (2 s, on a device that has
- * stopped making progress): its outputs are then invalid.  Rows
+ * int32 of the workspace is 1 after a call one of whose bounded waits expired (2 s in one wait, on a device that
+ * has stopped making progress): its outputs are then invalid.  Rows
  * are dense, in_dim is a multiple of 8, pointers are aligned to 16 bytes; a row of `grad` is
  * grad_ld >= out_dim values long, a multiple of 8, and those behind out_dim are zero.
  * ------------------------------------------------------------------------------------------ */

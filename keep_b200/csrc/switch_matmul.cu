@@ -431,26 +431,26 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
             __syncwarp();
             if (lane == 0 && col < cols) tma_store_3d(&out_map, col, it.n0 + c0, it.set, piece + flip);
             flip ^= 32 * 64;
-            continue;
-          }
+          } else {
 #pragma unroll
-          for (int u = 0; u < 4; ++u) store_transposed(st_row + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);
-          __syncwarp();
+            for (int u = 0; u < 4; ++u) store_transposed(st_row + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);
+            __syncwarp();
 #pragma unroll
-          for (int u = 0; u < 4; ++u) {
-            uint32_t w[4];
-            asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(ld_row + u * 512) : "memory");
-            uint16_t* dst = static_cast<uint16_t*>(a.out) + to[u] * cols + c;
-            if (to[u] < 0) continue;
-            if (whole) {
-              if (c < cols) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-            } else {
+            for (int u = 0; u < 4; ++u) {
+              uint32_t w[4];
+              asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(ld_row + u * 512) : "memory");
+              uint16_t* dst = static_cast<uint16_t*>(a.out) + to[u] * cols + c;
+              if (to[u] < 0) continue;
+              if (whole) {
+                if (c < cols) *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+              } else {
 #pragma unroll
-              for (int d = 0; d < 8; ++d)
-                if (c + d < cols) dst[d] = static_cast<uint16_t>(w[d >> 1] >> (16 * (d & 1)));
+                for (int d = 0; d < 8; ++d)
+                  if (c + d < cols) dst[d] = static_cast<uint16_t>(w[d >> 1] >> (16 * (d & 1)));
+              }
             }
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
       if (it.k_blocks > 0) {
