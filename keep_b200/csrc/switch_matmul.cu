@@ -423,14 +423,18 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
           }
           if (c0 + TURN < it.n) load(c0 + TURN);
           if (MODE == WEIGHT_GRAD) {
-            if (lane == 0) tma_stores_read<1>();
-            __syncwarp();
+            // a piece is written, and the turn passed on, only with a store of its own: "all but the last store have read"
+            // then always means the store from this piece, also where a tile's columns end in front of this warp's
+            if (col < cols) {
+              if (lane == 0) tma_stores_read<1>();
+              __syncwarp();
 #pragma unroll
-            for (int u = 0; u < 4; ++u) store_transposed(st_row + flip + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0 && col < cols) tma_store_3d(&out_map, col, it.n0 + c0, it.set, piece + flip);
-            flip ^= 32 * 64;
+              for (int u = 0; u < 4; ++u) store_transposed(st_row + flip + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);
+              asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+              __syncwarp();
+              if (lane == 0) tma_store_3d(&out_map, col, it.n0 + c0, it.set, piece + flip);
+              flip ^= 32 * 64;
+            }
           } else {
 #pragma unroll
             for (int u = 0; u < 4; ++u) store_transposed(st_row + u * 512, pair[u][0], pair[u][1], pair[u][2], pair[u][3]);

@@ -290,3 +290,17 @@ def test_rows_beyond_32_bit_offsets(cuda):
     ref.close(dx[ends], want[0])
     assert not dx[9:tokens - 9].any()
     ref.close(dweight, want[1])
+
+
+@pytest.mark.parametrize("inp,out,experts", [(520, 300, 40), (1416, 520, 32)])
+def test_weight_gradients_whose_last_columns_fill_no_tile(cuda, inp, out, experts):
+    """Blocks take several tiles each, now inside the matrix, now across or behind its last columns, and experts without routes
+    between them (whose zeros wait for nothing): no tile's values may end up in another's place.  Calls enqueued one after the other."""
+    from keep_b200.dense_switch import switch_matmul_grads
+
+    for used, tokens in ((experts, 300), (experts // 3, 90)):
+        x, weight, _, grad = make(cuda, tokens, 2, experts, inp, out, seed=inp)
+        indices = 3 * ref.picks(torch.Generator(device=cuda).manual_seed(4), tokens, 2, used) if used < experts else ref.picks(torch.Generator(device=cuda).manual_seed(4), tokens, 2, used)
+        want = ref.matmul_grads(grad, x, weight, indices)[1]
+        for got in [switch_matmul_grads(grad, x, weight, indices, x_grad=False)[1] for _ in range(20)]:
+            ref.close(got, want)
