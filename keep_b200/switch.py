@@ -40,11 +40,21 @@ def _check_low_rank(low_rank: LowRank | None, num_experts: int, output_dims: int
             raise ValueError(f"low_rank must correct (experts, out, in) = {(num_experts, output_dims, input_dims)}, found {found}")
 
 
+def _refuse_gradient(x: torch.Tensor) -> None:
+    """The product over codes has no gradient formula.  By itself its result requires no gradient, and a backward pass fails;
+    beside an operator that records one, x would silently be left with that operator's part."""
+    if x.requires_grad and torch.is_grad_enabled():
+        raise _lib.KeepVQError("QuantizedVQSwitchLinear: the product over codes has no gradient, so its input cannot require one beside operators that "
+                               "record theirs (low_rank, 16-bit projections); detach it, or call under torch.no_grad()")
+
+
 class QuantizedVQSwitchLinear:
     """Switch-linear layer backed by stacked E8 VQ expert tensors.
 
     ``x [..., in]`` with ``indices [..., k]`` (token layout) gives ``[..., k, out]``; ``x [..., k, in]``
-    with ``indices [..., k]`` (one row per route) gives the same shape.
+    with ``indices [..., k]`` (one row per route) gives the same shape.  With ``low_rank`` the factors are
+    recorded by autograd where they require a gradient; an ``x`` that requires one is refused, for the
+    product over codes has none.
     """
 
     def __init__(self, *, input_dims: int, output_dims: int, num_experts: int, codes: torch.Tensor, scales: torch.Tensor,
@@ -109,6 +119,8 @@ class QuantizedVQSwitchLinear:
         return self.scales.float() * torch.exp(self.continuous_scale_delta)
 
     def __call__(self, x: torch.Tensor, indices: torch.Tensor, *, sorted_indices: bool = False) -> torch.Tensor:
+        if self.low_rank is not None:
+            _refuse_gradient(x)
         scales = self.effective_scales()
         common = dict(input_dims=self.input_dims, output_dims=self.output_dims, group_size=self.group_size, code_bits=self.code_bits)
         token_layout = x.ndim >= 2 and indices.ndim >= 2 and tuple(x.shape[:-1]) == tuple(indices.shape[:-1])

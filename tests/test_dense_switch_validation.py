@@ -133,3 +133,28 @@ def test_the_sixteen_bit_holder_refuses():
             HighPrecisionSwitchLinear(**{**ok, **change})
     with pytest.raises(_lib.KeepVQError, match="no CPU path"):
         HighPrecisionSwitchLinear(**ok)
+
+
+def holder_of_codes(monkeypatch, out=16, low_rank=None):
+    """A quantised holder of CPU tensors: enough for what is refused in front of any product."""
+    from keep_b200.switch import QuantizedVQSwitchLinear
+
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "require_cuda", lambda *tensors: torch.device("cpu"))
+        return QuantizedVQSwitchLinear(input_dims=16, output_dims=out, num_experts=3, codes=torch.zeros((3, out, 2), dtype=torch.uint16), scales=rows(3, out, 1),
+                                       codebook=torch.zeros(256, dtype=torch.int32), group_size=16, code_bits=16, low_rank=low_rank)
+
+
+def test_a_corrected_holder_of_codes_refuses_an_input_that_requires_a_gradient(monkeypatch):
+    """The product over codes records nothing: the input would be left with the correction's part of its gradient."""
+    factors = LowRank(rows(3, 16, 4).requires_grad_(), rows(3, 4, 16).requires_grad_())
+    layer, indices = holder_of_codes(monkeypatch, low_rank=factors), torch.zeros(4, 2, dtype=torch.int32)
+    for x in (rows(4, 16), rows(4, 2, 16)):
+        with pytest.raises(_lib.KeepVQError, match="has no gradient"):
+            layer(x.requires_grad_(), indices)
+        with pytest.raises(_lib.KeepVQError, match="no CPU path"):  # as far as CPU tensors come: the factors may require one
+            layer(x.detach(), indices)
+        with torch.no_grad(), pytest.raises(_lib.KeepVQError, match="no CPU path"):
+            layer(x, indices)
+    with pytest.raises(_lib.KeepVQError, match="no CPU path"):  # without a correction nothing records, and backward() says so
+        holder_of_codes(monkeypatch)(rows(4, 16).requires_grad_(), indices)

@@ -165,3 +165,24 @@ def test_custom_ops_refuse_recorded_captures(cuda):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+def test_gradients_of_a_correction_on_a_holder_of_codes(cuda):
+    """The factors' gradients are those of the correction alone (the base is frozen); an input that requires one is refused."""
+    from keep_b200 import _lib
+    from keep_b200.low_rank import LowRank, switch_low_rank_grads
+    from keep_b200.switch import QuantizedVQSwitchLinear
+
+    gen, rng = torch.Generator(device=cuda).manual_seed(6), np.random.default_rng(6)
+    codes, scales = (torch.from_numpy(t).to(cuda) for t in synthetic.projection(rng, 6, 48, 256))
+    low = pair(gen, 6, 48, 256)
+    leaves = [t.clone().requires_grad_() for t in (low.left, low.right)]
+    layer = QuantizedVQSwitchLinear(input_dims=256, output_dims=48, num_experts=6, codes=codes, scales=scales, group_size=256, code_bits=16, low_rank=LowRank(*leaves, low.scale))
+    x, indices, grad = rand(gen, 7, 256), ref.picks(gen, 7, 3, 6), rand(gen, 7, 3, 48)
+    layer(x, indices).backward(grad)
+    want = switch_low_rank_grads(grad, x, low.left, low.right, indices, scale=low.scale, x_grad=False)
+    assert torch.equal(leaves[0].grad, want[1]) and torch.equal(leaves[1].grad, want[2])
+    with pytest.raises(_lib.KeepVQError, match="has no gradient"):
+        layer(x.requires_grad_(), indices)
+    with torch.no_grad():
+        assert torch.equal(layer(x, indices), layer(x.detach(), indices))
