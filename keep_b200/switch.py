@@ -214,7 +214,8 @@ class QuantizedVQSwitchGLU:
     With 16-bit E8P codes, no bias, sidecars or low-rank corrections and plain or limited SwiGLU, a call
     runs the fused layer kernels (activation quantisation, gate + up + SwiGLU in one launch, down in
     another); any other configuration (a projection in 16 bits among them) composes the three
-    projections as the reference does.
+    projections as the reference does.  Where some of the three record gradients (16-bit weights, low-rank
+    corrections) and a projection over codes would have to pass one on, the call is refused.
     """
 
     def __init__(self, *, gate_proj: QuantizedVQSwitchLinear, up_proj: QuantizedVQSwitchLinear, down_proj: QuantizedVQSwitchLinear,
@@ -279,6 +280,15 @@ class QuantizedVQSwitchGLU:
             picks = indices.to(torch.int64)
             dead = (picks < 0) | (picks >= self.gate_proj.num_experts)  # rows the kernels never write
             return out.masked_fill_(dead[..., None], 0)
+        projs = (self.gate_proj, self.up_proj, self.down_proj)
+        records = any(isinstance(p, HighPrecisionSwitchLinear) or getattr(p, "low_rank", None) is not None for p in projs)
+
+        def frozen(rows: torch.Tensor, *through) -> torch.Tensor:
+            if records and any(isinstance(p, QuantizedVQSwitchLinear) for p in through):
+                _refuse_gradient(rows)
+            return rows
+
+        x = frozen(x, self.gate_proj, self.up_proj)
         gate = self.gate_proj(x, indices)
         up = self.up_proj(x, indices)
-        return self.down_proj(self._apply_activation(up, gate), indices)
+        return self.down_proj(frozen(self._apply_activation(up, gate), self.down_proj), indices)

@@ -158,3 +158,41 @@ def test_a_corrected_holder_of_codes_refuses_an_input_that_requires_a_gradient(m
             layer(x, indices)
     with pytest.raises(_lib.KeepVQError, match="no CPU path"):  # without a correction nothing records, and backward() says so
         holder_of_codes(monkeypatch)(rows(4, 16).requires_grad_(), indices)
+
+
+def test_a_mixed_glu_refuses_where_a_gradient_would_have_to_pass_codes(monkeypatch):
+    """Codes beside a 16-bit projection, or beside a correction: x would get a part of its gradient, or the projections in
+    front of the codes none at all."""
+    from keep_b200.switch import HighPrecisionSwitchLinear, QuantizedVQSwitchGLU
+
+    indices, factors = torch.zeros(4, 2, dtype=torch.int32), LowRank(rows(3, 16, 4), rows(3, 4, 16))
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "require_cuda", lambda *tensors: torch.device("cpu"))
+        dense = HighPrecisionSwitchLinear(input_dims=16, output_dims=16, num_experts=3, weight=rows(3, 16, 16))
+    codes, corrected = holder_of_codes(monkeypatch), holder_of_codes(monkeypatch, low_rank=factors)
+    glu = lambda gate, up, down: QuantizedVQSwitchGLU(gate_proj=gate, up_proj=up, down_proj=down)  # noqa: E731
+    for trio in ((dense, codes, dense), (codes, dense, codes), (codes, codes, dense), (codes, corrected, codes), (codes, codes, corrected)):
+        with pytest.raises(_lib.KeepVQError, match="has no gradient"):
+            glu(*trio)(rows(4, 16).requires_grad_(), indices)
+        with pytest.raises(_lib.KeepVQError, match="no CPU path"):
+            glu(*trio)(rows(4, 16), indices)
+    with pytest.raises(_lib.KeepVQError, match="no CPU path"):  # everything recorded
+        glu(dense, dense, dense)(rows(4, 16).requires_grad_(), indices)
+
+
+def test_a_hidden_row_that_requires_a_gradient_does_not_enter_codes(monkeypatch):
+    from keep_b200.switch import HighPrecisionSwitchLinear, QuantizedVQSwitchGLU
+
+    class Recorded(HighPrecisionSwitchLinear):
+        def __init__(self):
+            self.input_dims = self.output_dims = 16
+            self.num_experts = 3
+
+        def __call__(self, x, indices):
+            return rows(4, 2, 16).requires_grad_()
+
+    layer = QuantizedVQSwitchGLU(gate_proj=Recorded(), up_proj=Recorded(), down_proj=holder_of_codes(monkeypatch))
+    with pytest.raises(_lib.KeepVQError, match="has no gradient"):
+        layer(rows(4, 16), torch.zeros(4, 2, dtype=torch.int32))
+    with torch.no_grad(), pytest.raises(_lib.KeepVQError, match="no CPU path"):
+        layer(rows(4, 16), torch.zeros(4, 2, dtype=torch.int32))
