@@ -244,25 +244,27 @@ class QuantizedVQSwitchGLU:
     def _fused_layer(self, top_k: int):
         """The three projections as one ``RoutedMoELayer`` with ``top_k`` picks per token (its
         router unused), or None when the configuration does not fit the layer kernels."""
-        if top_k not in self._fused:
+        projs = (self.gate_proj, self.up_proj, self.down_proj)
+        plain = all(isinstance(p, QuantizedVQSwitchLinear) and p.code_bits == 16 and p.bias is None and p.low_rank is None
+                    and not p.has_continuous_sidecar and p.use_gather_vqmm for p in projs)
+        if not plain or not (self.activation is None or hasattr(self.activation, "limit")):
+            return None
+        # a layer holds the tensors that it was made of: it stays while the projections hold the same ones
+        held = (self.activation, *(t for p in projs for t in (p.codes, p.scales, p.codebook)))
+        parts, layer = self._fused.get(top_k, ((), None))
+        if len(parts) != len(held) or any(a is not b for a, b in zip(parts, held)):
             from .moe import Projection, RoutedMoELayer
 
-            projs = (self.gate_proj, self.up_proj, self.down_proj)
-            plain = all(isinstance(p, QuantizedVQSwitchLinear) and p.code_bits == 16 and p.bias is None and p.low_rank is None
-                        and not p.has_continuous_sidecar and p.use_gather_vqmm for p in projs)
-            act_ok = self.activation is None or hasattr(self.activation, "limit")
-            same_book = plain and all(p.codebook is self.gate_proj.codebook or (p.codebook is not None and self.gate_proj.codebook is not None
-                                                                     and torch.equal(p.codebook, self.gate_proj.codebook)) for p in projs)
-            self._fused[top_k] = None
-            if plain and act_ok and same_book:
-                g = self.gate_proj
+            g, layer = self.gate_proj, None
+            if all(p.codebook is g.codebook or (p.codebook is not None and g.codebook is not None and torch.equal(p.codebook, g.codebook)) for p in projs):
                 layer = RoutedMoELayer(torch.zeros((g.num_experts, g.input_dims), dtype=torch.bfloat16, device=g.codes.device),
                                        Projection(g.codes, g.scales), Projection(self.up_proj.codes, self.up_proj.scales),
                                        Projection(self.down_proj.codes, self.down_proj.scales), top_k=top_k, codebook=g.codebook,
                                        swiglu_limit=float(getattr(self.activation, "limit", 0.0)))
-                if layer.kernel_path == "tensor":
-                    self._fused[top_k] = layer
-        return self._fused[top_k]
+                if layer.kernel_path != "tensor":
+                    layer = None
+            self._fused[top_k] = (held, layer)
+        return layer
 
     def __call__(self, x: torch.Tensor, indices: torch.Tensor) -> torch.Tensor:
         fits = x.ndim == 2 and indices.ndim == 2 and x.shape[0] == indices.shape[0] and x.dtype in (torch.bfloat16, torch.float16)

@@ -186,3 +186,33 @@ def test_gradients_of_a_correction_on_a_holder_of_codes(cuda):
         layer(x.requires_grad_(), indices)
     with torch.no_grad():
         assert torch.equal(layer(x, indices), layer(x.detach(), indices))
+
+
+def codes_linear(cuda, rng, experts, out, inp, **kw):
+    from keep_b200.switch import QuantizedVQSwitchLinear
+
+    codes, scales = (torch.from_numpy(t).to(cuda) for t in synthetic.projection(rng, experts, out, inp))
+    return QuantizedVQSwitchLinear(input_dims=inp, output_dims=out, num_experts=experts, codes=codes, scales=scales, group_size=256, code_bits=16, **kw)
+
+
+def test_a_glu_follows_what_its_projections_hold(cuda):
+    """The fused layer is kept from call to call; what is attached, exchanged or taken off between calls counts for the next one."""
+    from keep_b200.switch import QuantizedVQSwitchGLU, limited_swiglu
+
+    gen, rng = torch.Generator(device=cuda).manual_seed(7), np.random.default_rng(7)
+    gate, up, down, other = (codes_linear(cuda, rng, 5, 256, 256) for _ in range(4))
+    x, indices = rand(gen, 40, 256, scale=0.3), ref.picks(gen, 40, 2, 5)
+    glu = QuantizedVQSwitchGLU(gate_proj=gate, up_proj=up, down_proj=down)
+    fresh = lambda: QuantizedVQSwitchGLU(gate_proj=glu.gate_proj, up_proj=glu.up_proj, down_proj=glu.down_proj, activation=glu.activation)(x, indices)  # noqa: E731
+    first = glu(x, indices)
+    assert glu._fused_layer(2) is not None and glu._fused_layer(2) is glu._fused_layer(2)
+    seen = [first]
+    for change in (lambda: setattr(down, "low_rank", pair(gen, 5, 256, 256)), lambda: setattr(down, "low_rank", None), lambda: setattr(up, "bias", rand(gen, 5, 256)),
+                   lambda: setattr(up, "bias", None), lambda: setattr(glu, "up_proj", other), lambda: setattr(other, "scales", other.scales * 2),
+                   lambda: setattr(glu, "activation", limited_swiglu(0.01)), lambda: setattr(glu, "down_proj", dense_linear(rand(gen, 5, 256, 256, scale=1 / 16)))):
+        change()
+        got = glu(x, indices)
+        assert torch.equal(got, fresh())
+        assert not torch.equal(got, seen[-1])
+        seen.append(got)
+    assert torch.equal(seen[2], first) and torch.equal(seen[4], first)
