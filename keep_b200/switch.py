@@ -245,7 +245,7 @@ class QuantizedVQSwitchGLU:
         """The three projections as one ``RoutedMoELayer`` with ``top_k`` picks per token (its
         router unused), or None when the configuration does not fit the layer kernels."""
         projs = (self.gate_proj, self.up_proj, self.down_proj)
-        plain = all(isinstance(p, QuantizedVQSwitchLinear) and p.code_bits == 16 and p.bias is None and p.low_rank is None
+        plain = all(not isinstance(p, HighPrecisionSwitchLinear) and p.code_bits == 16 and p.bias is None and getattr(p, "low_rank", None) is None
                     and not p.has_continuous_sidecar and p.use_gather_vqmm for p in projs)
         if not plain or not (self.activation is None or hasattr(self.activation, "limit")):
             return None

@@ -216,3 +216,18 @@ def test_a_glu_follows_what_its_projections_hold(cuda):
         assert not torch.equal(got, seen[-1])
         seen.append(got)
     assert torch.equal(seen[2], first) and torch.equal(seen[4], first)
+
+
+def test_a_holder_of_its_own_class_runs_the_fused_layer(cuda):
+    """A projection is known by what it holds: one that is no QuantizedVQSwitchLinear and knows nothing of corrections runs as before."""
+    from types import SimpleNamespace
+
+    from keep_b200.switch import QuantizedVQSwitchGLU
+
+    gen, rng = torch.Generator(device=cuda).manual_seed(8), np.random.default_rng(8)
+    trio = [codes_linear(cuda, rng, 5, 256, 256) for _ in range(3)]
+    names = ("input_dims", "output_dims", "num_experts", "code_bits", "bias", "has_continuous_sidecar", "use_gather_vqmm", "codes", "scales", "codebook")
+    own = [SimpleNamespace(**{n: getattr(p, n) for n in names}) for p in trio]
+    x, indices = rand(gen, 40, 256, scale=0.3), ref.picks(gen, 40, 2, 5)
+    make = lambda t: QuantizedVQSwitchGLU(gate_proj=t[0], up_proj=t[1], down_proj=t[2])  # noqa: E731
+    assert torch.equal(make(own)(x, indices), make(trio)(x, indices))
