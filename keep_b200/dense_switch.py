@@ -15,6 +15,7 @@ an order that depends on the call alone: the same call gives the same bits.
 ``switch_matmul`` records a gradient formula where grad mode is on and an input requires one.  A CUDA graph
 captures ``switch_matmul`` under ``torch.no_grad()`` and ``switch_matmul_grads``, not a recorded backward
 pass: autograd would tie the capture to the streams of whatever other graphs of the same leaves are alive.
+There are no derivatives of gradients and no forward-mode ones: arguments that carry a tangent are refused.
 """
 
 from __future__ import annotations
@@ -22,6 +23,7 @@ from __future__ import annotations
 from functools import lru_cache
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .vq import as_device
@@ -75,6 +77,12 @@ def _grad_rows(grad: torch.Tensor, out_shape: tuple, dtype: torch.dtype) -> tupl
 def _no_capture(what: str, grads: str) -> None:
     if torch.cuda.is_current_stream_capturing():
         raise _lib.KeepVQError(f"{what}: a recorded gradient cannot be captured; capture the call under torch.no_grad() and {grads}")
+
+
+def _no_tangents(what: str, *tensors) -> None:
+    """Forward-mode derivatives are not formed: a result without a tangent would read as one that does not depend on its inputs."""
+    if getattr(forward_ad, "_current_level", 0) >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise _lib.KeepVQError(f"{what} has no forward-mode derivative: an argument carries a tangent")
 
 
 @lru_cache(maxsize=1024)
@@ -132,6 +140,7 @@ def switch_matmul_grads(grad: torch.Tensor, x: torch.Tensor, weight: torch.Tenso
     """The gradients of ``x`` and ``weight`` where ``grad`` is that of ``switch_matmul(x, weight, indices)``,
     in their dtype; None for one that is not wanted.  A row's gradient is the fp32 sum over its picks,
     rounded once; experts without routes get zeros."""
+    _no_tangents("switch_matmul_grads", grad, x, weight)
     device, indices, problem = _check(x, weight, indices)
     _lib.require_cuda(x, grad)
     grad, grad_ld = _grad_rows(grad, problem[6], x.dtype)
@@ -162,6 +171,7 @@ class _SwitchMatmul(torch.autograd.Function):
 def switch_matmul(x: torch.Tensor, weight: torch.Tensor, indices) -> torch.Tensor:
     """``x`` [tokens, in] with ``indices`` [tokens, k] -> [tokens, k, out]; ``x`` [..., k, in] with
     ``indices`` [..., k] -> [..., k, out]: every route against the expert it names."""
+    _no_tangents("switch_matmul", x, weight)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad):
         _lib.require_cuda(x, weight)
         _no_capture("switch_matmul", "switch_matmul_grads")

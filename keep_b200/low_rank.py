@@ -5,7 +5,7 @@ projection, or a correction per expert of a routed layer.
 * ``switch_low_rank_grads(grad, x, left, right, indices, scale=)``   the gradients of ``x``, ``left`` and ``right``
   (that of ``base`` is ``grad`` itself)
 
-Layouts, indices and the rules for captures are those of ``dense_switch``; a dead route (a request without an
+Layouts, indices and the rules for captures and derivatives are those of ``dense_switch``; a dead route (a request without an
 adapter) leaves its base as it is.  ``left`` is ``[sets, out, rank]``, ``right`` ``[sets, rank, in]``, both in x's
 dtype (fp16 or bf16), rank 1 to 128: ranks that are not a multiple of 8 are padded on every call, so a caller
 who keeps such adapters pads them once instead.  ``base`` has x's dtype or is fp32, and so has the result;
@@ -22,7 +22,7 @@ from functools import lru_cache
 import torch
 
 from . import _lib
-from .dense_switch import _DTYPES, _dense, _grad_rows, _indices, _no_capture, _x_div
+from .dense_switch import _DTYPES, _dense, _grad_rows, _indices, _no_capture, _no_tangents, _x_div
 from .vq import as_device
 
 __all__ = ["LowRank", "switch_low_rank", "switch_low_rank_grads"]
@@ -134,6 +134,7 @@ def switch_low_rank_grads(grad: torch.Tensor, x: torch.Tensor, left: torch.Tenso
                           x_grad: bool = True, weight_grad: bool = True):
     """The gradients of ``x``, ``left`` and ``right`` where ``grad`` (in x's dtype) is that of
     ``switch_low_rank(x, left, right, indices, base=..., scale=scale)``; None for those not wanted."""
+    _no_tangents("switch_low_rank_grads", grad, x, left, right)
     device, indices, problem = _check(x, left, right, indices)
     _lib.require_cuda(x, grad)
     grad, grad_ld = _grad_rows(grad, problem[7], x.dtype)
@@ -174,6 +175,7 @@ class _SwitchLowRank(torch.autograd.Function):
 def switch_low_rank(x: torch.Tensor, left: torch.Tensor, right: torch.Tensor, indices, *, base: torch.Tensor | None = None, scale: float = 1.0) -> torch.Tensor:
     """``x`` [rows, in] with ``indices`` [rows] -> [rows, out] (an adapter per row), or the routed layouts
     of ``dense_switch.switch_matmul``; ``base`` has the result's shape (zeros when None)."""
+    _no_tangents("switch_low_rank", x, left, right, base)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, left, right, base)):
         _lib.require_cuda(x, left, right, base)
         _no_capture("switch_low_rank", "switch_low_rank_grads")

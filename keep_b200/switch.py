@@ -22,7 +22,7 @@ from typing import Callable
 import torch
 
 from . import _lib
-from .dense_switch import _indices, switch_matmul
+from .dense_switch import _indices, _no_tangents, switch_matmul
 from .kernels import e8p_m1_per_route, e8p_m1_token_layout, should_use_e8p_m1
 from .low_rank import LowRank
 from .vq import table_on
@@ -46,6 +46,7 @@ def _refuse_gradient(x: torch.Tensor) -> None:
     if x.requires_grad and torch.is_grad_enabled():
         raise _lib.KeepVQError("QuantizedVQSwitchLinear: the product over codes has no gradient, so its input cannot require one beside operators that "
                                "record theirs (low_rank, 16-bit projections); detach it, or call under torch.no_grad()")
+    _no_tangents("QuantizedVQSwitchLinear", x)
 
 
 class QuantizedVQSwitchLinear:

@@ -25,7 +25,8 @@ Arguments are tensors and plain scalars only (what a schema can carry): tables a
 explicitly, tuples of the nested operators are flattened, keyword-only arguments keep their names.
 None of the ops mutates an argument; outputs are fresh tensors.  The operators over codes have no autograd
 formula: they are an inference path.  ``switch_matmul`` and ``switch_low_rank`` have one, whose work is done by
-``switch_matmul_grads`` and ``switch_low_rank_grads`` (empty tensors for gradients that are not wanted).
+``switch_matmul_grads`` and ``switch_low_rank_grads`` (empty tensors for gradients that are not wanted); these four
+refuse to be called inside forward-mode differentiation.
 """
 
 from __future__ import annotations
@@ -34,9 +35,10 @@ from typing import Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 from torch.library import custom_op
 
-from . import dense_switch, kernels, low_rank, moe, router, vq_switch
+from . import _lib, dense_switch, kernels, low_rank, moe, router, vq_switch
 
 __all__ = ["OPS"]
 
@@ -242,12 +244,20 @@ def _(x, router_w, w1_codes, w1_scales, w3_codes, w3_scales, w2_codes, w2_scales
 
 # ---- 16-bit experts and low-rank adapters ---------------------------------------------------------------
 
+def _no_forward_mode(what: str) -> None:
+    """An operator of the dispatcher may be handed its arguments without the tangents that they carry (``torch.func.jvp``), so it
+    cannot tell which have one, as the functions behind it can."""
+    if getattr(forward_ad, "_current_level", -1) >= 0:
+        raise _lib.KeepVQError(f"keepvq::{what} has no forward-mode derivative and is not called inside of one")
+
+
 def _wanted(grads, like):
     return tuple(like.new_empty((0,)) if g is None else g for g in grads)
 
 
 @custom_op("keepvq::switch_matmul", mutates_args=(), device_types=_CUDA)
 def switch_matmul(x: Tensor, weight: Tensor, indices: Tensor) -> Tensor:
+    _no_forward_mode("switch_matmul")
     return dense_switch._forward(x, weight, indices)
 
 
@@ -258,6 +268,7 @@ def _(x, weight, indices):
 
 @custom_op("keepvq::switch_matmul_grads", mutates_args=(), device_types=_CUDA)
 def switch_matmul_grads(grad: Tensor, x: Tensor, weight: Tensor, indices: Tensor, x_grad: bool, weight_grad: bool) -> Tuple[Tensor, Tensor]:
+    _no_forward_mode("switch_matmul_grads")
     return _wanted(dense_switch.switch_matmul_grads(grad, x, weight, indices, x_grad=x_grad, weight_grad=weight_grad), x)
 
 
@@ -284,6 +295,7 @@ switch_matmul.register_autograd(_matmul_backward, setup_context=_matmul_context)
 
 @custom_op("keepvq::switch_low_rank", mutates_args=(), device_types=_CUDA)
 def switch_low_rank(x: Tensor, left: Tensor, right: Tensor, indices: Tensor, base: Optional[Tensor], scale: float) -> Tensor:
+    _no_forward_mode("switch_low_rank")
     return low_rank._forward(x, left, right, indices, base, scale)
 
 
@@ -295,6 +307,7 @@ def _(x, left, right, indices, base, scale):
 @custom_op("keepvq::switch_low_rank_grads", mutates_args=(), device_types=_CUDA)
 def switch_low_rank_grads(grad: Tensor, x: Tensor, left: Tensor, right: Tensor, indices: Tensor, scale: float, x_grad: bool,
                           weight_grad: bool) -> Tuple[Tensor, Tensor, Tensor]:
+    _no_forward_mode("switch_low_rank_grads")
     return _wanted(low_rank.switch_low_rank_grads(grad, x, left, right, indices, scale=scale, x_grad=x_grad, weight_grad=weight_grad), x)
 
 

@@ -196,3 +196,44 @@ def test_a_hidden_row_that_requires_a_gradient_does_not_enter_codes(monkeypatch)
         layer(rows(4, 16), torch.zeros(4, 2, dtype=torch.int32))
     with torch.no_grad(), pytest.raises(_lib.KeepVQError, match="no CPU path"):
         layer(rows(4, 16), torch.zeros(4, 2, dtype=torch.int32))
+
+
+def forward_calls():
+    """(name, call over a list of arguments, those arguments) of everything that takes values which may carry tangents."""
+    indices, low = torch.zeros(4, 2, dtype=torch.int32), (rows(3, 8, 4), rows(3, 4, 16))
+    yield "switch_matmul", lambda t: switch_matmul(*t, indices), [rows(4, 16), rows(3, 8, 16)]
+    yield "switch_matmul_grads", lambda t: switch_matmul_grads(*t, indices), [rows(4, 2, 8), rows(4, 16), rows(3, 8, 16)]
+    yield "switch_low_rank", lambda t: switch_low_rank(*t[:3], indices, base=t[3]), [rows(4, 16), *low, rows(4, 2, 8)]
+    yield "switch_low_rank_grads", lambda t: switch_low_rank_grads(*t, indices), [rows(4, 2, 8), rows(4, 16), *low]
+
+
+def test_tangents_are_refused():
+    """A result that came back without one would read as independent of the argument."""
+    from torch.autograd import forward_ad
+
+    for name, call, args in forward_calls():
+        for i in range(len(args)):
+            for leaf in (args[i], args[i].clone().requires_grad_()):
+                with forward_ad.dual_level():
+                    dual = forward_ad.make_dual(leaf, torch.ones_like(args[i]))
+                    for grad_mode in (torch.enable_grad, torch.no_grad):
+                        with grad_mode(), pytest.raises(_lib.KeepVQError, match=f"{name} has no forward-mode derivative"):
+                            call([*args[:i], dual, *args[i + 1:]])
+            with pytest.raises(_lib.KeepVQError, match="no forward-mode derivative"):
+                torch.func.jvp(lambda t: call([*args[:i], t, *args[i + 1:]]), (args[i],), (torch.ones_like(args[i]),))
+        with forward_ad.dual_level(), pytest.raises(_lib.KeepVQError, match="no CPU path"):  # nothing carries one
+            call(args)
+
+
+def test_a_mixed_glu_refuses_tangents_that_would_have_to_pass_codes(monkeypatch):
+    from torch.autograd import forward_ad
+
+    from keep_b200.switch import HighPrecisionSwitchLinear, QuantizedVQSwitchGLU
+
+    with monkeypatch.context() as m:
+        m.setattr(_lib, "require_cuda", lambda *tensors: torch.device("cpu"))
+        dense = HighPrecisionSwitchLinear(input_dims=16, output_dims=16, num_experts=3, weight=rows(3, 16, 16))
+    codes = holder_of_codes(monkeypatch)
+    layer = QuantizedVQSwitchGLU(gate_proj=codes, up_proj=codes, down_proj=dense)
+    with forward_ad.dual_level(), pytest.raises(_lib.KeepVQError, match="QuantizedVQSwitchLinear has no forward-mode derivative"):
+        layer(forward_ad.make_dual(rows(4, 16), rows(4, 16)), torch.zeros(4, 2, dtype=torch.int32))

@@ -231,3 +231,19 @@ def test_a_holder_of_its_own_class_runs_the_fused_layer(cuda):
     x, indices = rand(gen, 40, 256, scale=0.3), ref.picks(gen, 40, 2, 5)
     make = lambda t: QuantizedVQSwitchGLU(gate_proj=t[0], up_proj=t[1], down_proj=t[2])  # noqa: E731
     assert torch.equal(make(own)(x, indices), make(trio)(x, indices))
+
+
+def test_custom_ops_refuse_forward_mode_differentiation(cuda):
+    from keep_b200 import _lib, torch_ops  # noqa: F401
+
+    gen, ops = torch.Generator(device=cuda).manual_seed(9), torch.ops.keepvq
+    x, weight, low, indices, grad = rand(gen, 12, 64), rand(gen, 4, 48, 64), pair(gen, 4, 48, 64, 8), ref.picks(gen, 12, 2, 4), rand(gen, 12, 2, 48)
+    calls = {"switch_matmul": lambda t: ops.switch_matmul(t, weight, indices), "switch_matmul_grads": lambda t: ops.switch_matmul_grads(grad, t, weight, indices, True, True),
+             "switch_low_rank": lambda t: ops.switch_low_rank(t, low.left, low.right, indices, None, 0.5),
+             "switch_low_rank_grads": lambda t: ops.switch_low_rank_grads(grad, t, low.left, low.right, indices, 0.5, True, True)}
+    for name, call in calls.items():
+        with pytest.raises(_lib.KeepVQError, match=f"keepvq::{name} has no forward-mode derivative"):
+            torch.func.jvp(call, (x,), (x,))
+        with torch.autograd.forward_ad.dual_level(), pytest.raises(_lib.KeepVQError, match="no forward-mode derivative"):
+            call(torch.autograd.forward_ad.make_dual(x, x))
+        call(x)
