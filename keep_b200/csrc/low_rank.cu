@@ -66,6 +66,14 @@ __device__ __forceinline__ void split(float x, float y, uint32_t& high, uint32_t
   const float2 h = Mma<T>::unpack(high);
   low = Mma<T>::pack(isinf(h.x) ? 0.0f : x - h.x, isinf(h.y) ? 0.0f : y - h.y);
 }
+// What the low parts add up to, as something that an infinity can be added to: the largest number in the place of an infinity or of
+// no value.  A factor's infinity meets both parts of an inner value; with the low one, zero or of the other sign, it would undo
+// what the high one makes of it.  (The smaller magnitude, of the one that is a number, with v's sign.)
+__device__ __forceinline__ float finite(float v) {
+  float f;
+  asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(f) : "f"(v), "f"(__uint_as_float(0x7F7FFFFFu)));
+  return f;
+}
 // An 8 x 8 matrix of 16-bit values, a row's pairs in four lanes, transposed.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t t;
@@ -442,19 +450,23 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
           }
       }
       const int n = n0 + 8 * q;
-      float d[4][4];
+      float d[4][4], e[4][4];  // of the high parts, and of the low ones
 #pragma unroll
       for (int t = 0; t < 4; ++t) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) d[t][i] = 0.0f;
+        for (int i = 0; i < 4; ++i) d[t][i] = e[t][i] = 0.0f;
       }
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
 #pragma unroll
-        for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], low[c], b[t][c][0], b[t][c][1]);
+        for (int t = 0; t < 4; ++t) Mma<T>::run(e[t], low[c], b[t][c][0], b[t][c][1]);
 #pragma unroll
         for (int t = 0; t < 4; ++t) Mma<T>::run(d[t], high[c], b[t][c][0], b[t][c][1]);
       }
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) d[t][i] += finite(e[t][i]);
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int r = h * 8 + g;

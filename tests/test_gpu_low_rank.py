@@ -291,3 +291,40 @@ def test_rows_beyond_32_bit_offsets(cuda):
     assert not dx[9:tokens - 9].any()
     ref.close(dleft, want[1])
     ref.close(dright, want[2])
+
+
+def same_infinities(got, want_and_bound):
+    """The definition's infinities and undefined values in their places, and everything else as near as ever."""
+    want, bound = want_and_bound
+    finite = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got.double()[torch.isinf(want)], want[torch.isinf(want)])
+    ref.close(got[finite], (want[finite], bound[finite]))
+
+
+def with_infinities(t, step):
+    """An infinity, of either sign in turn, in some of a matrix's rows, at one of their places each."""
+    sets, n, width = t.shape
+    t = t.clone()
+    rows = torch.arange(0, n, step, device=t.device)
+    t[:, rows, rows % width] = torch.where(rows // step % 2 == 0, float("inf"), float("-inf")).to(t.dtype)
+    return t
+
+
+# rows, sets, in, out, rank: a tile per row, and tiles of the plan
+INFINITE = [(24, 2, 128, 72, 8), (24, 3, 264, 136, 40), (300, 2, 136, 200, 16), (180, 4, 136, 72, 100)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,sets,inp,out,rank", INFINITE)
+def test_an_infinity_of_a_factor_is_one_of_the_result(cuda, rows, sets, inp, out, rank, dtype):
+    """A vector that enters the second product in two parts meets it with both: zero, or of the other sign, times infinity is no value."""
+    from keep_b200.low_rank import switch_low_rank, switch_low_rank_grads
+
+    x, left, right, indices, base, grad = make(cuda, rows, 1, sets, inp, out, rank, dtype=dtype, base=dtype, seed=rank)
+    low = with_infinities(left, 5)
+    want = ref.low_rank(x, low, right, indices, base, 0.5)
+    assert torch.isinf(want[0]).any() and not torch.isnan(want[0]).any()
+    same_infinities(switch_low_rank(x, low, right, indices, base=base, scale=0.5), want)
+    high = with_infinities(right.transpose(1, 2), 7).transpose(1, 2)
+    same_infinities(switch_low_rank_grads(grad, x, left, high, indices, weight_grad=False)[0], ref.low_rank_grads(grad, x, left, high, indices, 1.0)[0])
