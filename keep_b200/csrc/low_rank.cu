@@ -357,7 +357,7 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
     float sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < LR_WARPS; ++w) sum += part[w * ROWS * RP + i];
-    own[i] = sum * a.first_scale;
+    own[i] = i % RP < a.rank ? sum * a.first_scale : 0.0f;  // (a row's infinity times the zeros of ranks that are not there is no zero)
   }
   meet<T, RP, ROWS>(own, inner, unit, ctas);
   if (a.keep.high && rank == 0) keep_inner<RP, ROWS>(a, inner, start, size);

@@ -328,3 +328,18 @@ def test_an_infinity_of_a_factor_is_one_of_the_result(cuda, rows, sets, inp, out
     same_infinities(switch_low_rank(x, low, right, indices, base=base, scale=0.5), want)
     high = with_infinities(right.transpose(1, 2), 7).transpose(1, 2)
     same_infinities(switch_low_rank_grads(grad, x, left, high, indices, weight_grad=False)[0], ref.low_rank_grads(grad, x, left, high, indices, 1.0)[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,sets,inp,out,rank", [*INFINITE[:3], (180, 4, 136, 72, 104), (200, 2, 72, 136, 24)])
+def test_an_infinity_of_a_row_is_one_of_its_results(cuda, rows, sets, inp, out, rank, dtype):
+    from keep_b200.low_rank import switch_low_rank, switch_low_rank_grads
+
+    x, left, right, indices, base, grad = make(cuda, rows, 1, sets, inp, out, rank, dtype=dtype, base=dtype, seed=rank + 1)
+    x[::3, 5], grad[1::4, 0, 9] = float("inf"), float("-inf")
+    left[:, ::2], right[:, :, ::2] = left[:, ::2].abs(), right[:, :, ::2].abs()
+    right[:, :, 5], left[:, 9] = right[:, :, 5].abs(), left[:, 9].abs()
+    want = ref.low_rank(x, left, right, indices, base, 0.5)
+    assert torch.isinf(want[0]).any()
+    same_infinities(switch_low_rank(x, left, right, indices, base=base, scale=0.5), want)
+    same_infinities(switch_low_rank_grads(grad, x, left, right, indices, weight_grad=False)[0], ref.low_rank_grads(grad, x, left, right, indices, 1.0)[0])
