@@ -100,10 +100,10 @@ __device__ __forceinline__ uint4 piece16(uint32_t at) {
   return v;
 }
 
-// A power of two not below `most`, within what has a reciprocal; 1 for zero and for what is not finite.
+// A power of two not below `most` (finite), within what has a reciprocal; 1 for zero.
 __device__ __forceinline__ float power_above(float most) {
   const uint32_t e = (__float_as_uint(most) >> 23) & 0xFFu;
-  return most == 0.0f || e == 255u ? 1.0f : __uint_as_float(min(max(e + 1u, 2u), 252u) << 23);
+  return most == 0.0f ? 1.0f : __uint_as_float(min(max(e + 1u, 2u), 252u) << 23);
 }
 
 __device__ __forceinline__ uint32_t lr_cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r)); return r; }
@@ -200,7 +200,10 @@ __device__ __forceinline__ void meet(const float* own, float* inner, float* unit
   if (Mma<T>::SCALED) {
     if (tid < ROWS) {
       float most = 0.0f;
-      for (int j = 0; j < RP; ++j) most = fmaxf(most, fabsf(inner[tid * RP + (j + tid) % RP]));
+      for (int j = 0; j < RP; ++j) {  // of those that are numbers: beside an infinity the others still have to fit
+        const float v = fabsf(inner[tid * RP + (j + tid) % RP]);
+        if (!isinf(v)) most = fmaxf(most, v);
+      }
       unit[tid] = power_above(most);
     }
     __syncthreads();

@@ -343,3 +343,24 @@ def test_an_infinity_of_a_row_is_one_of_its_results(cuda, rows, sets, inp, out, 
     assert torch.isinf(want[0]).any()
     same_infinities(switch_low_rank(x, left, right, indices, base=base, scale=0.5), want)
     same_infinities(switch_low_rank_grads(grad, x, left, right, indices, weight_grad=False)[0], ref.low_rank_grads(grad, x, left, right, indices, 1.0)[0])
+
+
+@pytest.mark.parametrize("rows", [24, 200])
+def test_inner_vectors_beyond_the_range_of_fp16_beside_an_infinity(cuda, rows):
+    """One inner value is infinite, the others are finite but beyond fp16: they do not become infinities of the other sign."""
+    from keep_b200.low_rank import switch_low_rank, switch_low_rank_grads
+
+    x, left, right, indices, _, grad = make(cuda, rows, 1, 2, 256, 72, 16, dtype=FP16)
+    right, x, left = right * 16, 6000 * x.sign(), left * 2.0 ** -14
+    x[:, 3], right[:, 5, 3] = 1, float("inf")
+    inner = x.double() @ right[0].double().T
+    assert (inner.abs() > 65504).sum(1).ge(2).any()
+    want = ref.low_rank(x, left, right, indices, None, 1.0)
+    assert torch.isinf(want[0]).all()
+    same_infinities(switch_low_rank(x, left, right, indices), want)
+    # the same on the way back: q = B^T grad with one infinite entry
+    grad, left = 6000 * grad.sign(), left * 2.0 ** 18
+    grad[:, :, 3], left[:, 3, 5], right = 1, float("inf"), right.nan_to_num(posinf=1.0) * 2.0 ** -18
+    want = ref.low_rank_grads(grad, x, left, right, indices, 1.0)[0]
+    assert torch.isinf(want[0]).any()
+    same_infinities(switch_low_rank_grads(grad, x, left, right, indices, weight_grad=False)[0], want)
