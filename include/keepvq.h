@@ -536,6 +536,10 @@ typedef struct keepvq_switch_low_rank_args {
 int64_t keepvq_switch_low_rank_workspace_bytes(int64_t routes, int64_t sets, int64_t out_dim, int64_t in_dim, int64_t rank, int32_t x_div, int32_t grads);
 int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream);
 int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* stream);
+/* The same with factors of `ranks` ranks (at most args->rank) that are filled up to args->rank by zeros.  What
+ * is filled up then counts for nothing also in a row that is not finite; its own gradients mean nothing. */
+int keepvq_switch_low_rank_padded(const keepvq_switch_low_rank_args* args, int32_t ranks, void* stream);
+int keepvq_switch_low_rank_grads_padded(const keepvq_switch_low_rank_args* args, int32_t ranks, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Expert parallelism: packing routes for the dispatch all-to-all and summing them after the

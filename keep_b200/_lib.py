@@ -200,6 +200,8 @@ _SIGNATURES = {
     "keepvq_switch_low_rank_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_int32]),
     "keepvq_switch_low_rank": (c_int, [POINTER(SwitchLowRankArgs), c_void_p]),
     "keepvq_switch_low_rank_grads": (c_int, [POINTER(SwitchLowRankArgs), c_void_p]),
+    "keepvq_switch_low_rank_padded": (c_int, [POINTER(SwitchLowRankArgs), c_int32, c_void_p]),
+    "keepvq_switch_low_rank_grads_padded": (c_int, [POINTER(SwitchLowRankArgs), c_int32, c_void_p]),
     "keepvq_ep_pack": (c_int, [POINTER(EpPackArgs), c_void_p]),
     "keepvq_ep_combine": (c_int, [POINTER(EpCombineArgs), c_void_p]),
     "keepvq_ep_dispatch_peer": (c_int, [POINTER(EpPackArgs), POINTER(EpPeerArgs), c_void_p]),

@@ -134,7 +134,7 @@ struct LowRankArgs {
   const uint16_t* first;   // its factor: right, or left (transposed)
   const uint16_t* second;  // left, or right (transposed); null: no second product
   int64_t depth, width;    // of the first contraction; of the result
-  int rank, sets;
+  int rank, ranks, sets;   // in memory; of these, those that are no padding
   float first_scale, second_scale;
   const void* base;        // null: zeros
   int64_t base_ld;
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(LR_THREADS, LowRankShape<RP, BACK>::CTAS) low_
     float sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < LR_WARPS; ++w) sum += part[w * ROWS * RP + i];
-    own[i] = i % RP < a.rank ? sum * a.first_scale : 0.0f;  // (a row's infinity times the zeros of ranks that are not there is no zero)
+    own[i] = i % RP < a.ranks ? sum * a.first_scale : 0.0f;  // (a row's infinity times the zeros of ranks that are not there is no zero)
   }
   meet<T, RP, ROWS>(own, inner, unit, ctas);
   if (a.keep.high && rank == 0) keep_inner<RP, ROWS>(a, inner, start, size);
@@ -814,11 +814,12 @@ int64_t keepvq_switch_low_rank_workspace_bytes(int64_t routes, int64_t sets, int
   return lay_out_low_rank(nullptr, routes, sets, in_dim, rank, x_div, grads != 0).bytes;
 }
 
-int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream) {
+int keepvq_switch_low_rank_padded(const keepvq_switch_low_rank_args* args, int32_t ranks, void* stream) {
   using namespace keepvq::dense;
   if (!args) return KEEPVQ_ERR_NULL;
   const keepvq_switch_low_rank_args& a = *args;
   if (const int rc = check_low_rank(a, false)) return rc;
+  if (ranks <= 0 || ranks > a.rank) return KEEPVQ_ERR_SHAPE;
   const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.in_dim, a.rank, a.x_div, false);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   if (l.bytes > 0 && !a.workspace) return KEEPVQ_ERR_NULL;
@@ -837,6 +838,7 @@ int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream
   k.second = static_cast<const uint16_t*>(a.left);
   k.width = a.out_dim;
   k.rank = static_cast<int>(a.rank);
+  k.ranks = ranks;
   k.sets = static_cast<int>(a.sets);
   k.first_scale = 1.0f;
   k.second_scale = a.scale;
@@ -851,11 +853,12 @@ int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream
   return launch_low_rank_any(a.dtype, false, k, p, s);
 }
 
-int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* stream) {
+int keepvq_switch_low_rank_grads_padded(const keepvq_switch_low_rank_args* args, int32_t ranks, void* stream) {
   using namespace keepvq::dense;
   if (!args) return KEEPVQ_ERR_NULL;
   const keepvq_switch_low_rank_args& a = *args;
   if (const int rc = check_low_rank(a, true)) return rc;
+  if (ranks <= 0 || ranks > a.rank) return KEEPVQ_ERR_SHAPE;
   const LowRankLayout l = lay_out_low_rank(a.workspace, a.routes, a.sets, a.in_dim, a.rank, a.x_div, true);
   if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
   if (l.bytes > 0 && !a.workspace) return KEEPVQ_ERR_NULL;
@@ -874,6 +877,7 @@ int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* 
   k.plan = l.plan;
   if (const int rc = make_plan(k.indices, a.routes, a.sets, ROW_STEP, ROW_STEP, l.plan, s)) return rc;
   k.rank = static_cast<int>(a.rank);
+  k.ranks = ranks;
   k.sets = static_cast<int>(a.sets);
   // q = scale B^T grad, and dx = A^T q
   k.in = static_cast<const uint16_t*>(a.grad);
@@ -911,6 +915,14 @@ int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* 
   FactorGradArgs right{static_cast<const uint16_t*>(a.x), a.in_dim, a.x_div, a.dright ? a.in_dim : 0, static_cast<int>(a.rank), row_parts, 1.0f, l.plan, l.back, static_cast<uint16_t*>(a.dright)};
   FactorGradArgs left{static_cast<const uint16_t*>(a.grad), a.grad_ld, 1, a.dleft ? a.out_dim : 0, static_cast<int>(a.rank), row_parts, a.scale, l.plan, l.inner, static_cast<uint16_t*>(a.dleft)};
   return a.dtype == KEEPVQ_BF16 ? launch_factor_grads_of<__nv_bfloat16>(p.rp, right, left, a.sets, s) : launch_factor_grads_of<__half>(p.rp, right, left, a.sets, s);
+}
+
+int keepvq_switch_low_rank(const keepvq_switch_low_rank_args* args, void* stream) {
+  return keepvq_switch_low_rank_padded(args, args ? static_cast<int32_t>(args->rank) : 0, stream);
+}
+
+int keepvq_switch_low_rank_grads(const keepvq_switch_low_rank_args* args, void* stream) {
+  return keepvq_switch_low_rank_grads_padded(args, args ? static_cast<int32_t>(args->rank) : 0, stream);
 }
 
 }  // extern "C"

@@ -61,13 +61,13 @@ def _check_pair(left_shape, right_shape, left_dtype, right_dtype) -> None:
 @lru_cache(maxsize=1024)
 def _problem(x_shape, left_shape, right_shape, indices_shape, x_dtype, left_dtype, right_dtype) -> tuple:
     """What follows from shapes and types alone, checked once for each: (routes per row of x, routes, sets, out, in, rank rounded
-    up, dtype tag, result's shape)."""
+    up, dtype tag, result's shape, rank)."""
     _check_pair(left_shape, right_shape, left_dtype, right_dtype)
     if x_dtype != left_dtype:
         raise ValueError(f"x must be {left_dtype} as left and right, found {x_dtype}")
     sets, out_dim, rank = left_shape
     x_div, routes = _x_div(x_shape, indices_shape, right_shape[2])
-    return max(x_div, 1), routes, sets, out_dim, right_shape[2], -(-rank // 8) * 8, _lib.dtype_tag(x_dtype), (*indices_shape, out_dim)
+    return max(x_div, 1), routes, sets, out_dim, right_shape[2], -(-rank // 8) * 8, _lib.dtype_tag(x_dtype), (*indices_shape, out_dim), rank
 
 
 def _check(x, left, right, indices):
@@ -94,7 +94,7 @@ def _scratch_bytes(routes: int, sets: int, out_dim: int, in_dim: int, rank: int,
 
 
 def _call(name, device, x, left, right, grad, indices, problem, grad_ld, scale, out_tag, base, base_ld, out, dx, dleft, dright):
-    x_div, routes, sets, out_dim, in_dim, rank, tag, _ = problem
+    x_div, routes, sets, out_dim, in_dim, rank, tag, _, ranks = problem
     nbytes = _scratch_bytes(routes, sets, out_dim, in_dim, rank, x_div, grad is not None)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
     args = _lib.pack_switch_low_rank_args(
@@ -102,7 +102,7 @@ def _call(name, device, x, left, right, grad, indices, problem, grad_ld, scale, 
         x_div, routes, sets, out_dim, in_dim, rank, grad_ld, scale, out_tag, 0 if base is None else base.data_ptr(), base_ld, 0 if out is None else out.data_ptr(), out_dim,
         0 if dx is None else dx.data_ptr(), 0 if dleft is None else dleft.data_ptr(), 0 if dright is None else dright.data_ptr(), 0 if ws is None else ws.data_ptr(), nbytes)
     with _lib.on_device(device):
-        _lib.check(getattr(_lib.load(), name)(args, _lib.raw_stream(device)), name)
+        _lib.check(getattr(_lib.load(), name)(args, ranks, _lib.raw_stream(device)), name)
 
 
 def _forward(x, left, right, indices, base, scale) -> torch.Tensor:
@@ -126,7 +126,7 @@ def _forward(x, left, right, indices, base, scale) -> torch.Tensor:
                 base = base.contiguous()
     if problem[1]:
         left, right = _whole_ranks(left, right)
-        _call("keepvq_switch_low_rank", device, _dense(x), left, right, None, indices, problem, 0, scale, out_tag, base, base_ld, out, None, None, None)
+        _call("keepvq_switch_low_rank_padded", device, _dense(x), left, right, None, indices, problem, 0, scale, out_tag, base, base_ld, out, None, None, None)
     return out
 
 
@@ -147,7 +147,7 @@ def switch_low_rank_grads(grad: torch.Tensor, x: torch.Tensor, left: torch.Tenso
             if t is not None:
                 t.zero_()
     elif x_grad or weight_grad:
-        _call("keepvq_switch_low_rank_grads", device, _dense(x), left, right, grad, indices, problem, grad_ld, float(scale), problem[6], None, 0, None, dx, dleft, dright)
+        _call("keepvq_switch_low_rank_grads_padded", device, _dense(x), left, right, grad, indices, problem, grad_ld, float(scale), problem[6], None, 0, None, dx, dleft, dright)
     if weight_grad and int(left.shape[2]) != rank:
         dleft, dright = dleft[:, :, :rank].contiguous(), dright[:, :rank].contiguous()
     return dx, dleft, dright

@@ -237,3 +237,11 @@ def test_a_mixed_glu_refuses_tangents_that_would_have_to_pass_codes(monkeypatch)
     layer = QuantizedVQSwitchGLU(gate_proj=codes, up_proj=codes, down_proj=dense)
     with forward_ad.dual_level(), pytest.raises(_lib.KeepVQError, match="QuantizedVQSwitchLinear has no forward-mode derivative"):
         layer(forward_ad.make_dual(rows(4, 16), rows(4, 16)), torch.zeros(4, 2, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("ranks", [0, -1, 9, 1 << 20])
+def test_ranks_beyond_the_factors_are_refused(ranks):
+    lib = _lib.load()
+    assert lib.keepvq_switch_low_rank_padded(low_rank_args(), ranks, None) == SHAPE
+    assert lib.keepvq_switch_low_rank_grads_padded(low_rank_args(), ranks, None) == SHAPE
+    assert lib.keepvq_switch_low_rank_padded(low_rank_args(routes=0), 5, None) == 0

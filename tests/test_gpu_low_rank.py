@@ -364,3 +364,18 @@ def test_inner_vectors_beyond_the_range_of_fp16_beside_an_infinity(cuda, rows):
     want = ref.low_rank_grads(grad, x, left, right, indices, 1.0)[0]
     assert torch.isinf(want[0]).any()
     same_infinities(switch_low_rank_grads(grad, x, left, right, indices, weight_grad=False)[0], want)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,rank", [(24, 1), (24, 5), (180, 12), (180, 100)])
+def test_ranks_that_fill_up_a_multiple_of_eight_stay_out_of_rows_that_are_not_finite(cuda, rows, rank, dtype):
+    from keep_b200.low_rank import switch_low_rank, switch_low_rank_grads
+
+    x, left, right, indices, base, grad = make(cuda, rows, 1, 3, 136, 72, rank, dtype=dtype, base=dtype, seed=rank)
+    x[::3, 5], grad[1::4, 0, 9] = float("inf"), float("-inf")
+    left[:, ::2], right[:, :, ::2] = left[:, ::2].abs(), right[:, :, ::2].abs()
+    right[:, :, 5], left[:, 9] = right[:, :, 5].abs(), left[:, 9].abs()
+    want = ref.low_rank(x, left, right, indices, base, 0.5)
+    assert torch.isinf(want[0]).any()
+    same_infinities(switch_low_rank(x, left, right, indices, base=base, scale=0.5), want)
+    same_infinities(switch_low_rank_grads(grad, x, left, right, indices, weight_grad=False)[0], ref.low_rank_grads(grad, x, left, right, indices, 1.0)[0])
