@@ -527,6 +527,54 @@ struct FactorGradArgs {
   uint16_t* out;
 };
 
+// The gradients of a warp's 32 columns and RH ranks that have no value, once more from the high parts alone: an infinity times a
+// low part (zero, or of the other sign) undoes what it makes of the high one, which is the definition's.  Plain sums, four ranks
+// at a time, up to where none of them can have a value any more; a call whose inputs are finite never comes here.
+template <typename T, int RP, bool LEFT>
+__device__ __noinline__ void factor_grad_undefined(const FactorGradArgs& a, int set, int64_t col0, int j0, int ranks) {
+  const int64_t col = col0 + (threadIdx.x & 31);
+  const bool mine = col < a.width;
+  const int start = a.plan.offset[set], size = a.plan.count[set];
+  T* out = reinterpret_cast<T*>(a.out) + static_cast<int64_t>(set) * a.rank * a.width + (LEFT ? col * a.rank : col);
+  const T* in = reinterpret_cast<const T*>(a.in) + (mine ? col : 0);
+  for (int j = j0; j < a.rank && j < j0 + ranks; j += 4) {
+    bool undefined[4], some = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) some |= undefined[i] = mine && isnan(static_cast<float>(out[(j + i) * (LEFT ? 1 : a.width)]));
+    if (!__any_sync(0xFFFFFFFFu, some)) continue;
+    float sum[4] = {};
+    for (int block = 0; block < size; block += 16) {
+      const int place = a.plan.order[start + block + (threadIdx.x & 15)];
+      const uint4* inner = reinterpret_cast<const uint4*>(a.inner.high + (static_cast<int64_t>((start + block) / 16) * RP + j) * 16);
+      float x[16];
+      uint4 parts[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) parts[i] = __ldg(inner + i);
+#pragma unroll
+      for (int p = 0; p < 16; ++p) {
+        const int route = __shfl_sync(0xFFFFFFFFu, place, p);
+        x[p] = static_cast<float>(in[static_cast<int64_t>(max(route, 0) / a.in_div) * a.in_ld]);
+        if (route < 0) x[p] = 0.0f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {  // (the order of Inner: places 2 (w / 2) + 8 (w % 2) and the next)
+          const uint32_t two = word(parts[2 * i + w / 4], w % 4);
+          const int p = w / 2 * 2 + w % 2 * 8;
+          sum[i] = fmaf(__uint_as_float(two & 0xFFFF0000u), x[p + 1], fmaf(__uint_as_float(two << 16), x[p], sum[i]));
+        }
+      bool open = false;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) open |= undefined[i] && !isnan(sum[i]);
+      if (!__any_sync(0xFFFFFFFFu, open)) break;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (undefined[i]) out[(j + i) * (LEFT ? 1 : a.width)] = static_cast<T>(a.scale * sum[i]);
+  }
+}
+
 // A warp has 32 columns of x (or grad) and RH ranks, and walks the set's rows 16 at a time; the warps that share
 // them add their sums up in shared memory in their order.
 //   right: D[rank][column] = inner^T rows       left: D[column][rank] = rows^T inner
@@ -631,6 +679,9 @@ __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, in
 #pragma unroll
       for (int i = 0; i < SUMS; ++i) acc[i / 4][i % 4] += sm[((warp + p) * SUMS + i) * 32 + lane];
   }
+  float any = 0.0f;
+#pragma unroll
+  for (int i = 0; i < SUMS; ++i) any += acc[i / 4][i % 4];
   if (!LEFT) {
 #pragma unroll
     for (int m = 0; m < RH / 16; ++m)
@@ -660,10 +711,14 @@ __device__ __forceinline__ void factor_grad(const FactorGradArgs& a, int set, in
           if (j + 2 * w < a.rank) *reinterpret_cast<uint2*>(row + j + 2 * w) = make_uint2(packed[w], packed[w + 1]);
       }
   }
+  if (__any_sync(0xFFFFFFFFu, isnan(any))) {
+    __syncwarp();  // (values that other lanes stored)
+    factor_grad_undefined<T, RP, LEFT>(a, set, col0, j0, RH);
+  }
 }
 
 template <typename T, int RP>
-__global__ void __launch_bounds__(LR_THREADS) factor_grad_kernel(FactorGradArgs right, FactorGradArgs left, int right_slabs) {
+__global__ void __launch_bounds__(LR_THREADS) factor_grad_kernel(const __grid_constant__ FactorGradArgs right, const __grid_constant__ FactorGradArgs left, int right_slabs) {
   extern __shared__ __align__(16) float sm[];
   const int slab = blockIdx.x;
   if (slab < right_slabs) factor_grad<T, RP, false>(right, blockIdx.y, slab, blockIdx.z, sm);

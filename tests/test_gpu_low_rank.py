@@ -379,3 +379,24 @@ def test_ranks_that_fill_up_a_multiple_of_eight_stay_out_of_rows_that_are_not_fi
     assert torch.isinf(want[0]).any()
     same_infinities(switch_low_rank(x, left, right, indices, base=base, scale=0.5), want)
     same_infinities(switch_low_rank_grads(grad, x, left, right, indices, weight_grad=False)[0], ref.low_rank_grads(grad, x, left, right, indices, 1.0)[0])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("rows,sets,inp,out,rank", [(24, 2, 128, 72, 8), (70, 3, 264, 136, 40), (300, 2, 136, 200, 16), (180, 4, 136, 72, 100), (900, 3, 264, 100, 64), (600, 1, 72, 520, 128)])
+def test_an_infinity_of_a_row_is_one_of_the_factors_gradients(cuda, rows, sets, inp, out, rank, dtype):
+    """Inner vectors and, for fp16, the rows enter these products in two parts; so does what meets an infinity."""
+    from keep_b200.low_rank import switch_low_rank_grads
+
+    x, left, right, indices, _, grad = make(cuda, rows, 1, sets, inp, out, rank, dtype=dtype, seed=rank)
+    indices[:sets, 0] = torch.arange(sets, device=cuda)
+    inf = float("inf")
+    for of_x, of_grad in (([(0, 5, inf)], []), ([], [(0, 9, -inf)]), ([(0, 5, inf), (sets, 5, -inf), (sets + 1, 7, inf)], []), ([(0, 5, inf)], [(sets - 1, 9, inf), (sets + 2, 9, -inf)])):
+        a, g = x.clone(), grad.clone()
+        for r, c, v in of_x:
+            a[r, c] = v
+        for r, c, v in of_grad:
+            g[r, 0, c] = v
+        got, want = switch_low_rank_grads(g, a, left, right, indices, scale=0.5), ref.low_rank_grads(g, a, left, right, indices, 0.5)
+        assert torch.isinf(want[1][0]).any() or torch.isinf(want[2][0]).any()
+        same_infinities(got[1], want[1])
+        same_infinities(got[2], want[2])
