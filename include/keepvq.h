@@ -490,6 +490,13 @@ typedef struct keepvq_switch_matmul_args {
 int64_t keepvq_switch_matmul_workspace_bytes(int64_t routes, int64_t experts, int64_t out_dim, int64_t in_dim, int32_t x_div, int32_t grads);
 int keepvq_switch_matmul(const keepvq_switch_matmul_args* args, void* stream);
 int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stream);
+/* *word (device memory) = 1 if a bounded wait of any such call on this device expired since this was last asked, else 0;
+ * a call on another stream counts once it has finished.  For callers that do not keep their workspaces. */
+int keepvq_switch_matmul_wait_expired(int32_t* word, void* stream);
+/* Self-test of these waits: a call (grads 0: keepvq_switch_matmul, else keepvq_switch_matmul_grads) whose loaders of
+ * routes leave after their first tile, and whose waits run out after wait_ns (at most a second).  The other warps give up,
+ * the status words become 1, every block waits for its copies and returns, and the outputs are invalid. */
+int keepvq_switch_matmul_wait_selftest(const keepvq_switch_matmul_args* args, int32_t grads, int64_t wait_ns, void* stream);
 
 /* ------------------------------------------------------------------------------------------
  * Low-rank products chosen per route, added onto a base, and their gradients: adapters of many

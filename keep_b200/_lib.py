@@ -197,6 +197,8 @@ _SIGNATURES = {
     "keepvq_switch_matmul_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int32, c_int32]),
     "keepvq_switch_matmul": (c_int, [POINTER(SwitchMatmulArgs), c_void_p]),
     "keepvq_switch_matmul_grads": (c_int, [POINTER(SwitchMatmulArgs), c_void_p]),
+    "keepvq_switch_matmul_wait_expired": (c_int, [c_void_p, c_void_p]),
+    "keepvq_switch_matmul_wait_selftest": (c_int, [POINTER(SwitchMatmulArgs), c_int32, c_int64, c_void_p]),
     "keepvq_switch_low_rank_workspace_bytes": (c_int64, [c_int64, c_int64, c_int64, c_int64, c_int64, c_int32, c_int32]),
     "keepvq_switch_low_rank": (c_int, [POINTER(SwitchLowRankArgs), c_void_p]),
     "keepvq_switch_low_rank_grads": (c_int, [POINTER(SwitchLowRankArgs), c_void_p]),

@@ -148,15 +148,19 @@ __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, bool mn_major) {
   return static_cast<uint64_t>((addr & 0x3FFFFu) >> 4) | (lead << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
-// Wait of a whole warp, bounded by time: false after MM_WAIT_NS in this wait (a call as a whole may take longer), or when
+// Of this device: 1 since a wait of any call ran out, until asked for (keepvq_switch_matmul_wait_expired).  A call's own status word
+// lies in its workspace, which a caller need not keep.
+__device__ int32_t some_wait_expired;
+
+// Wait of a whole warp, bounded by time: false after wait_ns in this wait (a call as a whole may take longer), or when
 // another warp gave up.
-__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag) {
+__device__ __forceinline__ bool wait_for(uint32_t bar, uint32_t parity, volatile int* abort_flag, uint64_t wait_ns) {
   uint64_t deadline = 0;
   for (uint32_t spin = 0;; ++spin) {
     if (__all_sync(0xFFFFFFFFu, mbar_complete(bar, parity))) return true;
     if ((spin & 31u) == 31u) {
       if (__any_sync(0xFFFFFFFFu, *abort_flag)) return false;
-      if (!deadline) deadline = global_timer_ns() + MM_WAIT_NS;
+      if (!deadline) deadline = global_timer_ns() + wait_ns;
       else if (__any_sync(0xFFFFFFFFu, global_timer_ns() > deadline)) { *abort_flag = 1; return false; }
     }
   }
@@ -187,6 +191,8 @@ struct MatmulArgs {
   void* out;        // result rows
   float* route_dx;  // dx before the pick sum, or null
   Plan plan;
+  uint64_t wait_ns;  // limit of one wait
+  int stall;         // the self-test's: the loader of the N operand leaves after its first tile
 };
 
 __device__ __forceinline__ uint32_t round_pair(uint32_t x, uint32_t y, bool bf16) {
@@ -277,6 +283,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     Ring<STAGES> r;
     const uint32_t tile = ring + (warp == WARP_N ? S::A_BYTES : 0);
     const CUtensorMap* map = warp == WARP_M ? &m_map : &n_map;
+    int left = a.stall && warp == WARP_N ? 1 : -1;  // tiles until this loader leaves; -1: it does not
     for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       const int half = it.n_pad / CTAS;  // of the N operand, in this CTA
@@ -287,8 +294,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
         rows = make_int4(row_at(q), row_at(q + 1), row_at(q + 2), row_at(q + 3));
       }
       for (int kb = 0; kb < it.k_blocks; ++kb) {
-        ok = wait_for(empty + 8 * r.index, r.phase ^ 1u, aborted);
+        ok = left != 0 && wait_for(empty + 8 * r.index, r.phase ^ 1u, aborted, a.wait_ns);
         if (!ok) break;
+        if (left > 0) --left;
         const uint32_t bar = full0 + 8 * r.index, dst = tile + r.index * S::STAGE_BYTES;
         if (!MANY && warp == WARP_N) {
           if (lane == 0) expect_bytes<MANY>(bar, static_cast<uint32_t>((it.size + 3) / 4 * 512));
@@ -324,10 +332,10 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks == 0) continue;  // (an expert without routes: the epilogue writes zeros)
-      ok = wait_for(acc_empty + 8 * acc.index, acc.phase ^ 1u, aborted);
+      ok = wait_for(acc_empty + 8 * acc.index, acc.phase ^ 1u, aborted, a.wait_ns);
       const uint32_t idesc = idesc0 | (static_cast<uint32_t>(it.n_pad >> 3) << 17);
       for (int kb = 0; kb < it.k_blocks && ok; ++kb) {
-        ok = wait_for(full + 8 * r.index, r.phase, aborted);
+        ok = wait_for(full + 8 * r.index, r.phase, aborted, a.wait_ns);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         const int steps = MODE == WEIGHT_GRAD ? min(4, (it.size - kb * K_BLOCK + ROW_STEP - 1) / ROW_STEP) : 4;  // of 16
@@ -369,7 +377,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
     for (int i = first_item; i < items && ok; i += item_step) {
       const Item it = item_at(i);
       if (it.k_blocks > 0) {
-        ok = wait_for(acc_full + 8 * acc.index, acc.phase, aborted);
+        ok = wait_for(acc_full + 8 * acc.index, acc.phase, aborted, a.wait_ns);
         if (!ok) break;
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
       }
@@ -470,7 +478,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) switch_matmul_kernel(MatmulArgs
   __syncthreads();  // every role has left its loop
   if (*aborted) {
     // What is in flight is waited for, bounded: the issuer's products by one more commit, copies by time.
-    if (tid == 0) atomicExch(a.plan.status, 1);
+    if (tid == 0) { atomicExch(a.plan.status, 1); atomicExch(&some_wait_expired, 1); }
     const uint64_t grace = global_timer_ns() + 20000000ull;
     if (warp == WARP_MMA && mma_issued && elect_one()) mma_commit<MANY>(acc_full);
     while (global_timer_ns() < grace) __nanosleep(1000);
@@ -509,6 +517,10 @@ static int value_map(CUtensorMap* map, const void* base, int dtype, int64_t widt
 // FEW / MANY: 8 routes each 169 / 185 us, 16 each 174 / 188, 24 each 206 / 192, 32 each 238 / 196); MANY wants tiles enough for its pairs.
 static bool many_routes(int64_t routes, int64_t experts) { return routes > 16 * experts && routes >= 256; }
 
+struct Waits {
+  uint64_t ns = MM_WAIT_NS;
+  int stall = 0;
+};
 struct Layout {
   Plan plan;
   uint16_t *x, *grad;  // rows in the plan's order (MANY)
@@ -538,9 +550,9 @@ static int check_sizes(int64_t routes, int64_t experts, int64_t out_dim, int64_t
 }
 
 template <int MODE, bool MANY>
-static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, cudaStream_t s) {
+static int launch_tiles(const keepvq_switch_matmul_args& a, const Layout& l, const Waits& waits, cudaStream_t s) {
   using S = Shape<MANY>;
-  MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan};
+  MatmulArgs m{a.x_div, static_cast<int>(a.experts), a.dtype, a.out_dim, a.in_dim, MODE == FORWARD ? a.out : MODE == INPUT_GRAD ? a.dx : a.dweight, l.route_dx, l.plan, waits.ns, waits.stall};
   const int64_t places = max_places(a.routes, a.experts), grad_ld = MANY ? align_up(a.out_dim, 8) : a.grad_ld;
   CUtensorMap m_map, n_map, out_map;
   int rc = MODE == WEIGHT_GRAD ? value_map(&m_map, l.x, a.dtype, a.in_dim, a.in_dim, places, 1, K_BLOCK)
@@ -594,6 +606,43 @@ static int check_call(const keepvq_switch_matmul_args& a, bool grads) {
   return KEEPVQ_OK;
 }
 
+static int forward_call(const keepvq_switch_matmul_args& a, const Waits& waits, cudaStream_t s) {
+  if (const int rc = check_call(a, false)) return rc;
+  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.out_dim, a.in_dim, a.x_div, false);
+  if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
+  if (a.routes == 0) return KEEPVQ_OK;
+  const bool many = many_routes(a.routes, a.experts);
+  if (const int rc = make_plan({a.indices, a.index_bits}, a.routes, a.experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX, many ? Shape<true>::PAD : N_STEP, l.plan, s)) return rc;
+  if (!many) return launch_tiles<FORWARD, false>(a, l, waits, s);
+  const RowCopy x{a.x, l.x, a.in_dim, a.in_dim, a.x_div};
+  if (const int rc = copy_rows(&x, 1, a.routes, a.experts, l.plan, s)) return rc;
+  return launch_tiles<FORWARD, true>(a, l, waits, s);
+}
+
+static int grads_call(const keepvq_switch_matmul_args& a, const Waits& waits, cudaStream_t s) {
+  if (const int rc = check_call(a, true)) return rc;
+  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.out_dim, a.in_dim, a.x_div, true);
+  if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
+  if (a.routes == 0) {
+    const cudaError_t e = a.dweight ? cudaMemsetAsync(a.dweight, 0, a.experts * a.out_dim * a.in_dim * 2, s) : cudaSuccess;
+    return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
+  }
+  const Indices indices{a.indices, a.index_bits};
+  const bool many = many_routes(a.routes, a.experts);
+  if (const int rc = make_plan(indices, a.routes, a.experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX, many ? Shape<true>::PAD : N_STEP, l.plan, s)) return rc;
+  const RowCopy copies[2] = {{a.grad, l.grad, a.grad_ld, align_up(a.out_dim, 8), 1}, {a.x, l.x, a.in_dim, a.in_dim, a.x_div}};
+  if (many || a.dweight)
+    if (const int rc = copy_rows(copies, a.dweight ? 2 : 1, a.routes, a.experts, l.plan, s)) return rc;
+  if (a.dx) {
+    if (const int rc = many ? launch_tiles<INPUT_GRAD, true>(a, l, waits, s) : launch_tiles<INPUT_GRAD, false>(a, l, waits, s)) return rc;
+    if (l.route_dx)
+      if (const int rc = sum_picks(l.route_dx, indices, a.experts, a.routes / a.x_div, a.x_div, a.in_dim, a.dx, a.dtype, s)) return rc;
+  }
+  return a.dweight ? launch_tiles<WEIGHT_GRAD, true>(a, l, waits, s) : KEEPVQ_OK;
+}
+
+__global__ void take_wait_expired(int32_t* word) { *word = atomicExch(&some_wait_expired, 0); }
+
 }  // namespace dense
 }  // namespace keepvq
 
@@ -606,46 +655,27 @@ int64_t keepvq_switch_matmul_workspace_bytes(int64_t routes, int64_t experts, in
 }
 
 int keepvq_switch_matmul(const keepvq_switch_matmul_args* args, void* stream) {
-  using namespace keepvq::dense;
-  if (!args) return KEEPVQ_ERR_NULL;
-  const keepvq_switch_matmul_args& a = *args;
-  if (const int rc = check_call(a, false)) return rc;
-  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.out_dim, a.in_dim, a.x_div, false);
-  if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
-  if (a.routes == 0) return KEEPVQ_OK;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const bool many = many_routes(a.routes, a.experts);
-  if (const int rc = make_plan({a.indices, a.index_bits}, a.routes, a.experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX, many ? Shape<true>::PAD : N_STEP, l.plan, s)) return rc;
-  if (!many) return launch_tiles<FORWARD, false>(a, l, s);
-  const RowCopy x{a.x, l.x, a.in_dim, a.in_dim, a.x_div};
-  if (const int rc = copy_rows(&x, 1, a.routes, a.experts, l.plan, s)) return rc;
-  return launch_tiles<FORWARD, true>(a, l, s);
+  return args ? keepvq::dense::forward_call(*args, {}, static_cast<cudaStream_t>(stream)) : KEEPVQ_ERR_NULL;
 }
 
 int keepvq_switch_matmul_grads(const keepvq_switch_matmul_args* args, void* stream) {
+  return args ? keepvq::dense::grads_call(*args, {}, static_cast<cudaStream_t>(stream)) : KEEPVQ_ERR_NULL;
+}
+
+int keepvq_switch_matmul_wait_expired(int32_t* word, void* stream) {
+  if (!word) return KEEPVQ_ERR_NULL;
+  if (!keepvq::aligned_to(word, 4)) return KEEPVQ_ERR_ALIGN;
+  keepvq::dense::take_wait_expired<<<1, 1, 0, static_cast<cudaStream_t>(stream)>>>(word);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? KEEPVQ_OK : keepvq::note_cuda_error(e);
+}
+
+int keepvq_switch_matmul_wait_selftest(const keepvq_switch_matmul_args* args, int32_t grads, int64_t wait_ns, void* stream) {
   using namespace keepvq::dense;
   if (!args) return KEEPVQ_ERR_NULL;
-  const keepvq_switch_matmul_args& a = *args;
-  if (const int rc = check_call(a, true)) return rc;
-  const Layout l = lay_out(a.workspace, a.routes, a.experts, a.out_dim, a.in_dim, a.x_div, true);
-  if (l.bytes > a.workspace_bytes) return KEEPVQ_ERR_CAPACITY;
-  cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (a.routes == 0) {
-    const cudaError_t e = a.dweight ? cudaMemsetAsync(a.dweight, 0, a.experts * a.out_dim * a.in_dim * 2, s) : cudaSuccess;
-    return e == cudaSuccess ? KEEPVQ_OK : keepvq::note_cuda_error(e);
-  }
-  const Indices indices{a.indices, a.index_bits};
-  const bool many = many_routes(a.routes, a.experts);
-  if (const int rc = make_plan(indices, a.routes, a.experts, many ? Shape<true>::N_MAX : Shape<false>::N_MAX, many ? Shape<true>::PAD : N_STEP, l.plan, s)) return rc;
-  const RowCopy copies[2] = {{a.grad, l.grad, a.grad_ld, align_up(a.out_dim, 8), 1}, {a.x, l.x, a.in_dim, a.in_dim, a.x_div}};
-  if (many || a.dweight)
-    if (const int rc = copy_rows(copies, a.dweight ? 2 : 1, a.routes, a.experts, l.plan, s)) return rc;
-  if (a.dx) {
-    if (const int rc = many ? launch_tiles<INPUT_GRAD, true>(a, l, s) : launch_tiles<INPUT_GRAD, false>(a, l, s)) return rc;
-    if (l.route_dx)
-      if (const int rc = sum_picks(l.route_dx, indices, a.experts, a.routes / a.x_div, a.x_div, a.in_dim, a.dx, a.dtype, s)) return rc;
-  }
-  return a.dweight ? launch_tiles<WEIGHT_GRAD, true>(a, l, s) : KEEPVQ_OK;
+  if (wait_ns <= 0 || wait_ns > 1000000000ll) return KEEPVQ_ERR_SHAPE;
+  const Waits waits{static_cast<uint64_t>(wait_ns), 1};
+  return grads ? grads_call(*args, waits, static_cast<cudaStream_t>(stream)) : forward_call(*args, waits, static_cast<cudaStream_t>(stream));
 }
 
 }  // extern "C"

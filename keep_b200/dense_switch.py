@@ -15,6 +15,8 @@ an order that depends on the call alone: the same call gives the same bits.
 ``switch_matmul`` records a gradient formula where grad mode is on and an input requires one.  A CUDA graph
 captures ``switch_matmul`` under ``torch.no_grad()`` and ``switch_matmul_grads``, not a recorded backward
 pass: autograd would tie the capture to the streams of whatever other graphs of the same leaves are alive.
+The kernels' waits are bounded: ``switch_matmul_wait_expired`` tells whether one gave up (on a device that has stopped making
+progress), after which the outputs since the last time of asking are not to be used.
 There are no derivatives of gradients and no forward-mode ones: arguments that carry a tangent are refused.
 """
 
@@ -28,7 +30,7 @@ from torch.autograd import forward_ad
 from . import _lib
 from .vq import as_device
 
-__all__ = ["switch_matmul", "switch_matmul_grads"]
+__all__ = ["switch_matmul", "switch_matmul_grads", "switch_matmul_wait_expired"]
 
 _DTYPES = (torch.float16, torch.bfloat16)
 
@@ -177,3 +179,18 @@ def switch_matmul(x: torch.Tensor, weight: torch.Tensor, indices) -> torch.Tenso
         _no_capture("switch_matmul", "switch_matmul_grads")
         return _SwitchMatmul.apply(x, weight, as_device(indices, x.device))
     return _forward(x, weight, indices)
+
+
+def switch_matmul_wait_expired(device=None) -> bool:
+    """True when a bounded wait (2 s) expired in a call of ``switch_matmul`` or its gradients on ``device`` (the current one)
+    since this was last asked: outputs of such calls are invalid.  Reads one word back: synchronises the current
+    stream; calls on other streams count once they have finished."""
+    device = torch.device("cuda" if device is None else device)
+    if device.type != "cuda":
+        raise _lib.KeepVQError("keep_b200 operators need a CUDA device; there is no CPU path")
+    with _lib.on_device(torch.device("cuda", torch.cuda.current_device() if device.index is None else device.index)):
+        if torch.cuda.is_current_stream_capturing():
+            raise _lib.KeepVQError("switch_matmul_wait_expired: a word cannot be read back inside a graph capture")
+        word = torch.empty(1, dtype=torch.int32, device="cuda")
+        _lib.check(_lib.load().keepvq_switch_matmul_wait_expired(_lib.ptr(word), _lib.stream_handle(word.device)), "keepvq_switch_matmul_wait_expired")
+    return bool(word.item())

@@ -245,3 +245,18 @@ def test_ranks_beyond_the_factors_are_refused(ranks):
     assert lib.keepvq_switch_low_rank_padded(low_rank_args(), ranks, None) == SHAPE
     assert lib.keepvq_switch_low_rank_grads_padded(low_rank_args(), ranks, None) == SHAPE
     assert lib.keepvq_switch_low_rank_padded(low_rank_args(routes=0), 5, None) == 0
+
+
+def test_the_wait_entry_points_refuse():
+    from keep_b200.dense_switch import switch_matmul_wait_expired
+
+    lib = _lib.load()
+    assert lib.keepvq_switch_matmul_wait_expired(None, None) == NULL
+    assert lib.keepvq_switch_matmul_wait_expired(258, None) == ALIGN
+    assert lib.keepvq_switch_matmul_wait_selftest(None, 0, 1000, None) == NULL
+    for grads in (0, 1):
+        for limit in (0, -1, 1_000_000_001):
+            assert lib.keepvq_switch_matmul_wait_selftest(matmul_args(), grads, limit, None) == SHAPE
+        assert lib.keepvq_switch_matmul_wait_selftest(matmul_args(weight=264), grads, 1000, None) == ALIGN
+    with pytest.raises(_lib.KeepVQError, match="no CPU path"):
+        switch_matmul_wait_expired("cpu")

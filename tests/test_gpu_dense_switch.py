@@ -304,3 +304,40 @@ def test_weight_gradients_whose_last_columns_fill_no_tile(cuda, inp, out, expert
         want = ref.matmul_grads(grad, x, weight, indices)[1]
         for got in [switch_matmul_grads(grad, x, weight, indices, x_grad=False)[1] for _ in range(20)]:
             ref.close(got, want)
+
+
+@pytest.mark.parametrize("size", [(9, 2, 4, 256, 136), (700, 2, 3, 320, 520)])
+def test_a_wait_that_runs_out_is_reported(cuda, size):
+    """A call whose loaders of routes leave after their first tile: every other warp's wait runs into its limit of 2 ms, the blocks
+    return, the device says so once, and the next calls are what they always are.  Both forms of the kernel, both directions."""
+    import time
+
+    from keep_b200 import _lib
+    from keep_b200.dense_switch import switch_matmul, switch_matmul_grads, switch_matmul_wait_expired
+
+    x, weight, indices, grad = make(cuda, *size)
+    tokens, k, experts, inp, out = size
+    want = (switch_matmul(x, weight, indices), *switch_matmul_grads(grad, x, weight, indices))
+    assert not switch_matmul_wait_expired() and not switch_matmul_wait_expired(cuda)
+    lib = _lib.load()
+    result, dx, dweight = torch.empty_like(grad), torch.empty_like(x), torch.empty_like(weight)
+    for grads in (0, 1):
+        nbytes = int(lib.keepvq_switch_matmul_workspace_bytes(tokens * k, experts, out, inp, k, grads))
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=cuda)
+        args = _lib.SwitchMatmulArgs(x=x.data_ptr(), weight=weight.data_ptr(), grad=grad.data_ptr(), dtype=_lib.dtype_tag(BF16), indices=indices.data_ptr(), index_bits=32, x_div=k,
+                                     routes=tokens * k, experts=experts, out_dim=out, in_dim=inp, grad_ld=out, out=result.data_ptr(), dx=dx.data_ptr(),
+                                     dweight=dweight.data_ptr(), workspace=ws.data_ptr(), workspace_bytes=nbytes)
+        start = time.monotonic()
+        _lib.check(lib.keepvq_switch_matmul_wait_selftest(args, grads, 2_000_000, _lib.stream_handle(cuda)), "keepvq_switch_matmul_wait_selftest")
+        assert switch_matmul_wait_expired()
+        assert time.monotonic() - start < 1.0
+        assert int(ws[:4].view(torch.int32).item()) == 1
+        assert not switch_matmul_wait_expired()  # told once
+    for _ in range(3):
+        again = (switch_matmul(x, weight, indices), *switch_matmul_grads(grad, x, weight, indices))
+        assert all(torch.equal(a, b) for a, b in zip(again, want))
+    assert not switch_matmul_wait_expired()
+    with torch.cuda.graph(torch.cuda.CUDAGraph()):
+        switch_matmul(x, weight, indices)
+        with pytest.raises(_lib.KeepVQError, match="inside a graph capture"):
+            switch_matmul_wait_expired()
