@@ -773,7 +773,7 @@ static int launch_low_rank_kernel(void (*kernel)(LowRankArgs), int bytes, uint64
     attribute.val.programmaticStreamSerializationAllowed = 1;
   }
   config.attrs = &attribute;
-  config.numAttrs = 1;
+  config.numAttrs = p.ctas > 1 || p.tiles <= EARLY_LAUNCH_MAX_BLOCKS ? 1 : 0;  // (common.cuh; 20,000 rows of 1024: 1 to 2 us of 48 for it)
   const cudaError_t e = cudaLaunchKernelEx(&config, kernel, a);
   return e == cudaSuccess ? KEEPVQ_OK : note_cuda_error(e);
 }
