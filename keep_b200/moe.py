@@ -61,6 +61,9 @@ class SharedExpert:
     Requests may bring low-rank adapters: ``shared(x, adapters={"w1": ..., "w3": ..., "w2": ...},
     adapter_indices=indices)`` adds those of ``low_rank.LowRank`` stacks to the products (in fp32, before
     anything is rounded), row by row: ``indices[t]`` is the adapter of token ``t``, -1 for none.
+    Autograd records the adapters' own products where their factors require a gradient: those of ``w2`` can be
+    trained.  The expert's library products have no derivative, so a backward pass that would have to go through
+    one (to ``w1``, ``w3`` or ``x``) fails.
     """
 
     def __init__(self, w1: torch.Tensor, w3: torch.Tensor, w2: torch.Tensor, *, swiglu_limit: float = 0.0):

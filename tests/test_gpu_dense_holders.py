@@ -247,3 +247,23 @@ def test_custom_ops_refuse_forward_mode_differentiation(cuda):
         with torch.autograd.forward_ad.dual_level(), pytest.raises(_lib.KeepVQError, match="no forward-mode derivative"):
             call(torch.autograd.forward_ad.make_dual(x, x))
         call(x)
+
+
+def test_gradients_of_adapters_beside_the_shared_expert(cuda):
+    """Those of w2 are its correction's; what would have to pass the library product fails instead of being left out."""
+    from keep_b200.low_rank import LowRank, switch_low_rank_grads
+    from keep_b200.moe import SharedExpert
+
+    gen = torch.Generator(device=cuda).manual_seed(10)
+    shared, x = SharedExpert(rand(gen, 264, 512, scale=1 / 22), rand(gen, 264, 512, scale=1 / 22), rand(gen, 512, 264, scale=1 / 16)), rand(gen, 33, 512)
+    indices = torch.randint(-1, 4, (33,), generator=gen, device=cuda)
+    low = {"w1": pair(gen, 4, 264, 512, 8), "w2": pair(gen, 4, 512, 264, 8)}
+    leaves = {n: LowRank(p.left.clone().requires_grad_(), p.right.clone().requires_grad_(), p.scale) for n, p in low.items()}
+    grad = rand(gen, 33, 512)
+    shared(x, adapters={"w2": leaves["w2"]}, adapter_indices=indices).backward(grad.float())
+    gate, up = torch.mm(x, shared.gate_up, out_dtype=torch.float32).split(264, dim=1)
+    h = (torch.nn.functional.silu(gate) * up).to(BF16)
+    want = switch_low_rank_grads(grad, h, low["w2"].left, low["w2"].right, indices, scale=0.5, x_grad=False)
+    assert torch.equal(leaves["w2"].left.grad, want[1]) and torch.equal(leaves["w2"].right.grad, want[2])
+    with pytest.raises(RuntimeError, match="not implemented"):
+        shared(x, adapters=leaves, adapter_indices=indices).backward(grad.float())
