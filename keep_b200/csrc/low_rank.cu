@@ -15,13 +15,15 @@
 // the inner vectors never leave the SMs, and one row of one set still has a whole cluster's loads in
 // flight.  Forward: A, then B.  Input gradient: B^T, then A^T, whose fragments are transposed in registers.
 //
-// Measured on a B200, 4096 -> 4096, bf16: one row of rank 16 6 us on the device, 61 rows of rank 32 11 us cold; 251 tokens with
-// six of 384 corrections of rank 8 20 us; 4096 rows of rank 16 / 64 / 128 35 / 47 / 82 us with the plan, where x, base and
-// results are 100 MB.  What bounds it then is instructions and latency per 16 rows, not bytes.  Tiles of 64 rows shared
+// Measured on a B200, 4096 -> 4096, bf16: one row of rank 16 5 us on the device, 61 rows of rank 32 10 us; 251 tokens with
+// six of 384 corrections of rank 8 20 us; 4096 rows of rank 16 / 64 / 128 31 / 45 / 85 us with the plan (56 / 69 / 124 with an
+// fp32 base), where x, base and results are 100 MB.  What bounds it then is instructions and latency per 16 rows, not bytes.  Tiles of 64 rows shared
 // by the warps through ldmatrix were slower at every rank from 32 on (4096 rows of rank 64: 67 us).
 //
 // Inner vectors are fp32 sums; for the second product each is split into the sum of two 16-bit values, scaled
-// by a power of two per row for fp16 so that neither its range nor its small values are lost.
+// by a power of two per row for fp16 so that neither its range nor its small values are lost.  The low parts' sums are kept apart
+// and made finite, so that an infinity of a factor comes through as the high parts have it (rank 16 and 32: no time; 64: 3 %
+// forward and 6 % for dx; 128: 9 and 4 %).
 #include "switch_plan.cuh"
 
 namespace keepvq {
@@ -966,7 +968,7 @@ int keepvq_switch_low_rank_grads_padded(const keepvq_switch_low_rank_args* args,
     if (const int rc = sum_picks(l.route_dx, k.indices, a.sets, a.routes / a.x_div, a.x_div, a.in_dim, a.dx, a.dtype, s)) return rc;
   if (!weights) return KEEPVQ_OK;
   const int64_t mean = a.routes / (a.routes < a.sets ? a.routes : a.sets);
-  const int row_parts = mean <= 16 ? 1 : mean <= 64 ? 2 : mean <= 256 ? 4 : 8;  // a part keeps four blocks of 16 rows or more
+  const int row_parts = mean <= 16 ? 1 : mean <= 64 ? 2 : mean <= 256 ? 4 : 8;  // a part has one to four blocks of 16 rows, more beyond 512 rows
   FactorGradArgs right{static_cast<const uint16_t*>(a.x), a.in_dim, a.x_div, a.dright ? a.in_dim : 0, static_cast<int>(a.rank), row_parts, 1.0f, l.plan, l.back, static_cast<uint16_t*>(a.dright)};
   FactorGradArgs left{static_cast<const uint16_t*>(a.grad), a.grad_ld, 1, a.dleft ? a.out_dim : 0, static_cast<int>(a.rank), row_parts, a.scale, l.plan, l.inner, static_cast<uint16_t*>(a.dleft)};
   return a.dtype == KEEPVQ_BF16 ? launch_factor_grads_of<__nv_bfloat16>(p.rp, right, left, a.sets, s) : launch_factor_grads_of<__half>(p.rp, right, left, a.sets, s);

@@ -9,7 +9,8 @@ Layouts, indices and the rules for captures and derivatives are those of ``dense
 adapter) leaves its base as it is.  ``left`` is ``[sets, out, rank]``, ``right`` ``[sets, rank, in]``, both in x's
 dtype (fp16 or bf16), rank 1 to 128: ranks that are not a multiple of 8 are padded on every call, so a caller
 who keeps such adapters pads them once instead.  ``base`` has x's dtype or is fp32, and so has the result;
-what flows back through an fp32 result reaches ``base`` as it is and the products rounded to x's dtype.
+what flows back through an fp32 result reaches ``base`` as it is and the products rounded to x's dtype (for fp16:
+infinite beyond its range, zero below it, as any gradient in that type).
 Inner vectors are fp32 sums and enter the second product with 16 bits each (bf16), or with 22 bits of a row's
 largest (fp16: their range does not matter).
 """
