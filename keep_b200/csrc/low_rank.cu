@@ -15,7 +15,7 @@
 // the inner vectors never leave the SMs, and one row of one set still has a whole cluster's loads in
 // flight.  Forward: A, then B.  Input gradient: B^T, then A^T, whose fragments are transposed in registers.
 //
-// Measured on a B200, 4096 -> 4096, bf16: one row of rank 16 5 us on the device, 61 rows of rank 32 10 us; 251 tokens with
+// Measured on a B200, 4096 -> 4096, bf16: one row of rank 16 6 us on the device, 61 rows of rank 32 11 us cold; 251 tokens with
 // six of 384 corrections of rank 8 20 us; 4096 rows of rank 16 / 64 / 128 31 / 45 / 85 us with the plan (56 / 69 / 124 with an
 // fp32 base), where x, base and results are 100 MB.  What bounds it then is instructions and latency per 16 rows, not bytes.  Tiles of 64 rows shared
 // by the warps through ldmatrix were slower at every rank from 32 on (4096 rows of rank 64: 67 us).
